@@ -1,0 +1,491 @@
+"""What the training operators around the decoder's vocabulary are measured on.
+
+Four operators: the token embedding with its gradient, the cross entropy of a linear vocabulary
+projection with its gradients, the norm of many gradients with the scaling that clips them, and the
+AdamW step over many parameters with its state in 32 or in 8 bits.  ``run`` computes a case in plain
+torch operations, or, with ``own`` set, through ``paccmann_generator_amd.ops``.
+
+    listed()            the cases, each with a name
+    draw(rng)           one more case of the same ranges
+    prepare(case, seed) the inputs of a case, on the GPU
+    run(state)          one pass, and its outputs
+    work(case)          the bytes and operations that a pass cannot do without
+    exact(case, seed)   the outputs from the definitions, in 64 bits
+"""
+import math
+
+import torch
+
+own = False
+
+TYPES = {'fp32': torch.float32, 'bf16': torch.bfloat16, 'fp16': torch.float16}
+BLOCK = 256           # values that share one scale of a state held in 8 bits
+IGNORE = -100         # target of a row that has no loss
+HYPER = dict(lr=3e-4, beta1=0.9, beta2=0.98, eps=1e-8, weight_decay=0.01)
+STEPS_BEFORE = 100    # the step counter a case starts from
+MAX_NORM = 1.0
+
+
+# ------------------------------------------------------------------------------------------ cases
+def listed():
+    return [
+        # one decoding step: the rows of 64 sequences' last tokens
+        dict(name='embed_decode', op='embed', train=False, dtype='bf16', n=64, v=128000, e=4096, scale=1.0, pad=-1),
+        # a training batch of a mid-size vocabulary with a padded tail, scaled by sqrt(e)
+        dict(name='embed_train', op='embed', train=True, dtype='bf16', n=32767, v=32000, e=2048, scale=45.25, pad=0),
+        # the decoder's own table (60 tokens of 128) over 4096 sequences of 102 tokens: every row of the
+        # gradient is a sum over thousands of positions
+        dict(name='embed_decoder', op='embed', train=True, dtype='fp32', n=417792, v=60, e=128, scale=1.0, pad=0),
+        # scoring one next token while serving: the whole projection is read for one row
+        dict(name='ce_score_token', op='ce', train=False, dtype='bf16', n=1, v=128000, h=4096, bias=False, weighted=False,
+             ignored=0.0, strided=False),
+        # teacher-forced training of the decoder's projection with rewards, 4096 sequences of 128 tokens
+        dict(name='ce_decoder', op='ce', train=True, dtype='fp32', n=524288, v=60, h=512, bias=True, weighted=True,
+             ignored=0.0, strided=False),
+        # an odd batch over an odd vocabulary, a fifth of the rows without a target
+        dict(name='ce_train_odd', op='ce', train=True, dtype='bf16', n=4095, v=32001, h=2048, bias=True, weighted=False,
+             ignored=0.2, strided=False),
+        # the largest: 8192 tokens over 128000
+        dict(name='ce_train_large', op='ce', train=True, dtype='bf16', n=8192, v=128000, h=4096, bias=False,
+             weighted=False, ignored=0.0, strided=False),
+        # clipping the gradients of the decoder (15 tensors) after a step
+        dict(name='clip_decoder', op='clip', dtype='fp32', layout='decoder', d=512, layers=1, v=60),
+        # clipping those of a model of 468 M parameters
+        dict(name='clip_large', op='clip', dtype='bf16', layout='blocks', d=2048, layers=8, v=32000),
+        # the update of the decoder as the learner makes it: coupled decay, gradients clipped on the way
+        dict(name='adamw_decoder', op='adamw', dtype='fp32', layout='decoder', d=512, layers=1, v=60, bits=32,
+             master=False, decoupled=False, clip=True),
+        # 468 M parameters in bf16 with their 32-bit copies
+        dict(name='adamw_master', op='adamw', dtype='bf16', layout='blocks', d=2048, layers=8, v=32000, bits=32,
+             master=True, decoupled=True, clip=False),
+        # 184 M parameters with the state in 8 bits, its values read back as for a checkpoint
+        dict(name='adamw_8bit', op='adamw', dtype='fp32', layout='blocks', d=1024, layers=12, v=32000, bits=8,
+             master=False, decoupled=True, clip=False),
+    ]
+
+
+def _spread(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    op = rng.choice(['embed', 'ce', 'ce', 'clip', 'adamw'])
+    if op == 'embed':
+        train = rng.random() < 0.7
+        v, e = _spread(rng, 2, 128000), _spread(rng, 8, 4096)
+        most = max(64, min(524288, (1 << 30) // (4 * e)))
+        return dict(op=op, train=train, dtype=rng.choice(['fp32', 'bf16', 'fp16']), n=_spread(rng, 1, most), v=v, e=e,
+                    scale=rng.choice([1.0, 0.5, 11.3]), pad=rng.choice([-1, 0]))
+    if op == 'ce':
+        dtype = rng.choice(['fp32', 'bf16', 'bf16'])
+        train = rng.random() < 0.7
+        v, h = _spread(rng, 2, 128000), _spread(rng, 16, 4096)
+        if rng.random() < 0.7:
+            h = -(-h // 16) * 16
+        most = 8192 * 128000 * 4096 // (64 if dtype == 'fp32' else 2)
+        n = _spread(rng, 1, max(2, min(most // (v * h), 1000000000 // (v + h), 524288)))
+        return dict(op=op, train=train, dtype=dtype, n=n, v=v, h=h, bias=rng.random() < 0.5, weighted=rng.random() < 0.3,
+                    ignored=rng.choice([0.0, 0.1, 0.5]), strided=rng.random() < 0.25)
+    layout = rng.choice(['decoder', 'blocks', 'blocks'])
+    if layout == 'decoder':
+        d, layers, v = rng.choice([128, 256, 512, 1024]), rng.choice([1, 2, 3, 4]), rng.randint(23, 1024)
+    else:
+        d, layers = _spread(rng, 33, 2048), rng.randint(1, 24)
+        layers = max(1, min(layers, 400000000 // (12 * d * d)))
+        v = _spread(rng, 100, 32000)
+    if op == 'clip':
+        return dict(op=op, dtype=rng.choice(['fp32', 'bf16', 'fp16']), layout=layout, d=d, layers=layers, v=v)
+    dtype = rng.choice(['fp32', 'bf16'])
+    return dict(op=op, dtype=dtype, layout=layout, d=d, layers=layers, v=v, bits=rng.choice([32, 8]),
+                master=dtype != 'fp32' and rng.random() < 0.6, decoupled=rng.random() < 0.7, clip=rng.random() < 0.5)
+
+
+def _shapes(case):
+    """The parameter shapes of a case: the StackGRU decoder's (embedding 128, stack width 50, latent 256), or
+    those of a stack of generic blocks of width d with a vocabulary."""
+    d, layers, v = case['d'], case['layers'], case['v']
+    if case['layout'] == 'decoder':
+        got = [(3, d), (3,), (50, d), (50,), (v, 128)]
+        for k in range(layers):
+            got += [(3 * d, 128 + 50 if k == 0 else d), (3 * d, d), (3 * d,), (3 * d,)]
+        return got + [(d, 256), (d,), (v, d), (v,)]
+    got = [(v, d)]
+    for _ in range(layers):
+        got += [(d, d)] * 4 + [(4 * d, d), (d, 4 * d), (d,), (d,)]
+    return got
+
+
+def _numel(case):
+    return sum(math.prod(s) for s in _shapes(case))
+
+
+def _size(case):
+    return 4 if case['dtype'] == 'fp32' else 2
+
+
+def work(case):
+    op, size = case['op'], _size(case)
+    if op == 'embed':
+        n, v, e = case['n'], case['v'], case['e']
+        seen = min(n, v)
+        moved = 8 * n + seen * e * size + n * e * size
+        if case['train']:
+            moved += n * e * size + v * e * size
+        return dict(bytes=moved, flops=n * e * (2 if case['train'] else 1))
+    if op == 'ce':
+        n, v, h = case['n'], case['v'], case['h']
+        moved = (n * h + v * h + (v if case['bias'] else 0)) * size + 12 * n
+        flops = 2 * n * v * h
+        if case['train']:      # the gradients of both factors; the logits are not kept, so they are formed twice
+            moved += (n * h + v * h + (v if case['bias'] else 0)) * size
+            flops = 8 * n * v * h
+        return dict(bytes=moved, flops=flops)
+    n = _numel(case)
+    if op == 'clip':
+        return dict(bytes=n * 3 * size, flops=3 * n)
+    blocks = n / BLOCK
+    state = 16 * n if case['bits'] == 32 else 4 * n + 16 * blocks
+    moved = n * 3 * size + state + (8 * n if case['master'] else 0) + (n * size if case['clip'] else 0)
+    if case['bits'] == 8:      # and the values that the state stands for, written out
+        moved += 2 * n + 8 * blocks + 8 * n
+    return dict(bytes=moved, flops=15 * n)
+
+
+# ----------------------------------------------------------------------------------------- inputs
+def _generator(seed):
+    g = torch.Generator(device='cuda')
+    g.manual_seed(int(seed) + 12345)
+    return g
+
+
+def _ids(g, n, v):
+    """Token ids with a few frequent ones and a long tail."""
+    u = torch.rand(n, generator=g, device='cuda', dtype=torch.float64)
+    return (u.pow(3) * v).long().clamp_(max=v - 1)
+
+
+def _normal(g, shape, dtype, std):
+    return torch.randn(shape, generator=g, device='cuda', dtype=torch.float32).mul_(std).to(dtype)
+
+
+def prepare(case, seed):
+    g = _generator(seed)
+    dtype = TYPES[case['dtype']]
+    if case['op'] == 'embed':
+        n, v, e = case['n'], case['v'], case['e']
+        weight = _normal(g, (v, e), dtype, 1.0)
+        ids = _ids(g, n, v)
+        if case['pad'] >= 0:
+            ids[n - n // 8:] = case['pad']
+        state = dict(case=case, weight=weight, ids=ids)
+        if case['train']:
+            weight.requires_grad_(True)
+            state['grad'] = _normal(g, (n, e), dtype, 1e-2)
+        return state
+    if case['op'] == 'ce':
+        n, v, h = case['n'], case['v'], case['h']
+        wide = h + (16 if case['strided'] else 0)
+        hidden = _normal(g, (n, wide), dtype, 1.0)[:, :h]
+        weight = _normal(g, (v, h), dtype, 2.0 / math.sqrt(h))
+        targets = _ids(g, n, v)
+        if case['ignored'] > 0:
+            drop = torch.rand(n, generator=g, device='cuda') < case['ignored']
+            drop[0] = False
+            targets[drop] = IGNORE
+        bias = _normal(g, (v,), dtype, 0.1) if case['bias'] else None
+        rows = torch.rand(n, generator=g, device='cuda') if case['weighted'] else None
+        if case['train']:
+            hidden, weight = hidden.detach().requires_grad_(True), weight.requires_grad_(True)
+            bias = bias.requires_grad_(True) if bias is not None else None
+        return dict(case=case, hidden=hidden, weight=weight, bias=bias, targets=targets, rows=rows)
+    # many tensors, each at the start of a block of one buffer
+    shapes = _shapes(case)
+    sizes = [math.prod(s) for s in shapes]
+    starts, total = [], 0
+    for s in sizes:
+        starts.append(total)
+        total += -(-s // BLOCK) * BLOCK
+    held = torch.zeros(total, device='cuda', dtype=torch.bool)
+    for a, s in zip(starts, sizes):
+        held[a:a + s] = True
+
+    def flat(values, to):
+        return values.masked_fill_(~held, 0).to(to)
+
+    def views(buffer):
+        return [buffer[a:a + s].view(shape) for a, s, shape in zip(starts, sizes, shapes)]
+
+    def normal(std):
+        return torch.randn(total, generator=g, device='cuda').mul_(std)
+
+    state = dict(case=case, grad=flat(normal(1e-2), dtype))
+    state['grads'] = views(state['grad'])
+    if case['op'] == 'clip':
+        return state
+    state['param'] = flat(normal(0.02), dtype)
+    state['params'] = views(state['param'])
+    if case['master']:
+        state['master'] = state['param'].float() + flat(normal(1e-5), torch.float32)
+        state['param'].copy_(state['master'])
+        state['masters'] = views(state['master'])
+    state['step'] = torch.full((1,), STEPS_BEFORE, dtype=torch.int64, device='cuda')
+    m, v = flat(normal(3e-3), torch.float32), flat(normal(1e-2).square_(), torch.float32)
+    if case['bits'] == 32:
+        state['m'], state['v'] = m, v
+        state['ms'], state['vs'] = views(m), views(v)
+        return state
+    blocks = total // BLOCK
+    for name, x, signed in (('m', m, True), ('v', v, False)):
+        x = x.view(blocks, BLOCK)
+        top = x.abs().amax(1, keepdim=True)
+        part = x.abs() / torch.where(top > 0, top, torch.ones_like(top))
+        code = (part.sqrt() * 127).round() * x.sign() if signed else (part.sqrt().sqrt() * 255).round()
+        code = code.view(-1).to(torch.int8 if signed else torch.uint8)
+        top = top.view(-1).contiguous()
+        state[name], state[name + '_top'] = code, top
+        state[name + 's'] = views(code)
+        state[name + '_tops'] = [top[a // BLOCK:a // BLOCK + -(-s // BLOCK)] for a, s in zip(starts, sizes)]
+    return state
+
+
+# -------------------------------------------------------------------------------------- one pass
+def run(state):
+    return _RUN[state['case']['op']](state)
+
+
+def _embed(state):
+    case, weight, ids = state['case'], state['weight'], state['ids']
+    pad = case['pad']
+    if own:
+        from paccmann_generator_amd import ops
+        out = ops.embedding(weight, ids, scale=case['scale'], padding_idx=pad if pad >= 0 else None, trusted_tokens=True)
+        if not case['train']:
+            return out
+        grad, = torch.autograd.grad(out, weight, state['grad'])
+        return out.detach(), grad
+    with torch.no_grad():
+        out = (weight[ids].float() * case['scale']).to(weight.dtype)
+        if not case['train']:
+            return out
+        grad = torch.zeros(weight.shape, dtype=torch.float32, device=ids.device)
+        grad.index_add_(0, ids, state['grad'].float())
+        if pad >= 0:
+            grad[pad] = 0
+        return out, (grad * case['scale']).to(weight.dtype)
+
+
+def _ce(state):
+    case, hidden, weight, bias = state['case'], state['hidden'], state['weight'], state['bias']
+    targets, rows = state['targets'], state['rows']
+    if own:
+        from paccmann_generator_amd import ops
+        loss, lse = ops.linear_cross_entropy(hidden, weight, targets, bias=bias, row_weight=rows, ignore_index=IGNORE,
+                                             reduction='mean' if case['train'] else 'none', trusted_tokens=True)
+        if not case['train']:
+            return loss, lse
+        leaves = [hidden, weight] + ([bias] if bias is not None else [])
+        return (loss.detach(), lse.detach(), *torch.autograd.grad(loss, leaves))
+    with torch.no_grad():
+        x, w = hidden.float(), weight.float()
+        logits = x @ w.t()
+        if bias is not None:
+            logits += bias.float()
+        top = logits.amax(1, keepdim=True)
+        e = (logits - top).exp_()
+        total = e.sum(1, keepdim=True)
+        lse = (top + total.log()).squeeze(1)
+        used = targets != IGNORE
+        at = torch.where(used, targets, torch.zeros_like(targets)).unsqueeze(1)
+        nll = torch.where(used, lse - logits.gather(1, at).squeeze(1), torch.zeros_like(lse))
+        scale = used.float() if rows is None else torch.where(used, rows, torch.zeros_like(rows))
+        if not case['train']:
+            return nll * scale, lse
+        scale = scale / used.sum()
+        loss = (nll.double() * scale.double()).sum().float()
+        d = e.mul_((scale / total.squeeze(1)).unsqueeze(1))
+        d.scatter_add_(1, at, -scale.unsqueeze(1))
+        out = [loss, lse, (d @ w).to(hidden.dtype), (d.t() @ x).to(weight.dtype)]
+        if bias is not None:
+            out.append(d.sum(0).to(bias.dtype))
+        return tuple(out)
+
+
+def _norm(grad):
+    return grad.double().square().sum().sqrt().float()
+
+
+def _factor(norm):
+    return (MAX_NORM / (norm.double() + 1e-6)).clamp(max=1.0).float()
+
+
+def _clip(state):
+    if own:
+        from paccmann_generator_amd import ops
+        return ops.clip_grad_norm_(state['grads'], MAX_NORM), state['grad']
+    norm = _norm(state['grad'])
+    state['grad'].copy_(state['grad'].float() * _factor(norm))
+    return norm, state['grad']
+
+
+def _adamw(state):
+    case, h = state['case'], HYPER
+    out = {}
+    if own:
+        from paccmann_generator_amd import ops
+        if case['clip']:
+            out['norm'] = ops.grad_norm(state['grads'])
+        ops.adamw_step(state['params'], state['grads'], state['ms'], state['vs'], state['step'], lr=h['lr'],
+                       betas=(h['beta1'], h['beta2']), eps=h['eps'], weight_decay=h['weight_decay'],
+                       decoupled=case['decoupled'], exp_avg_top=state.get('m_tops'), exp_avg_sq_top=state.get('v_tops'),
+                       master=state.get('masters'), grad_norm=out.get('norm'), max_norm=MAX_NORM if case['clip'] else 0.0)
+        if case['bits'] == 8:
+            out['m'], out['v'] = ops.adamw_state_values(state['m'], state['m_top']), ops.adamw_state_values(state['v'], state['v_top'])
+    else:
+        # every product, sum and quotient is rounded by itself: the codes of an 8-bit state depend on the last bit
+        grad = state['grad'].float()
+        if case['clip']:
+            out['norm'] = _norm(state['grad'])
+            grad = grad * _factor(out['norm'])
+        p = state['master'] if case['master'] else state['param'].float()
+        state['step'] += 1
+        t = state['step'].double()
+        rate = (h['lr'] / (1 - h['beta1'] ** t)).float()
+        root = (1 / (1 - h['beta2'] ** t).sqrt()).float()
+        if not case['decoupled']:
+            grad = grad + h['weight_decay'] * p
+        if case['bits'] == 8:
+            m, v = _value(state['m'], state['m_top']), _value(state['v'], state['v_top'])
+        else:
+            m, v = state['m'], state['v']
+        m = m * h['beta1'] + grad * (1 - h['beta1'])
+        v = v * h['beta2'] + grad * grad * (1 - h['beta2'])
+        move = (m * rate) / (v.sqrt() * root + h['eps'])
+        p = (p * (1 - h['lr'] * h['weight_decay']) if case['decoupled'] else p) - move
+        state['param'].copy_(p)
+        if case['master']:
+            state['master'].copy_(p)
+        if case['bits'] == 8:
+            _hold(state['m'], state['m_top'], m)
+            _hold(state['v'], state['v_top'], v)
+            out['m'], out['v'] = _value(state['m'], state['m_top']), _value(state['v'], state['v_top'])
+        else:
+            state['m'].copy_(m)
+            state['v'].copy_(v)
+    if case['bits'] == 32:
+        out['m'], out['v'] = state['m'], state['v']
+    out['param'] = state['param']
+    if case['master']:
+        out['master'] = state['master']
+    return out
+
+
+def _value(code, top):
+    """What codes stand for: sign (c / 127)^2 of the block's largest magnitude, or (c / 255)^4 of it for squares."""
+    c = code.view(-1, BLOCK).float()
+    if code.dtype == torch.int8:
+        c = c * (1 / 127)
+        return (c * c.abs() * top.unsqueeze(1)).view(-1)
+    c = c * (1 / 255)
+    c = c * c
+    return (c * c * top.unsqueeze(1)).view(-1)
+
+
+def _hold(code, top, x):
+    x = x.view(-1, BLOCK)
+    most = x.abs().amax(1)
+    part = (x.abs() / most.unsqueeze(1)).nan_to_num(0.0).sqrt()
+    if code.dtype == torch.int8:
+        c = (part * 127).round() * x.sign()
+    else:       # a square above zero keeps a code above zero: the root that divides the step never vanishes
+        c = (part.sqrt() * 255).round()
+        c = torch.where(x > 0, c.clamp(min=1), c)
+    code.copy_(c.view(-1))
+    top.copy_(most)
+
+
+_RUN = dict(embed=_embed, ce=_ce, clip=_clip, adamw=_adamw)
+
+
+# ------------------------------------------------------------------------------- the definitions
+def exact(case, seed):
+    state = prepare(case, seed)
+    with torch.no_grad():
+        return _EXACT[case['op']](case, state)
+
+
+def _exact_embed(case, state):
+    table = state['weight'].detach().double() * case['scale']
+    out = torch.nn.functional.embedding(state['ids'], table)
+    if not case['train']:
+        return out
+    order = torch.sort(state['ids'], stable=True).indices
+    sums = torch.zeros(case['n'] + 1, case['e'], dtype=torch.float64, device='cuda')
+    torch.cumsum(state['grad'].double()[order], 0, out=sums[1:])
+    ends = torch.bincount(state['ids'], minlength=case['v']).cumsum(0)
+    begins = torch.cat([ends.new_zeros(1), ends[:-1]])
+    grad = (sums[ends] - sums[begins]) * case['scale']
+    if case['pad'] >= 0:
+        grad[case['pad']].zero_()
+    return out, grad
+
+
+def _exact_ce(case, state):
+    x, w = state['hidden'].detach().double(), state['weight'].detach().double()
+    logits = torch.mm(x, w.t().contiguous())
+    if state['bias'] is not None:
+        logits += state['bias'].detach().double()
+    lse = torch.logsumexp(logits, 1)
+    keep = state['targets'].ne(IGNORE)
+    weight = torch.ones_like(lse) if state['rows'] is None else state['rows'].double()
+    weight = weight * keep
+    row = torch.arange(case['n'], device='cuda')
+    picked = logits[row, state['targets'].clamp(min=0)]
+    if not case['train']:
+        return torch.where(keep, (lse - picked) * weight, torch.zeros_like(lse)), lse
+    weight = weight / keep.sum()
+    loss = ((lse - picked) * weight).sum()
+    slope = logits.sub_(lse.unsqueeze(1)).exp_().mul_(weight.unsqueeze(1))
+    slope[row[keep], state['targets'][keep]] -= weight[keep]
+    out = [loss, lse, torch.mm(slope, w), torch.mm(slope.t().contiguous(), x)]
+    if state['bias'] is not None:
+        out.append(slope.sum(0))
+    return tuple(out)
+
+
+def _exact_clip(case, state):
+    g = state['grad'].double()
+    norm = torch.linalg.vector_norm(g)
+    return norm, g * min(1.0, MAX_NORM / (float(norm) + 1e-6))
+
+
+def _exact_adamw(case, state):
+    h, t = HYPER, STEPS_BEFORE + 1
+    g = state['grad'].double()
+    norm = torch.linalg.vector_norm(g)
+    if case['clip']:
+        g = g * min(1.0, MAX_NORM / (float(norm) + 1e-6))
+    p = (state['master'] if case['master'] else state['param']).double()
+    if case['bits'] == 8:
+        share = state['m'].double() / 127
+        m = share * share.abs() * state['m_top'].double().repeat_interleave(BLOCK)
+        v = (state['v'].double() / 255) ** 4 * state['v_top'].double().repeat_interleave(BLOCK)
+    else:
+        m, v = state['m'].double(), state['v'].double()
+    if not case['decoupled']:
+        g = g + h['weight_decay'] * p
+    m = h['beta1'] * m + (1 - h['beta1']) * g
+    v = h['beta2'] * v + (1 - h['beta2']) * g ** 2
+    unbiased_m, unbiased_v = m / (1 - h['beta1'] ** t), v / (1 - h['beta2'] ** t)
+    if case['decoupled']:
+        p = p - h['lr'] * h['weight_decay'] * p
+    p = p - h['lr'] * unbiased_m / (unbiased_v.sqrt() + h['eps'])
+    # codes of 8 bits have no exact value: a state next to the border of two codes may take either
+    out = dict(param=p, m=None, v=None) if case['bits'] == 8 else dict(param=p, m=m, v=v)
+    if case['clip']:
+        out['norm'] = norm
+    if case['master']:
+        out['master'] = p
+    return out
+
+
+_EXACT = dict(embed=_exact_embed, ce=_exact_ce, clip=_exact_clip, adamw=_exact_adamw)
