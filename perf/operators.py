@@ -393,7 +393,8 @@ def _value(code, top):
 def _hold(code, top, x):
     x = x.view(-1, BLOCK)
     most = x.abs().amax(1)
-    part = (x.abs() / most.unsqueeze(1)).nan_to_num(0.0).sqrt()
+    share = torch.where(most >= torch.finfo(torch.float32).tiny, 1 / most, torch.zeros_like(most))
+    part = (x.abs() * share.unsqueeze(1)).sqrt().nan_to_num(0.0)
     if code.dtype == torch.int8:
         c = (part * 127).round() * x.sign()
     else:       # a square above zero keeps a code above zero: the root that divides the step never vanishes
