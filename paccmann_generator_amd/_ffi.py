@@ -52,11 +52,40 @@ class PmgGrads(C.Structure):
     ]
 
 
+# include/pmg_lm.h
+PMG_F32, PMG_BF16, PMG_F16 = 0, 1, 2
+PMG_STATE_BLOCK = 256
+PMG_ADAMW_WS = 64
+
+
+class PmgAdamw(C.Structure):
+    _fields_ = [
+        ('n', C.c_int), ('dtype', C.c_int), ('grad_dtype', C.c_int), ('state_bits', C.c_int), ('decoupled', C.c_int),
+        ('numel', _F), ('param', _F), ('grad', _F), ('m', _F), ('v', _F), ('m_top', _F), ('v_top', _F), ('master', _F),
+        ('step', _F), ('lr_dev', _F), ('norm', _F),
+        ('lr', C.c_double), ('beta1', C.c_double), ('beta2', C.c_double), ('eps', C.c_double),
+        ('weight_decay', C.c_double), ('max_norm', C.c_double),
+    ]
+
+
 EXPORTS = (
     'pmg_abi_version', 'pmg_strerror', 'pmg_check_shape', 'pmg_workspace_bytes',
     'pmg_decode', 'pmg_logprob_fwd', 'pmg_reinforce_bwd', 'pmg_step', 'pmg_detokenize',
     'pmg_decode_noalloc', 'pmg_noalloc_scratch_bytes', 'pmg_reinforce_bptt', 'pmg_reinforce_wgrad', 'pmg_uses_cluster',
 )
+
+# entry points of include/pmg_lm.h with their arguments
+_P, _I, _L, _SIZE = C.c_void_p, C.c_int, C.c_int64, C.POINTER(C.c_size_t)
+LM_EXPORTS = {
+    'pmg_embedding_fwd': [_P, _L, _P, _I, _L, _L, _L, _I, C.c_float, _P, _P],
+    'pmg_embedding_bwd_workspace': [_L, _L, _L, _SIZE],
+    'pmg_embedding_bwd': [_P, _L, _P, _I, _L, _L, _L, _I, C.c_float, _L, _P, _P, _P],
+    'pmg_grad_norm_workspace': [_P, _I, _SIZE],
+    'pmg_grad_norm': [_P, _P, _P, _I, _P, _P, _P],
+    'pmg_grad_clip': [_P, _P, _P, _I, _P, C.c_float, _P],
+    'pmg_adamw_step': [C.POINTER(PmgAdamw), _P, _P],
+    'pmg_adamw_values': [_P, _P, _L, _I, _P, _P],
+}
 
 
 def _load():
@@ -65,7 +94,7 @@ def _load():
             f'{LIB_PATH} is missing: build the HIP library first '
             f'(python -c "import __graft_entry__ as g; g.build()"). There is no CPU fallback.')
     lib = C.CDLL(LIB_PATH)
-    for name in EXPORTS:
+    for name in (*EXPORTS, *LM_EXPORTS):
         if not hasattr(lib, name):
             raise ImportError(f'{LIB_PATH} does not export {name}')
     lib.pmg_abi_version.restype = C.c_int
@@ -100,6 +129,9 @@ def _load():
     for name in EXPORTS[2:]:
         getattr(lib, name).restype = C.c_int
     lib.pmg_noalloc_scratch_bytes.restype = C.c_size_t
+    for name, args in LM_EXPORTS.items():
+        getattr(lib, name).argtypes = args
+        getattr(lib, name).restype = C.c_int
     if lib.pmg_abi_version() != PMG_ABI_VERSION:
         raise ImportError('libpmg.so ABI version mismatch')
     return lib

@@ -95,11 +95,13 @@ extern "C" const char* pmg_strerror(int code) {
     case PMG_E_STACK: return "unsupported stack: need 1<=W<=64, 2<=D";
     case PMG_E_VOCAB: return "unsupported vocabulary: need 2<=V<=1024";
     case PMG_E_LAYERS: return "unsupported n_layers: need 1<=L<=4";
-    case PMG_E_ALIGN: return "pointer not 16-byte aligned (b_l2h of pmg_decode, grad_h0 of pmg_reinforce_bwd)";
+    case PMG_E_ALIGN: return "pointer not 16-byte aligned (b_l2h of pmg_decode, grad_h0 of pmg_reinforce_bwd, workspaces) or not to its element type";
     case PMG_E_MODE: return "unknown workspace mode";
     case PMG_E_ARG: return "bad argument";
     case PMG_E_LDS: return "shape needs more than 160 KiB of LDS per workgroup";
     case PMG_E_SCRATCH: return "shape needs more scratch than the 32 MiB static array of pmg_decode_noalloc holds";
+    case PMG_E_DTYPE: return "unsupported element type or combination of element types";
+    case PMG_E_OVERLAP: return "a buffer that is written overlaps another buffer of the call";
   }
   return code > 0 ? "HIP runtime error (see hipGetErrorString)" : "unknown error";
 }

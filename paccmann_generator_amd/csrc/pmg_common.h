@@ -50,6 +50,8 @@ enum {
   PMG_E_ARG = -9,
   PMG_E_LDS = -10,
   PMG_E_SCRATCH = -11,
+  PMG_E_DTYPE = -12,
+  PMG_E_OVERLAP = -13,
 };
 
 // Derived dimensions, identical on host and device.
