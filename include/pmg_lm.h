@@ -45,6 +45,51 @@ int pmg_embedding_bwd_workspace(int64_t N, int64_t V, int64_t E, size_t* out);
 int pmg_embedding_bwd(const void* grad, int64_t ld_grad, const void* ids, int id_bits, int64_t N, int64_t V, int64_t E,
                       int dtype, float scale, int64_t padding_idx, void* grad_weight, void* ws, pmg_stream stream);
 
+/* --------------------------------------------------- cross entropy of a linear vocabulary projection */
+
+#define PMG_REDUCE_NONE 0
+#define PMG_REDUCE_SUM 1
+#define PMG_REDUCE_MEAN 2 /* over the rows with a target; 0 without any */
+
+/* With logits l = logit_scale (hidden weight^T + bias), never kept:
+ *   lse[n]  = log sum_v exp l[n,v]
+ *   nll[n]  = row_weight[n] (lse[n] - l[n,targets[n]]), 0 where targets[n] == ignore_index
+ *   loss    = nll [N] (PMG_REDUCE_NONE), its sum, or its sum / count; count[0] = rows with a target
+ * and, from grad_loss ([N] or [1], as loss) and grad_lse ([N]; either may be NULL: no slope), the
+ * gradients of hidden, weight and bias (each NULL: not formed).  row_weight has no gradient.  A row without
+ * a slope (ignored, of weight 0) has a zero gradient and adds nothing to the others, whatever it holds.
+ * A target outside [0,V) that is not ignore_index gives NaN (memory safety; validate on the host).
+ * dtype PMG_F32 or PMG_BF16; the slopes of the logits are rounded to it once, all sums are fp32. */
+typedef struct pmg_linear_ce {
+  int64_t N, V, H;
+  int dtype;               /* of hidden, weight, bias and their gradients */
+  int id_bits;             /* of targets: 32 or 64 */
+  int reduction;
+  float logit_scale;
+  int64_t ignore_index;
+  int64_t ld_hidden, ld_weight;
+  const void* hidden;      /* [N,H] */
+  const void* weight;      /* [V,H] */
+  const void* bias;        /* [V] or NULL */
+  const void* targets;     /* [N] */
+  const float* row_weight; /* [N] or NULL */
+  float* loss;             /* forward: written */
+  float* lse;              /* [N]; forward: written, backward: read */
+  float* count;            /* [1]; forward: written unless PMG_REDUCE_NONE (then NULL), backward: read with
+                              PMG_REDUCE_MEAN */
+  const float* grad_loss;  /* backward */
+  const float* grad_lse;
+  void* grad_hidden;       /* [N,H] contiguous */
+  void* grad_weight;       /* [V,H] contiguous */
+  void* grad_bias;         /* [V] */
+} pmg_linear_ce;
+
+/* Bytes of scratch of one direction.  It does not grow with N x V: the backward keeps the slopes of a
+ * piece of the vocabulary at a time. */
+int pmg_linear_ce_workspace(const pmg_linear_ce* a, int backward, size_t* out);
+int pmg_linear_ce_fwd(const pmg_linear_ce* a, void* ws, pmg_stream stream);
+int pmg_linear_ce_bwd(const pmg_linear_ce* a, void* ws, pmg_stream stream);
+
 /* ---------------------------------------------------------------- norm and clipping of many gradients */
 
 /* Bytes of scratch for pmg_grad_norm over `n` tensors of numel[i] elements (numel: HOST array). */

@@ -79,3 +79,42 @@ def adamw(p, g, m, v, t, lr, beta1, beta2, eps, wd, decoupled, factor=1.0):
     v = v * as_(beta2) + (g * g) * as_(1 - beta2)
     move = (m * rate) / (sqrt(v) * root + as_(eps))
     return p * as_(1 - lr * wd if decoupled else 1.0) - move, m, v
+
+
+def linear_ce(x, w, t, b=None, r=None, scale=1.0, reduction='mean', ignore=-100):
+    """Loss and log-sum-exp of scale (x w^T + b), with ``size`` (the largest sum of magnitudes behind a row's logits),
+    ``w`` (the rows' weights, 0 without a target) and ``count``."""
+    H = x.shape[-1]
+    X, W, T = x.double().reshape(-1, H), w.double(), t.reshape(-1).long()
+    logits = X @ W.t()
+    size = (X.abs() @ W.abs().t()).amax(1)
+    if b is not None:
+        logits = logits + b.double()
+        size = size + b.double().abs().amax()
+    logits = logits * scale
+    lse = torch.logsumexp(logits, 1)
+    keep = T != ignore
+    weight = keep.double() * (r.double().reshape(-1) if r is not None else 1.0)
+    nll = torch.where(keep, (lse - logits.gather(1, T.clamp(min=0).unsqueeze(1)).squeeze(1)) * weight, torch.zeros_like(lse))
+    count = int(keep.sum())
+    loss = nll if reduction == 'none' else nll.sum() if reduction == 'sum' else nll.sum() / max(1, count)
+    return dict(loss=loss, lse=lse, size=size * abs(scale), w=weight, count=count, logits=logits, keep=keep)
+
+
+def linear_ce_grads(x, w, t, b, r, scale, reduction, ignore, slope, lse_slope):
+    """Gradients of sum(slope loss) + sum(lse_slope lse), and under |name| the sums of magnitudes that form them."""
+    e = linear_ce(x, w, t, b, r, scale, reduction, ignore)
+    H = x.shape[-1]
+    X, W, T = x.double().reshape(-1, H), w.double(), t.reshape(-1).long()
+    c = e['w'] * slope.double().reshape(-1)
+    if reduction == 'mean':
+        c = c / max(1, e['count'])
+    a = c + (lse_slope.double().reshape(-1) if lse_slope is not None else 0.0)
+    d = (e['logits'] - e['lse'].unsqueeze(1)).exp() * a.unsqueeze(1)
+    mag = d.abs()
+    row = torch.arange(len(T), device=T.device)[e['keep']]
+    d[row, T[row]] -= c[row]
+    mag[row, T[row]] += c[row].abs()
+    d, mag = d * scale, mag * abs(scale)
+    return {'x': (d @ W).view(x.shape), '|x|': (mag @ W.abs()).view(x.shape), 'w': d.t().contiguous() @ X, '|w|': mag.t().contiguous() @ X.abs(),
+            'b': d.sum(0), '|b|': mag.sum(0)}

@@ -68,6 +68,19 @@ class PmgAdamw(C.Structure):
     ]
 
 
+PMG_REDUCE = {'none': 0, 'sum': 1, 'mean': 2}
+
+
+class PmgLinearCe(C.Structure):
+    _fields_ = [
+        ('N', C.c_int64), ('V', C.c_int64), ('H', C.c_int64), ('dtype', C.c_int), ('id_bits', C.c_int),
+        ('reduction', C.c_int), ('logit_scale', C.c_float), ('ignore_index', C.c_int64), ('ld_hidden', C.c_int64),
+        ('ld_weight', C.c_int64), ('hidden', _F), ('weight', _F), ('bias', _F), ('targets', _F), ('row_weight', _F),
+        ('loss', _F), ('lse', _F), ('count', _F), ('grad_loss', _F), ('grad_lse', _F), ('grad_hidden', _F),
+        ('grad_weight', _F), ('grad_bias', _F),
+    ]
+
+
 EXPORTS = (
     'pmg_abi_version', 'pmg_strerror', 'pmg_check_shape', 'pmg_workspace_bytes',
     'pmg_decode', 'pmg_logprob_fwd', 'pmg_reinforce_bwd', 'pmg_step', 'pmg_detokenize',
@@ -80,6 +93,9 @@ LM_EXPORTS = {
     'pmg_embedding_fwd': [_P, _L, _P, _I, _L, _L, _L, _I, C.c_float, _P, _P],
     'pmg_embedding_bwd_workspace': [_L, _L, _L, _SIZE],
     'pmg_embedding_bwd': [_P, _L, _P, _I, _L, _L, _L, _I, C.c_float, _L, _P, _P, _P],
+    'pmg_linear_ce_workspace': [C.POINTER(PmgLinearCe), _I, _SIZE],
+    'pmg_linear_ce_fwd': [C.POINTER(PmgLinearCe), _P, _P],
+    'pmg_linear_ce_bwd': [C.POINTER(PmgLinearCe), _P, _P],
     'pmg_grad_norm_workspace': [_P, _I, _SIZE],
     'pmg_grad_norm': [_P, _P, _P, _I, _P, _P, _P],
     'pmg_grad_clip': [_P, _P, _P, _I, _P, C.c_float, _P],

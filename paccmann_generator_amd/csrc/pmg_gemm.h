@@ -1,0 +1,234 @@
+// The tile product behind the linear cross entropy (pmg_lce.hip):  D[m][n] = sum_k A(m,k) B(n,k)  for one
+// BM x BN tile, on MFMA, operands in bf16 or fp32, sums in fp32.
+//
+// An operand lies in memory with k contiguous (rows of m or n) or with m / n contiguous (rows of k): the
+// vocabulary projection and the hidden states enter the logits the first way and their own gradients the
+// second way, so no transposed copy of either is made.
+//
+// LDS holds two stages of 128 bytes of k per row (64 bf16 or 32 fp32), filled by 16-byte loads that go
+// straight to LDS; while a stage is multiplied the next one is in flight.  The loads write LDS linearly, so
+// what keeps the reads free of bank conflicts is which global 16 bytes a lane fetches:
+//   k contiguous: 16-byte piece c of row r lies at piece c ^ (r & 7); a fragment is one ds_read_b128
+//   m contiguous: 32-byte (bf16) or 64-byte (fp32) pieces of row k lie at piece ^ f(k), f chosen so that the
+//                 rows one read touches fall into different banks; a bf16 fragment is two transposing
+//                 reads (ds_read_b64_tr_b16), an fp32 fragment four single ones
+// An operand may be read through a list of its rows (of m or n where k is contiguous, of k otherwise): the
+// training rows of a batch stay where they are.
+// Lane l of a wave holds of a 16x16 tile of D column n = l & 15 and rows m = 4 (l >> 4) .. + 3.
+#pragma once
+#include "pmg_kernels.h"
+#include "pmg_types.h"
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+
+typedef __attribute__((address_space(3))) char lds_char;
+
+template <typename T> struct pmg_frag;  // 16 bytes of k of one row
+template <> struct pmg_frag<bf16_t> {
+  typedef bf16x8 type;
+  static __device__ __forceinline__ f32x4 mma(type a, type b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+};
+template <> struct pmg_frag<float> {
+  typedef f32x4 type;
+  static __device__ __forceinline__ f32x4 mma(type a, type b, f32x4 c) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
+    return c;
+  }
+};
+
+// 16 bytes that stand for operand elements behind the end of k
+static __device__ const float4 pmg_zero16 = {0.f, 0.f, 0.f, 0.f};
+
+__device__ __forceinline__ void pmg_load_lds16(const char* src, lds_char* dst) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
+                                   (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
+}
+
+// One operand's share of a stage: R rows of m (or n), 128 bytes of k.
+//   KC: k contiguous.  WAVES waves fill it, 1 KB an instruction.  LIST: rows by a list.
+template <typename T, int R, bool KC, int WAVES, bool LIST> struct pmg_operand {
+  static constexpr int E16 = 16 / sizeof(T);
+  static constexpr int KSTEP = 128 / sizeof(T);
+  static constexpr int BYTES = R * 128;
+  static constexpr int CNT = BYTES / 1024 / WAVES;
+  static constexpr int ROWB = R * sizeof(T);      // bytes of a row of k (m contiguous)
+  static constexpr int PIECES = ROWB / 16;
+  static_assert(BYTES % (1024 * WAVES) == 0, "whole instructions");
+  static_assert(KC || PIECES >= 8, "the permutation stays inside a row");
+
+  static __device__ __forceinline__ int perm(int k) {  // of the 16-byte pieces of row k (m contiguous)
+    if (sizeof(T) == 2) return (((k & 3) | (((k >> 3) & 3) << 2)) & (PIECES / 2 - 1)) << 1;
+    return (((k >> 2) & 3) << 2) & (PIECES - 1);
+  }
+
+  const char* src[CNT];
+  int64_t step;   // bytes from stage to stage
+  int kofs[CNT];  // k of this lane's 16 bytes within a stage
+  // m contiguous with a list: the list's entries of the next stage, loaded a stage ahead
+  const int* list;
+  int64_t row_bytes;
+  int next[CNT];
+
+  __device__ __forceinline__ void look_up(int64_t left) {
+#pragma unroll
+    for (int j = 0; j < CNT; ++j) next[j] = kofs[j] < left ? list[kofs[j]] : 0;
+    list += KSTEP;
+  }
+
+  // rows row0 .. of R_all (clamped: rows behind the end repeat the last one and are not stored), k from k0
+  __device__ __forceinline__ void init(const void* base, int64_t ld, const int* rows, int64_t row0, int64_t R_all, int64_t k0,
+                                       int64_t left) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    step = KC ? 128 : (int64_t)KSTEP * ld * (int64_t)sizeof(T);
+#pragma unroll
+    for (int j = 0; j < CNT; ++j) {
+      const int byte = (wave * CNT + j) * 1024 + lane * 16;
+      if (KC) {
+        const int row = byte >> 7, c = ((byte >> 4) & 7) ^ (row & 7);
+        int64_t r = row0 + row < R_all ? row0 + row : R_all - 1;
+        if (LIST) r = rows[r];
+        kofs[j] = c * E16;
+        src[j] = (const char*)base + (r * ld + k0 + kofs[j]) * (int64_t)sizeof(T);
+      } else {
+        const int k = byte / ROWB, c = ((byte % ROWB) >> 4) ^ perm(k);
+        const int64_t last = ((R_all + E16 - 1) / E16 - 1) * E16;
+        const int64_t m = row0 + c * E16 < last ? row0 + c * E16 : last;
+        kofs[j] = k;
+        src[j] = (const char*)base + ((LIST ? 0 : (k0 + k) * ld) + m) * (int64_t)sizeof(T);
+      }
+    }
+    if (LIST && !KC) {
+      row_bytes = ld * (int64_t)sizeof(T);
+      list = rows + k0;
+      look_up(left);
+    }
+  }
+
+  // one stage into LDS at `dst`; `left`: k that remain (elements behind it read as zeros)
+  __device__ __forceinline__ void fetch(lds_char* dst, int64_t left) {
+    const int wave = threadIdx.x >> 6;
+    lds_char* d = dst + wave * (CNT * 1024);
+    if (LIST && !KC) {
+#pragma unroll
+      for (int j = 0; j < CNT; ++j)
+        pmg_load_lds16(kofs[j] < left ? src[j] + next[j] * row_bytes : (const char*)&pmg_zero16, d + j * 1024);
+      look_up(left - KSTEP);
+      return;
+    }
+    if (left >= KSTEP) {
+#pragma unroll
+      for (int j = 0; j < CNT; ++j) {
+        pmg_load_lds16(src[j], d + j * 1024);
+        src[j] += step;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < CNT; ++j) pmg_load_lds16(kofs[j] < left ? src[j] : (const char*)&pmg_zero16, d + j * 1024);
+    }
+  }
+
+  typedef typename pmg_frag<T>::type frag;
+  // the fragment of rows row .. row + 15 (of this operand's R) for half kk of the stage
+  static __device__ __forceinline__ frag read(const lds_char* s, int row, int kk) {
+    const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
+    if (KC) {
+      const int r = row + i;
+      return *(const __attribute__((address_space(3))) frag*)(s + r * 128 + (((kk * 4 + g) ^ (r & 7)) << 4));
+    } else if constexpr (sizeof(T) == 2) {
+      frag f;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int k = kk * 32 + 8 * g + 4 * h + (i >> 2);
+        const int c = (row >> 3) + ((i & 3) >> 1);
+        typedef short s16x4 __attribute__((ext_vector_type(4)));
+        const s16x4 t = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) s16x4*)(s + k * ROWB + ((c ^ perm(k)) << 4) + ((i & 1) << 3)));
+        const bf16x4 v = __builtin_bit_cast(bf16x4, t);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[4 * h + j] = v[j];
+      }
+      return f;
+    } else {
+      frag f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int k = kk * 16 + 4 * g + j, m = row + i;
+        f[j] = *(const __attribute__((address_space(3))) float*)(s + k * ROWB + (((m >> 2) ^ perm(k)) << 4) + ((m & 3) << 2));
+      }
+      return f;
+    }
+  }
+};
+
+// The tile of workgroup `id`: workgroups go round the 8 XCDs, so every XCD gets a run of neighbouring tiles
+// (its L2 then serves the operands' rows that they share), in blocks of 8 tiles of m by all of n.
+__device__ __forceinline__ void pmg_tile_of(int id, int tiles_m, int tiles_n, int* tm, int* tn) {
+  const int total = tiles_m * tiles_n, q = total >> 3, r = total & 7, x = id & 7;
+  const int t = x * q + (x < r ? x : r) + (id >> 3);
+  const int width = 8 * tiles_n, g = t / width, first = g * 8;
+  const int gm = tiles_m - first < 8 ? tiles_m - first : 8, in = t - g * width;
+  *tm = first + in % gm;
+  *tn = in / gm;
+}
+
+// acc[i][j]: the 16x16 tiles of wave (wm, wn)'s (BM / WM) x (BN / WN) part; k from k0 to k1 (k0 a multiple of the
+// stage).  Ends behind a barrier: LDS is free.
+template <typename T, int BM, int BN, int WM, int WN, bool AKC, bool BKC, bool ALIST, bool BLIST> struct pmg_tile {
+  static constexpr int WAVES = WM * WN, THREADS = WAVES * 64;
+  static constexpr int MI = BM / WM / 16, NI = BN / WN / 16;
+  typedef pmg_operand<T, BM, AKC, WAVES, ALIST> OpA;
+  typedef pmg_operand<T, BN, BKC, WAVES, BLIST> OpB;
+  static constexpr int STAGE = OpA::BYTES + OpB::BYTES;
+  static constexpr int LDS = 2 * STAGE;
+  static constexpr int KSTEP = OpA::KSTEP;
+
+  static __device__ __forceinline__ void run(f32x4 (&acc)[MI][NI], lds_char* lds, const void* A, int64_t lda, const int* rows_a,
+                                             int64_t m0, int64_t M, const void* B, int64_t ldb, const int* rows_b, int64_t n0,
+                                             int64_t N, int64_t k0, int64_t k1) {
+    const int wave = threadIdx.x >> 6, rowA = (wave / WN) * (BM / WM), rowB = (wave % WN) * (BN / WN);
+    OpA a;
+    OpB b;
+    a.init(A, lda, rows_a, m0, M, k0, k1 - k0);
+    b.init(B, ldb, rows_b, n0, N, k0, k1 - k0);
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NI; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    int64_t left = k1 - k0;
+    if (left <= 0) return;
+    a.fetch(lds, left);
+    b.fetch(lds + OpA::BYTES, left);
+    int cur = 0;
+    while (left > 0) {
+      // this stage has landed, and every wave is done with the other one
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      const lds_char* s = lds + cur * STAGE;
+      left -= KSTEP;
+      cur ^= 1;
+      if (left > 0) {
+        a.fetch(lds + cur * STAGE, left);
+        b.fetch(lds + cur * STAGE + OpA::BYTES, left);
+      }
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) {
+        typename OpA::frag fa[MI];
+        typename OpB::frag fb[NI];
+#pragma unroll
+        for (int i = 0; i < MI; ++i) fa[i] = OpA::read(s, rowA + i * 16, kk);
+#pragma unroll
+        for (int j = 0; j < NI; ++j) fb[j] = OpB::read(s + OpA::BYTES, rowB + j * 16, kk);
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+          for (int j = 0; j < NI; ++j) acc[i][j] = pmg_frag<T>::mma(fa[i], fb[j], acc[i][j]);
+      }
+    }
+    __syncthreads();
+  }
+};

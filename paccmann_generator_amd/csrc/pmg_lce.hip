@@ -1,0 +1,872 @@
+// Cross entropy of a linear vocabulary projection, with its gradients (include/pmg_lm.h); the logits are
+// never kept.
+//
+//   l = s (x W^T + b)     lse_n = log sum_v exp l_nv     nll_n = lse_n - l_{n,t_n}
+//   dl_nv = s (a_n exp(l_nv - lse_n) - c_n [v = t_n])    dx = dl W    dW = dl^T x    db = sum_n dl_n
+// where c_n is the slope of the loss in nll_n and a_n that plus the slope in lse_n.
+//
+// Forward: the tile product of pmg_gemm.h (m = vocabulary, n = tokens) whose epilogue leaves per token and
+// vocabulary tile the largest logit and the sum of exponentials below it, and the target's logit: 8 bytes
+// for 256 logits.  A second kernel joins them.  Few tokens (serving) take narrow tiles: W is streamed once.
+// Backward: the vocabulary goes in pieces; of each piece the logits are formed again, dl is written in the
+// operands' type (bf16: one rounding, relative 2^-9 like the operands themselves; the products sum in
+// fp32) and read by the two products for dx and dW.  dx is summed over the pieces in fp32.  Long sums with
+// few result tiles are split and joined in a fixed order.  No atomics: equal inputs give equal bits.
+// Rows without a slope (ignored targets, zero weights) take no part in the backward: the others are listed, the
+// products run over the list, and the rows left out get a zero gradient whatever they hold.
+// Bound by the matrix units for many tokens (8 N V H operations, two of them for the second forming of the
+// logits), by reading W for few.
+#include "pmg_gemm.h"
+
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+template <typename T> __device__ __forceinline__ float exp_of(float x);
+template <> __device__ __forceinline__ float exp_of<float>(float x) { return expf(x); }
+// behind bf16 operands the hardware's 2^x of a rounded product is exact enough: relative 2^-24 |x| log2(e)
+template <> __device__ __forceinline__ float exp_of<bf16_t>(float x) { return __builtin_amdgcn_exp2f(x * LOG2E); }
+
+// ------------------------------------------------------------------------------------------ arguments
+struct LogitArgs {
+  const void *W, *X, *bias;
+  int64_t ldw, ldx;
+  int64_t V, N, K;       // vocabulary rows of this piece, tokens, hidden size
+  int64_t v0;            // first vocabulary entry of the piece
+  int tiles_m, tiles_n;
+  float scale;
+  const void* targets;
+  int id_bits;
+  // forward
+  float2* part;          // [tiles_m][N]
+  float* at_target;      // [N]
+  // backward: over the listed rows
+  const struct Row* row; // [count]
+  const int* list;       // [count] their places in X
+  const int* count;
+  void* dl;              // [count][ldl], columns V .. ldl zero
+  int64_t ldl;
+  float* dbias;          // [tiles_n][ldl] or null
+};
+
+__device__ __forceinline__ int64_t target_of(const void* t, int bits, int64_t n) {
+  return bits == 64 ? ((const int64_t*)t)[n] : (int64_t)((const int32_t*)t)[n];
+}
+
+// A row that takes part in the backward
+struct Row {
+  float lse, a, c;       // a_n, c_n
+  int target;            // -1: outside the vocabulary
+};
+
+// ------------------------------------------------------------------------------------------ logits
+template <typename T, int BM, int BN, int WM, int WN, bool BACKWARD>
+__global__ __launch_bounds__(WM* WN * 64) void lce_logits_kernel(const LogitArgs a) {
+  typedef pmg_tile<T, BM, BN, WM, WN, true, true, false, BACKWARD> Tile;
+  constexpr int MI = Tile::MI, NI = Tile::NI;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  int tm, tn;
+  pmg_tile_of(blockIdx.x, a.tiles_m, a.tiles_n, &tm, &tn);
+  const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
+  const int64_t N = BACKWARD ? a.count[0] : a.N;
+  if (BACKWARD && n0 >= N) return;
+  f32x4 acc[MI][NI];
+  Tile::run(acc, (lds_char*)smem, a.W, a.ldw, nullptr, m0, a.V, a.X, a.ldx, a.list, n0, N, 0, a.K);
+
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / WN, wn = wave % WN;
+  const int g = lane >> 4, col = lane & 15;
+  const int64_t mw = m0 + wm * (BM / WM) + 4 * g;  // this lane's rows: mw + 16 i + e
+  const T* bias = (const T*)a.bias;
+  // logits; entries behind the vocabulary's end do not take part
+#pragma unroll
+  for (int i = 0; i < MI; ++i) {
+    f32x4 b = {0.f, 0.f, 0.f, 0.f};
+    if (bias) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (mw + i * 16 + e < a.V) b[e] = (float)bias[mw + i * 16 + e];
+    }
+#pragma unroll
+    for (int j = 0; j < NI; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        acc[i][j][e] = mw + i * 16 + e < a.V ? (acc[i][j][e] + b[e]) * a.scale : -__builtin_inff();
+  }
+
+  if constexpr (!BACKWARD) {
+    float2* red = (float2*)smem;  // [WM][BN]
+#pragma unroll
+    for (int j = 0; j < NI; ++j) {
+      const int64_t n = n0 + wn * (BN / WN) + j * 16 + col;
+      float top = -__builtin_inff();
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = fmaxf(top, acc[i][j][e]);
+      top = fmaxf(top, __shfl_xor(top, 16, 64));
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      const float base = top == -__builtin_inff() ? 0.0f : top;  // nothing but -inf: the sum is 0
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum += exp_of<T>(acc[i][j][e] - base);  // a NaN logit makes a NaN sum
+      sum += __shfl_xor(sum, 16, 64);
+      sum += __shfl_xor(sum, 32, 64);
+      if (g == 0) red[wm * BN + wn * (BN / WN) + j * 16 + col] = make_float2(top, sum);
+      if (n < a.N) {
+        const int64_t t = target_of(a.targets, a.id_bits, n) - a.v0;
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (mw + i * 16 + e == t && t < a.V) a.at_target[n] = acc[i][j][e];
+      }
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < BN; c += Tile::THREADS) {
+      float top = -__builtin_inff(), sum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < WM; ++w) top = fmaxf(top, red[w * BN + c].x);
+#pragma unroll
+      for (int w = 0; w < WM; ++w) {
+        const float2 r = red[w * BN + c];
+        sum += r.x == -__builtin_inff() ? r.y : r.y * exp_of<T>(r.x - top);
+      }
+      if (n0 + c < a.N) a.part[(int64_t)tm * a.N + n0 + c] = make_float2(top, sum);
+    }
+  } else {
+    T* dl = (T*)a.dl;
+    float db[MI][4];
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) db[i][e] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NI; ++j) {
+      const int64_t n = n0 + wn * (BN / WN) + j * 16 + col;
+      if (n < N) {
+        const Row r = a.row[n];
+        const float as = r.a * a.scale, cs = r.c * a.scale;
+        const int64_t t = (int64_t)r.target - a.v0;
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+          f32x4 d;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int64_t v = mw + i * 16 + e;
+            float x = v < a.V ? as * exp_of<T>(acc[i][j][e] - r.lse) : 0.0f;  // entries behind the end are zero
+            if (v == t && v < a.V) x -= cs;
+            d[e] = x;
+            db[i][e] += x;
+          }
+          const int64_t v = mw + i * 16;
+          if (v < a.ldl) pmg_store4(dl + n * a.ldl + v, d);  // ldl is a multiple of 64
+        }
+      }
+    }
+    if (a.dbias) {
+      float* red = (float*)smem;  // [WN][BM]
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float s = db[i][e];
+          s += __shfl_xor(s, 1, 64);
+          s += __shfl_xor(s, 2, 64);
+          s += __shfl_xor(s, 4, 64);
+          s += __shfl_xor(s, 8, 64);
+          if (col == 0) red[wn * BM + wm * (BM / WM) + i * 16 + 4 * g + e] = s;
+        }
+      __syncthreads();
+      for (int r = threadIdx.x; r < BM; r += Tile::THREADS) {
+        float s = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WN; ++w) s += red[w * BM + r];
+        if (m0 + r < a.ldl) a.dbias[(int64_t)tn * a.ldl + m0 + r] = s;
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------ gradients
+// out[n][m] (m contiguous) = sum_k A(m,k) B(n,k), A with m contiguous: dx (A = W, B = dl) and dW (A = x, B = dl).
+struct GradArgs {
+  const void *A, *B;
+  int64_t lda, ldb;
+  int64_t M, N, K;
+  const int* list;       // of the rows that the backward takes, and their number:
+  const int* count;      // dx: row n of the result is row list[n] of out, N = count; dW: rows k of A, K = count
+  int tiles_m, tiles_n, splits;
+  void* out;             // of T, row stride ldo; or null: the fp32 sums go to acc
+  int64_t ldo;
+  float* acc;            // fp32 [splits][N][M], where the sums go (splits > 1) or are added up over pieces
+  int add;               // add what acc holds
+};
+
+template <typename T, int BM, int BN, int WM, int WN, bool BKC>
+__global__ __launch_bounds__(WM* WN * 64) void lce_grad_kernel(const GradArgs a) {
+  typedef pmg_tile<T, BM, BN, WM, WN, false, BKC, !BKC, false> Tile;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  int tm, tn;
+  pmg_tile_of(blockIdx.x, a.tiles_m, a.tiles_n, &tm, &tn);
+  const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
+  const int64_t rows = a.count[0], N = BKC ? rows : a.N, K = BKC ? a.K : rows;
+  if (n0 >= N) return;
+  const int64_t steps = (K + Tile::KSTEP - 1) / Tile::KSTEP, per = (steps + a.splits - 1) / a.splits * Tile::KSTEP;
+  const int64_t k0 = per * blockIdx.y, k1 = k0 + per < K ? k0 + per : K;
+  f32x4 acc[Tile::MI][Tile::NI];
+  Tile::run(acc, (lds_char*)smem, a.A, a.lda, a.list, m0, a.M, a.B, a.ldb, nullptr, n0, N, k0, k1);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t mw = m0 + (wave / WN) * (BM / WM) + 4 * (lane >> 4), nw = n0 + (wave % WN) * (BN / WN) + (lane & 15);
+  float* sums = a.acc ? a.acc + (int64_t)blockIdx.y * a.N * a.M : nullptr;
+  const bool als = (a.M & 3) == 0, alo = ((a.ldo & 3) == 0) && pmg_aligned4((const T*)a.out);
+#pragma unroll
+  for (int j = 0; j < Tile::NI; ++j) {
+    const int64_t n = nw + j * 16;
+    if (n >= N) continue;
+    const int64_t o = BKC && a.out ? a.list[n] : n;
+#pragma unroll
+    for (int i = 0; i < Tile::MI; ++i) {
+      const int64_t m = mw + i * 16;
+      if (m >= a.M) continue;
+      f32x4 x = acc[i][j];
+      float* s = sums + n * a.M + m;
+      if (a.add) x += pmg_load4(s, als, a.M - m);
+      if (a.out) pmg_store4((T*)a.out + o * a.ldo + m, x, alo, a.M - m);
+      else pmg_store4(s, x, als, a.M - m);
+    }
+  }
+}
+
+// out row r (list[r] with a list) = sum over the splits of acc[split][r], in order
+template <typename T>
+__global__ __launch_bounds__(256) void lce_join_kernel(const float* __restrict__ acc, int splits, int64_t rows, int64_t M,
+                                                       const int* list, const int* count, T* __restrict__ out, int64_t ldo) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, total = rows * M;
+  const int64_t r = i / M;
+  if (i >= total || (list && r >= count[0])) return;
+  float s = 0.0f;
+#pragma unroll 8
+  for (int k = 0; k < splits; ++k) s += acc[(int64_t)k * total + i];
+  out[(list ? list[r] : r) * ldo + (i - r * M)] = (T)s;
+}
+
+// db[v] = sum over the tiles of BN tokens
+template <typename T>
+__global__ __launch_bounds__(256) void lce_dbias_kernel(const float* __restrict__ part, int BN, const int* count, int64_t ldl,
+                                                        int64_t V, T* __restrict__ db) {
+  const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (v >= V) return;
+  const int tiles = (count[0] + BN - 1) / BN;
+  float s = 0.0f;
+#pragma unroll 8
+  for (int k = 0; k < tiles; ++k) s += part[(int64_t)k * ldl + v];
+  db[v] = (T)s;
+}
+
+// ------------------------------------------------------------------------------------------ rows
+// A workgroup's 1024 threads are `r` rows by 1024 / r groups; a group joins every (1024 / r)-th part of its row.
+struct RowArgs {
+  const float2* part;
+  const float* at_target;
+  int tiles;
+  int64_t N, V;
+  const void* targets;
+  int id_bits;
+  int64_t ignore;
+  const float* weight;   // [N] or null
+  float* lse;
+  float* nll;            // [N], weighted; null: not wanted
+  struct LossPart* sums; // [workgroups] or null
+  int rows;
+};
+
+struct LossPart {
+  double sum;
+  int64_t count;
+};
+
+// Sum over a workgroup of 1024; valid in thread 0.
+__device__ __forceinline__ LossPart block_sum(double s, int64_t c) {
+  __shared__ double ws[16];
+  __shared__ long long wc[16];
+  long long k = c;
+  for (int o = 32; o > 0; o >>= 1) {
+    s += __shfl_xor(s, o, 64);
+    k += __shfl_xor(k, o, 64);
+  }
+  if ((threadIdx.x & 63) == 0) {
+    ws[threadIdx.x >> 6] = s;
+    wc[threadIdx.x >> 6] = k;
+  }
+  __syncthreads();
+  LossPart p = {0.0, 0};
+  if (threadIdx.x == 0)
+    for (int w = 0; w < 16; ++w) {
+      p.sum += ws[w];
+      p.count += wc[w];
+    }
+  return p;
+}
+
+__global__ __launch_bounds__(1024) void lce_rows_kernel(const RowArgs a) {
+  __shared__ float2 red[1024];
+  const int r = threadIdx.x % a.rows, grp = threadIdx.x / a.rows, groups = 1024 / a.rows;
+  const int64_t n = (int64_t)blockIdx.x * a.rows + r;
+  float top = -__builtin_inff(), sum = 0.0f;
+  if (n < a.N) {
+#pragma unroll 4
+    for (int t = grp; t < a.tiles; t += groups) {
+      const float2 p = a.part[(int64_t)t * a.N + n];
+      const float m = fmaxf(top, p.x);
+      // below -inf there is nothing to rescale (and inf - inf would be NaN); a NaN sum stays
+      sum = (top == -__builtin_inff() ? sum : sum * expf(top - m)) + (p.x == -__builtin_inff() ? p.y : p.y * expf(p.x - m));
+      top = m;
+    }
+  }
+  red[threadIdx.x] = make_float2(top, sum);
+  for (int half = groups >> 1; half > 0; half >>= 1) {
+    __syncthreads();
+    if (grp < half) {
+      const float2 p = red[threadIdx.x], q = red[threadIdx.x + half * a.rows];
+      const float m = fmaxf(p.x, q.x);
+      const float s = (p.x == -__builtin_inff() ? p.y : p.y * expf(p.x - m)) + (q.x == -__builtin_inff() ? q.y : q.y * expf(q.x - m));
+      red[threadIdx.x] = make_float2(m, s);
+    }
+  }
+  float nll = 0.0f;
+  bool in = false;
+  if (grp == 0 && n < a.N) {
+    const float2 p = red[threadIdx.x];
+    const float lse = p.x + logf(p.y);
+    a.lse[n] = lse;
+    const int64_t t = target_of(a.targets, a.id_bits, n);
+    in = t != a.ignore;
+    if (in) nll = t >= 0 && t < a.V ? (lse - a.at_target[n]) * (a.weight ? a.weight[n] : 1.0f) : __builtin_nanf("");
+    if (a.nll) a.nll[n] = nll;
+  }
+  if (a.sums) {
+    const LossPart p = block_sum((double)nll, in);
+    if (threadIdx.x == 0) a.sums[blockIdx.x] = p;
+  }
+}
+
+// count[0] = rows with a target; loss[0] = sum of nll (mean: over those rows; 0 without any).  One workgroup
+// over the workgroups of the rows, sums in fp64, in one order.
+__global__ __launch_bounds__(1024) void lce_loss_kernel(const LossPart* __restrict__ sums, int n, int mean,
+                                                        float* __restrict__ loss, float* __restrict__ count) {
+  double s = 0.0;
+  int64_t c = 0;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < n; i += 1024) {
+    s += sums[i].sum;
+    c += sums[i].count;
+  }
+  const LossPart p = block_sum(s, c);
+  if (threadIdx.x == 0) {
+    loss[0] = (float)(mean ? (p.count > 0 ? p.sum / (double)p.count : 0.0) : p.sum);
+    count[0] = (float)p.count;
+  }
+}
+
+// The rows with a slope, in their order: counts per 1024 rows (WRITE false), their scan, the list (WRITE true).
+struct SlopeArgs {
+  const float *g_loss, *g_lse, *lse, *count, *weight;
+  int per_row, mean;
+  const void* targets;
+  int id_bits;
+  int64_t ignore, N, V;
+  int* first;            // [groups]: rows with a slope in a group, then before it
+  int groups;
+  Row* row;
+  int* list;
+  int* total;
+  uint8_t* used;         // [N]
+};
+
+__device__ __forceinline__ Row slope_of(const SlopeArgs& a, int64_t n) {
+  Row r = {0.0f, 0.0f, 0.0f, -1};
+  const int64_t t = target_of(a.targets, a.id_bits, n);
+  if (t != a.ignore && a.g_loss) {
+    r.c = a.g_loss[a.per_row ? n : 0] * (a.weight ? a.weight[n] : 1.0f);
+    if (a.mean) r.c /= a.count[0];
+    if (t >= 0 && t < a.V) r.target = (int)t;
+    else r.c = __builtin_nanf("");
+  }
+  r.a = r.c + (a.g_lse ? a.g_lse[n] : 0.0f);
+  return r;
+}
+
+template <bool WRITE> __global__ __launch_bounds__(1024) void lce_slopes_kernel(const SlopeArgs a) {
+  __shared__ int wsum[16];
+  const int64_t n = (int64_t)blockIdx.x * 1024 + threadIdx.x;
+  Row r = {0.0f, 0.0f, 0.0f, -1};
+  if (n < a.N) r = slope_of(a, n);
+  const bool used = r.a != 0.0f || r.c != 0.0f;
+  const uint64_t mask = __ballot(used);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (lane == 0) wsum[wave] = __popcll(mask);
+  __syncthreads();
+  int before = 0, all = 0;
+  for (int w = 0; w < 16; ++w) {
+    if (w < wave) before += wsum[w];
+    all += wsum[w];
+  }
+  if (!WRITE) {
+    if (threadIdx.x == 0) a.first[blockIdx.x] = all;
+    return;
+  }
+  const int base = a.groups > 1 ? a.first[blockIdx.x] : 0;
+  if (n < a.N) a.used[n] = used;
+  if (used) {
+    const int at = base + before + __popcll(mask & ((1ull << lane) - 1));
+    r.lse = a.lse[n];
+    a.row[at] = r;
+    a.list[at] = (int)n;
+  }
+  if (threadIdx.x == 0 && blockIdx.x == (unsigned)a.groups - 1) a.total[0] = base + all;
+}
+
+__global__ __launch_bounds__(1024) void lce_scan_kernel(int* __restrict__ first, int n) {
+  __shared__ int wsum[16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int carry = 0;
+  for (int base = 0; base < n; base += 1024) {
+    const int i = base + threadIdx.x, v = i < n ? first[i] : 0;
+    int inc = v;
+    for (int o = 1; o < 64; o <<= 1) {
+      const int u = __shfl_up(inc, o, 64);
+      if (lane >= o) inc += u;
+    }
+    if (lane == 63) wsum[wave] = inc;
+    __syncthreads();
+    int before = carry;
+    for (int w = 0; w < 16; ++w) {
+      if (w < wave) before += wsum[w];
+      carry += wsum[w];
+    }
+    if (i < n) first[i] = before + inc - v;
+    __syncthreads();
+  }
+}
+
+// zero rows of the gradient of hidden for the rows without a slope; a wave a row
+template <typename T>
+__global__ __launch_bounds__(256) void lce_zero_rows_kernel(const uint8_t* __restrict__ used, int64_t N, int64_t H,
+                                                            T* __restrict__ dx) {
+  const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (n >= N || used[n]) return;
+  const bool al = (H & 3) == 0 && pmg_aligned4(dx);
+  for (int64_t c = (threadIdx.x & 63) * 4; c < H; c += 256) pmg_store4(dx + n * H + c, f32x4{0.f, 0.f, 0.f, 0.f}, al, H - c);
+}
+
+// rows of `width` elements, `ld` apart, into rows of `wide` (a multiple of 16 bytes), zero behind the end
+template <typename T>
+__global__ __launch_bounds__(256) void lce_pack_kernel(const T* __restrict__ src, int64_t ld, int64_t rows, int64_t width,
+                                                       T* __restrict__ dst, int64_t wide) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= rows * wide) return;
+  const int64_t r = i / wide, c = i - r * wide;
+  dst[i] = c < width ? src[r * ld + c] : (T)0.0f;
+}
+
+// ------------------------------------------------------------------------------------------ host
+int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
+int64_t div_up(int64_t x, int64_t by) { return (x + by - 1) / by; }
+
+struct Shape {
+  int BM, BN, per_cu;  // per_cu: workgroups a CU's LDS holds
+};
+enum { S256, S128, S64, SN64, SM64, SK16W, SK16, SK32, SK64 };  // S: square, SN / SM: 64 of n / m, SK: few tokens
+constexpr Shape SHAPES[] = {{256, 256, 1}, {128, 128, 2}, {64, 64, 5}, {256, 64, 2}, {64, 256, 2},
+                            {128, 16, 4},  {64, 16, 8},   {128, 32, 4}, {128, 64, 3}};
+constexpr int CUS = 256;
+
+int64_t tiles_of(int s, int64_t M, int64_t N) { return div_up(M, SHAPES[s].BM) * div_up(N, SHAPES[s].BN); }
+
+// The tile shape whose rounds over the chip cost least: a round runs per_cu tiles on every CU.  The two larger
+// squares reach the same rate when they fill the chip, the small one about 0.6 of it.
+int best_square(int64_t M, int64_t N) {
+  int best = S256;
+  double least = 0;
+  for (int s = S256; s <= S64; ++s) {
+    const int64_t t = tiles_of(s, M, N);
+    const double rounds = (double)div_up(t, (int64_t)CUS * SHAPES[s].per_cu);
+    const double cost = rounds * SHAPES[s].per_cu * SHAPES[s].BM * SHAPES[s].BN * (s == S64 ? 1.6 : 1.0);
+    if (s == S256 || cost < least) {
+      best = s;
+      least = cost;
+    }
+  }
+  return best;
+}
+
+int logits_shape(int64_t V, int64_t N, bool backward) {
+  if (!backward && N <= 64) {
+    if (N <= 16) return div_up(V, 128) >= 3 * CUS ? SK16W : SK16;
+    return N <= 32 ? SK32 : SK64;
+  }
+  if (V <= 64) return div_up(N, 256) >= CUS ? SM64 : S64;
+  return best_square(V, N);
+}
+
+int dx_shape(int64_t H, int64_t N) { return best_square(H, N); }
+
+int dw_shape(int64_t H, int64_t V) {
+  if (V <= 64 && H >= 256) return SN64;
+  return best_square(H, V);
+}
+
+// Parts of a long sum when there are too few tiles for the chip; at least eight stages a part.
+int splits_of(int s, int64_t M, int64_t N, int64_t K, int kstep) {
+  const int64_t tiles = tiles_of(s, M, N), slots = (int64_t)CUS * SHAPES[s].per_cu;
+  if (tiles * 2 > slots) return 1;
+  int64_t want = slots / tiles;
+  const int64_t most = div_up(K, (int64_t)kstep * 8);
+  if (want > most) want = most;
+  return want < 1 ? 1 : want > 1024 ? 1024 : (int)want;
+}
+
+struct Problem {
+  int64_t N, V, H;
+  int dtype;
+  bool pack_x, pack_w;
+  int64_t Hp;       // hidden size of packed rows
+  size_t eb;
+  int kstep;
+};
+
+// Vocabulary entries of a backward piece: dl of a piece stays around 128 MB, which the chip's last-level cache
+// holds between the product that writes it and the two that read it.
+constexpr int64_t PIECE_BYTES = 128 << 20;
+int64_t piece_of(const Problem& p) {
+  if (p.V <= 256) return p.V;
+  int64_t v = PIECE_BYTES / (p.N * (int64_t)p.eb) / 256 * 256;
+  // at least a chip's worth of tiles of the logits' product
+  const int64_t fill = up(div_up((int64_t)CUS * 256, div_up(p.N, 256)), 256);
+  if (v < fill) v = fill;
+  if (v >= p.V) return p.V;
+  return up(div_up(p.V, div_up(p.V, v)), 256);
+}
+
+struct Layout {
+  size_t xp, wp, part, at, sums;                    // forward
+  size_t row, list, total, first, used, dl, dxacc, dwacc, dbias;  // backward
+  size_t bytes;
+};
+
+struct Taker {
+  size_t at = 0;
+  size_t operator()(size_t bytes) {
+    const size_t p = at;
+    at += (bytes + 255) & ~(size_t)255;
+    return p;
+  }
+};
+
+// Rows a workgroup of the joining kernel takes.  Few parts: rows side by side; few rows: threads side by side on the
+// parts of a row; 64 rows where there are as many, so that a wave reads neighbouring parts.
+int rows_of(int64_t N, int64_t tiles) {
+  int rows = 1;
+  while (rows < 1024 && rows < N && 1024 / rows > tiles) rows <<= 1;
+  while (rows < 64 && rows < N) rows <<= 1;
+  return rows;
+}
+
+Layout fwd_layout(const Problem& p) {
+  Layout L = {};
+  Taker take;
+  L.xp = take(p.pack_x ? (size_t)p.N * p.Hp * p.eb : 0);
+  L.wp = take(p.pack_w ? (size_t)p.V * p.Hp * p.eb : 0);
+  const int s = logits_shape(p.V, p.N, false);
+  L.part = take((size_t)div_up(p.V, SHAPES[s].BM) * p.N * sizeof(float2));
+  L.at = take((size_t)p.N * 4);
+  L.sums = take((size_t)div_up(p.N, rows_of(p.N, div_up(p.V, SHAPES[s].BM))) * sizeof(LossPart));
+  L.bytes = take.at + 256;
+  return L;
+}
+
+struct BwdPlan {
+  int64_t piece, ldl;
+  int s_dl, s_dx, s_dw, split_dx, split_dw;
+  int64_t pieces;
+};
+
+BwdPlan bwd_plan(const Problem& p) {
+  BwdPlan b;
+  b.piece = piece_of(p);
+  b.pieces = div_up(p.V, b.piece);
+  b.ldl = up(b.piece, 64);
+  b.s_dl = logits_shape(b.piece, p.N, true);
+  b.s_dx = dx_shape(p.H, p.N);
+  b.s_dw = dw_shape(p.H, b.piece);
+  b.split_dx = b.pieces == 1 ? splits_of(b.s_dx, p.H, p.N, b.piece, p.kstep) : 1;
+  b.split_dw = splits_of(b.s_dw, p.H, b.piece, p.N, p.kstep);
+  return b;
+}
+
+Layout bwd_layout(const Problem& p, const BwdPlan& b) {
+  Layout L = {};
+  Taker take;
+  L.xp = take(p.pack_x ? (size_t)p.N * p.Hp * p.eb : 0);
+  L.wp = take(p.pack_w ? (size_t)p.V * p.Hp * p.eb : 0);
+  L.row = take((size_t)p.N * sizeof(Row));
+  L.list = take((size_t)p.N * 4);
+  L.total = take(4);
+  L.first = take((size_t)div_up(p.N, 1024) * 4);
+  L.used = take((size_t)p.N);
+  L.dl = take((size_t)p.N * b.ldl * p.eb);
+  L.dxacc = take(b.pieces > 1 || b.split_dx > 1 ? (size_t)b.split_dx * p.N * p.H * 4 : 0);
+  L.dwacc = take(b.split_dw > 1 ? (size_t)b.split_dw * b.piece * p.H * 4 : 0);
+  L.dbias = take((size_t)div_up(p.N, SHAPES[b.s_dl].BN) * b.ldl * 4);
+  L.bytes = take.at + 256;
+  return L;
+}
+
+int problem_of(const pmg_linear_ce* a, Problem* p) {
+  if (a->N < 1 || a->V < 1 || a->H < 1 || a->N > 0x7fffff00 || a->V > 0x7fffff00 || a->H > 65536) return PMG_E_ARG;
+  if (a->dtype != PMG_F32 && a->dtype != PMG_BF16) return PMG_E_DTYPE;
+  if (a->id_bits != 32 && a->id_bits != 64) return PMG_E_DTYPE;
+  if (a->ld_hidden < a->H || a->ld_weight < a->H) return PMG_E_ARG;
+  if (a->reduction != PMG_REDUCE_NONE && a->reduction != PMG_REDUCE_SUM && a->reduction != PMG_REDUCE_MEAN) return PMG_E_ARG;
+  p->N = a->N; p->V = a->V; p->H = a->H; p->dtype = a->dtype;
+  p->eb = pmg_elem_bytes(a->dtype);
+  p->kstep = (int)(128 / p->eb);
+  const int64_t e16 = 16 / (int64_t)p->eb;
+  p->Hp = up(a->H, e16);
+  // 16-byte loads: rows that do not begin at multiples of 16 bytes, or whose end does not, are copied to rows that do
+  const bool tail = a->H % e16 != 0;
+  p->pack_x = tail || a->ld_hidden % e16 != 0 || ((uintptr_t)a->hidden & 15) != 0;
+  p->pack_w = tail || a->ld_weight % e16 != 0 || ((uintptr_t)a->weight & 15) != 0;
+  const size_t eb = p->eb;
+  if (((uintptr_t)a->hidden | (uintptr_t)a->weight | (uintptr_t)a->bias) & (eb - 1)) return PMG_E_ALIGN;
+  if (((uintptr_t)a->targets & (a->id_bits / 8 - 1)) || ((uintptr_t)a->row_weight & 3)) return PMG_E_ALIGN;
+  return PMG_OK;
+}
+
+template <typename T, int BM, int BN, int WM, int WN, bool BACKWARD>
+int launch_logits(const LogitArgs& a, hipStream_t st) {
+  typedef pmg_tile<T, BM, BN, WM, WN, true, true, false, BACKWARD> Tile;
+  static std::atomic<unsigned long long> done{0};
+  if (const hipError_t e = pmg_full_lds_once((const void*)&lce_logits_kernel<T, BM, BN, WM, WN, BACKWARD>, &done)) return (int)e;
+  hipLaunchKernelGGL((lce_logits_kernel<T, BM, BN, WM, WN, BACKWARD>), dim3((unsigned)((int64_t)a.tiles_m * a.tiles_n)),
+                     dim3(Tile::THREADS), Tile::LDS, st, a);
+  return (int)hipGetLastError();
+}
+
+template <typename T, bool BACKWARD> int logits(int s, LogitArgs a, hipStream_t st) {
+  a.tiles_m = (int)div_up(a.V, SHAPES[s].BM);
+  a.tiles_n = (int)div_up(a.N, SHAPES[s].BN);
+  if ((int64_t)a.tiles_m * a.tiles_n > 0x7fffffff) return PMG_E_ARG;
+  switch (s) {
+    case S256: return launch_logits<T, 256, 256, 2, 4, BACKWARD>(a, st);
+    case S128: return launch_logits<T, 128, 128, 2, 2, BACKWARD>(a, st);
+    case S64: return launch_logits<T, 64, 64, 2, 2, BACKWARD>(a, st);
+    case SM64: return launch_logits<T, 64, 256, 1, 4, BACKWARD>(a, st);
+  }
+  if constexpr (!BACKWARD) switch (s) {
+      case SK16W: return launch_logits<T, 128, 16, 2, 1, false>(a, st);
+      case SK16: return launch_logits<T, 64, 16, 2, 1, false>(a, st);
+      case SK32: return launch_logits<T, 128, 32, 2, 1, false>(a, st);
+      case SK64: return launch_logits<T, 128, 64, 2, 1, false>(a, st);
+    }
+  return PMG_E_ARG;
+}
+
+template <typename T, int BM, int BN, int WM, int WN, bool BKC> int launch_grad(const GradArgs& a, hipStream_t st) {
+  typedef pmg_tile<T, BM, BN, WM, WN, false, BKC, !BKC, false> Tile;
+  static std::atomic<unsigned long long> done{0};
+  if (const hipError_t e = pmg_full_lds_once((const void*)&lce_grad_kernel<T, BM, BN, WM, WN, BKC>, &done)) return (int)e;
+  hipLaunchKernelGGL((lce_grad_kernel<T, BM, BN, WM, WN, BKC>), dim3((unsigned)((int64_t)a.tiles_m * a.tiles_n), a.splits),
+                     dim3(Tile::THREADS), Tile::LDS, st, a);
+  return (int)hipGetLastError();
+}
+
+// The sums of a split go to acc and are joined into `out`.
+template <typename T, bool BKC> int grad(int s, GradArgs a, hipStream_t st) {
+  a.tiles_m = (int)div_up(a.M, SHAPES[s].BM);
+  a.tiles_n = (int)div_up(a.N, SHAPES[s].BN);
+  if ((int64_t)a.tiles_m * a.tiles_n > 0x7fffffff) return PMG_E_ARG;
+  void* out = a.out;
+  if (a.splits > 1) a.out = nullptr;
+  int rc = PMG_E_ARG;
+  switch (s) {
+    case S256: rc = launch_grad<T, 256, 256, 2, 4, BKC>(a, st); break;
+    case S128: rc = launch_grad<T, 128, 128, 2, 2, BKC>(a, st); break;
+    case S64: rc = launch_grad<T, 64, 64, 2, 2, BKC>(a, st); break;
+    case SN64:
+      if constexpr (!BKC) rc = launch_grad<T, 256, 64, 4, 1, BKC>(a, st);
+      break;
+  }
+  if (rc || a.splits == 1) return rc;
+  const int64_t total = a.N * a.M;
+  hipLaunchKernelGGL(lce_join_kernel<T>, dim3((unsigned)div_up(total, 256)), dim3(256), 0, st, a.acc, a.splits, a.N, a.M,
+                     BKC ? a.list : nullptr, a.count, (T*)out, a.ldo);
+  return (int)hipGetLastError();
+}
+
+template <typename T> int pack(const void* src, int64_t ld, int64_t rows, const Problem& p, void* dst, hipStream_t st) {
+  hipLaunchKernelGGL(lce_pack_kernel<T>, dim3((unsigned)div_up(rows * p.Hp, 256)), dim3(256), 0, st, (const T*)src, ld, rows, p.H,
+                     (T*)dst, p.Hp);
+  return (int)hipGetLastError();
+}
+
+// Operands as the tile product reads them
+template <typename T>
+int operands(const pmg_linear_ce* a, const Problem& p, const Layout& L, char* ws, LogitArgs* l, hipStream_t st) {
+  l->X = a->hidden; l->ldx = a->ld_hidden;
+  l->W = a->weight; l->ldw = a->ld_weight;
+  if (p.pack_x) {
+    if (const int rc = pack<T>(a->hidden, a->ld_hidden, p.N, p, ws + L.xp, st)) return rc;
+    l->X = ws + L.xp; l->ldx = p.Hp;
+  }
+  if (p.pack_w) {
+    if (const int rc = pack<T>(a->weight, a->ld_weight, p.V, p, ws + L.wp, st)) return rc;
+    l->W = ws + L.wp; l->ldw = p.Hp;
+  }
+  l->bias = a->bias;
+  l->N = p.N;
+  l->K = p.Hp;
+  l->scale = a->logit_scale;
+  l->targets = a->targets; l->id_bits = a->id_bits;
+  return PMG_OK;
+}
+
+template <typename T> int forward(const pmg_linear_ce* a, const Problem& p, char* ws, hipStream_t st) {
+  const Layout L = fwd_layout(p);
+  LogitArgs l = {};
+  if (const int rc = operands<T>(a, p, L, ws, &l, st)) return rc;
+  l.V = p.V;
+  l.v0 = 0;
+  l.part = (float2*)(ws + L.part);
+  l.at_target = (float*)(ws + L.at);
+  const int s = logits_shape(p.V, p.N, false);
+  if (const int rc = logits<T, false>(s, l, st)) return rc;
+  RowArgs r = {};
+  r.part = l.part;
+  r.at_target = l.at_target;
+  r.tiles = (int)div_up(p.V, SHAPES[s].BM);
+  r.N = p.N; r.V = p.V;
+  r.targets = a->targets; r.id_bits = a->id_bits; r.ignore = a->ignore_index;
+  r.weight = a->row_weight;
+  r.lse = a->lse;
+  const bool none = a->reduction == PMG_REDUCE_NONE;
+  r.nll = none ? a->loss : nullptr;
+  r.sums = none ? nullptr : (LossPart*)(ws + L.sums);
+  r.rows = rows_of(p.N, r.tiles);
+  const int groups = (int)div_up(p.N, r.rows);
+  hipLaunchKernelGGL(lce_rows_kernel, dim3((unsigned)groups), dim3(1024), 0, st, r);
+  if (!none)
+    hipLaunchKernelGGL(lce_loss_kernel, dim3(1), dim3(1024), 0, st, r.sums, groups, a->reduction == PMG_REDUCE_MEAN, a->loss,
+                       a->count);
+  return (int)hipGetLastError();
+}
+
+template <typename T> int backward(const pmg_linear_ce* a, const Problem& p, char* ws, hipStream_t st) {
+  const BwdPlan b = bwd_plan(p);
+  const Layout L = bwd_layout(p, b);
+  LogitArgs l = {};
+  if (const int rc = operands<T>(a, p, L, ws, &l, st)) return rc;
+  SlopeArgs sl = {};
+  sl.g_loss = a->grad_loss; sl.g_lse = a->grad_lse; sl.lse = a->lse; sl.count = a->count; sl.weight = a->row_weight;
+  sl.per_row = a->reduction == PMG_REDUCE_NONE;
+  sl.mean = a->reduction == PMG_REDUCE_MEAN;
+  sl.targets = a->targets; sl.id_bits = a->id_bits; sl.ignore = a->ignore_index;
+  sl.N = p.N; sl.V = p.V;
+  sl.first = (int*)(ws + L.first);
+  sl.groups = (int)div_up(p.N, 1024);
+  sl.row = (Row*)(ws + L.row);
+  sl.list = (int*)(ws + L.list);
+  sl.total = (int*)(ws + L.total);
+  sl.used = (uint8_t*)(ws + L.used);
+  if (sl.groups > 1) {
+    hipLaunchKernelGGL(lce_slopes_kernel<false>, dim3(sl.groups), dim3(1024), 0, st, sl);
+    hipLaunchKernelGGL(lce_scan_kernel, dim3(1), dim3(1024), 0, st, sl.first, sl.groups);
+  }
+  hipLaunchKernelGGL(lce_slopes_kernel<true>, dim3(sl.groups), dim3(1024), 0, st, sl);
+  if (a->grad_hidden)
+    hipLaunchKernelGGL(lce_zero_rows_kernel<T>, dim3((unsigned)div_up(p.N, 4)), dim3(256), 0, st, sl.used, p.N, p.H,
+                       (T*)a->grad_hidden);
+  l.row = sl.row;
+  l.list = sl.list;
+  l.count = sl.total;
+  l.dl = ws + L.dl;
+  l.ldl = b.ldl;
+  l.dbias = a->grad_bias ? (float*)(ws + L.dbias) : nullptr;
+  const char* W = (const char*)l.W;
+  const char* bias = (const char*)a->bias;
+  for (int64_t i = 0; i < b.pieces; ++i) {
+    const int64_t v0 = i * b.piece, v = v0 + b.piece < p.V ? b.piece : p.V - v0;
+    l.v0 = v0;
+    l.V = v;
+    l.W = W + v0 * l.ldw * (int64_t)p.eb;
+    l.bias = bias ? bias + v0 * (int64_t)p.eb : nullptr;
+    if (const int rc = logits<T, true>(b.s_dl, l, st)) return rc;
+    if (a->grad_bias)
+      hipLaunchKernelGGL(lce_dbias_kernel<T>, dim3((unsigned)div_up(v, 256)), dim3(256), 0, st, l.dbias,
+                         SHAPES[b.s_dl].BN, sl.total, b.ldl, v, (T*)a->grad_bias + v0);
+    if (a->grad_hidden) {
+      GradArgs g = {};
+      g.A = l.W; g.lda = l.ldw; g.M = p.H;
+      g.B = l.dl; g.ldb = b.ldl; g.N = p.N;
+      g.K = v;
+      g.list = sl.list;
+      g.count = sl.total;
+      g.splits = b.split_dx;
+      g.out = i == b.pieces - 1 ? a->grad_hidden : nullptr;
+      g.ldo = p.H;
+      g.acc = b.pieces > 1 || b.split_dx > 1 ? (float*)(ws + L.dxacc) : nullptr;
+      g.add = i > 0;
+      if (const int rc = grad<T, true>(b.s_dx, g, st)) return rc;
+    }
+    if (a->grad_weight) {
+      GradArgs g = {};
+      g.A = l.X; g.lda = l.ldx; g.M = p.H;
+      g.B = l.dl; g.ldb = b.ldl; g.N = v;
+      g.K = p.N;
+      g.list = sl.list;
+      g.count = sl.total;
+      g.splits = b.split_dw;
+      g.out = (T*)a->grad_weight + v0 * p.H;
+      g.ldo = p.H;
+      g.acc = b.split_dw > 1 ? (float*)(ws + L.dwacc) : nullptr;
+      if (const int rc = grad<T, false>(b.s_dw, g, st)) return rc;
+    }
+  }
+  return (int)hipGetLastError();
+}
+
+}  // namespace
+
+extern "C" int pmg_linear_ce_workspace(const pmg_linear_ce* a, int backward, size_t* out) {
+  if (!a || !out) return PMG_E_NULL;
+  Problem p;
+  if (const int rc = problem_of(a, &p)) return rc;
+  *out = backward ? bwd_layout(p, bwd_plan(p)).bytes : fwd_layout(p).bytes;
+  return PMG_OK;
+}
+
+extern "C" int pmg_linear_ce_fwd(const pmg_linear_ce* a, void* ws, pmg_stream stream) {
+  if (!a || !ws || !a->hidden || !a->weight || !a->targets || !a->loss || !a->lse) return PMG_E_NULL;
+  if (a->reduction != PMG_REDUCE_NONE && !a->count) return PMG_E_NULL;
+  Problem p;
+  if (const int rc = problem_of(a, &p)) return rc;
+  if (((uintptr_t)ws & 15) || (((uintptr_t)a->loss | (uintptr_t)a->lse | (uintptr_t)a->count) & 3)) return PMG_E_ALIGN;
+  hipStream_t st = (hipStream_t)stream;
+  return a->dtype == PMG_F32 ? forward<float>(a, p, (char*)ws, st) : forward<bf16_t>(a, p, (char*)ws, st);
+}
+
+extern "C" int pmg_linear_ce_bwd(const pmg_linear_ce* a, void* ws, pmg_stream stream) {
+  if (!a || !ws || !a->hidden || !a->weight || !a->targets || !a->lse) return PMG_E_NULL;
+  if (a->reduction == PMG_REDUCE_MEAN && !a->count) return PMG_E_NULL;
+  if (a->grad_bias && !a->bias) return PMG_E_NULL;
+  Problem p;
+  if (const int rc = problem_of(a, &p)) return rc;
+  if (((uintptr_t)ws & 15) || (((uintptr_t)a->grad_loss | (uintptr_t)a->grad_lse | (uintptr_t)a->lse | (uintptr_t)a->count) & 3))
+    return PMG_E_ALIGN;
+  if (((uintptr_t)a->grad_hidden | (uintptr_t)a->grad_weight | (uintptr_t)a->grad_bias) & (p.eb - 1)) return PMG_E_ALIGN;
+  if (!a->grad_hidden && !a->grad_weight && !a->grad_bias) return PMG_OK;
+  hipStream_t st = (hipStream_t)stream;
+  return a->dtype == PMG_F32 ? backward<float>(a, p, (char*)ws, st) : backward<bf16_t>(a, p, (char*)ws, st);
+}

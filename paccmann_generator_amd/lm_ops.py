@@ -2,6 +2,8 @@
 
     torch.ops.pmg.embedding     -> pmg_embedding_fwd   rows of a table by token id, scaled; differentiable
     torch.ops.pmg.embedding_bwd -> pmg_embedding_bwd   the gradient of the table, by sorted tokens
+    torch.ops.pmg.linear_cross_entropy     -> pmg_linear_ce_fwd   loss over a vocabulary, logits not kept; differentiable
+    torch.ops.pmg.linear_cross_entropy_bwd -> pmg_linear_ce_bwd   its gradients
     torch.ops.pmg.grad_norm     -> pmg_grad_norm       norm over many gradients
     torch.ops.pmg.clip_grad_norm_ -> pmg_grad_norm, pmg_grad_clip   and their scaling, in place
     torch.ops.pmg.adamw_step_   -> pmg_adamw_step      the Adam / AdamW update of many parameters
@@ -191,6 +193,160 @@ def embedding(weight: Tensor, tokens: Tensor, scale: float = 1.0, padding_idx: O
     if not trusted_tokens:
         check_ids(tokens, weight.shape[0], 'token ids')
     return torch.ops.pmg.embedding.default(weight, tokens, float(scale), -1 if padding_idx is None else int(padding_idx))
+
+
+# --------------------------------------------------------------------------- linear cross entropy
+_lib.define('linear_cross_entropy(Tensor hidden, Tensor weight, Tensor? bias, Tensor targets, Tensor? row_weight, '
+            'int ignore_index, float logit_scale, int reduction) -> (Tensor, Tensor, Tensor)')
+_lib.define('linear_cross_entropy_bwd(Tensor? grad_loss, Tensor? grad_lse, Tensor hidden, Tensor weight, Tensor? bias, '
+            'Tensor targets, Tensor? row_weight, Tensor lse, Tensor count, int ignore_index, float logit_scale, '
+            'int reduction, bool[3] wanted) -> (Tensor, Tensor, Tensor)')
+
+
+def _ce_struct(hidden, weight, bias, targets, row_weight, ignore_index, logit_scale, reduction):
+    """(arguments of the C call without the outputs, device index, tensors that must outlive the call)."""
+    tensors = [hidden, weight, targets, *(t for t in (bias, row_weight) if t is not None)]
+    index = _one_device(tensors)
+    if weight.dim() != 2 or weight.shape[0] == 0 or weight.shape[1] == 0:
+        raise _ffi.PmgError(f'pmg::linear_cross_entropy: weight must be [V, H], got {tuple(weight.shape)}')
+    V, H = weight.shape
+    if hidden.dim() < 1 or hidden.shape[-1] != H or hidden.shape[:-1] != targets.shape:
+        raise _ffi.PmgError(f'pmg::linear_cross_entropy: hidden [..., {H}] and targets [...] required, got '
+                            f'{tuple(hidden.shape)} and {tuple(targets.shape)}')
+    if hidden.dtype != weight.dtype or (bias is not None and bias.dtype != weight.dtype) or \
+            hidden.dtype not in (torch.float32, torch.bfloat16):
+        raise _ffi.PmgError('pmg::linear_cross_entropy: hidden, weight and bias must all be fp32 or all be bf16 (the '
+                            'slopes of the logits leave the range of fp16)')
+    if bias is not None and bias.shape != (V,):
+        raise _ffi.PmgError(f'pmg::linear_cross_entropy: bias must be [{V}], got {tuple(bias.shape)}')
+    if row_weight is not None and (row_weight.dtype != torch.float32 or row_weight.shape != targets.shape):
+        raise _ffi.PmgError('pmg::linear_cross_entropy: row_weight must be fp32, one value per target')
+    a = _ffi.PmgLinearCe()
+    x, ld_x = _rows(hidden, H)
+    w, ld_w = _rows(weight, H)
+    t = targets.contiguous()
+    b = bias.contiguous() if bias is not None else None
+    r = row_weight.contiguous() if row_weight is not None else None
+    a.N, a.V, a.H, a.dtype, a.id_bits = t.numel(), V, H, _dtype_code(weight), _id_bits(targets)
+    a.reduction, a.logit_scale, a.ignore_index, a.ld_hidden, a.ld_weight = reduction, logit_scale, ignore_index, ld_x, ld_w
+    a.hidden, a.weight, a.targets = x.data_ptr(), w.data_ptr(), t.data_ptr()
+    a.bias = b.data_ptr() if b is not None else None
+    a.row_weight = r.data_ptr() if r is not None else None
+    return a, index, (x, w, t, b, r)
+
+
+def _ce_workspace(a, backward: int, device) -> Tensor:
+    need = C.c_size_t(0)
+    _ffi.check(_ffi.lib.pmg_linear_ce_workspace(C.byref(a), backward, C.byref(need)), 'pmg_linear_ce_workspace')
+    return torch.empty(need.value, dtype=torch.uint8, device=device)
+
+
+def _ce_fwd(hidden, weight, bias, targets, row_weight, ignore_index, logit_scale, reduction):
+    a, index, keep = _ce_struct(hidden, weight, bias, targets, row_weight, ignore_index, logit_scale, reduction)
+    f32 = dict(dtype=torch.float32, device=hidden.device)
+    if a.N == 0:
+        return (torch.zeros(targets.shape if reduction == 0 else (), **f32), torch.zeros(targets.shape, **f32),
+                torch.zeros(() if reduction else (0,), **f32))
+    loss = torch.empty(targets.shape if reduction == 0 else (), **f32)
+    lse, count = torch.empty(targets.shape, **f32), torch.empty(() if reduction else (0,), **f32)
+    ws = _ce_workspace(a, 0, hidden.device)
+    a.loss, a.lse, a.count = loss.data_ptr(), lse.data_ptr(), count.data_ptr()
+    with _on(index) as stream:
+        rc = _ffi.lib.pmg_linear_ce_fwd(C.byref(a), ws.data_ptr(), stream)
+    _ffi.check(rc, 'pmg_linear_ce_fwd')
+    return loss, lse, count
+
+
+def _ce_bwd(grad_loss, grad_lse, hidden, weight, bias, targets, row_weight, lse, count, ignore_index, logit_scale, reduction,
+            wanted):
+    a, index, keep = _ce_struct(hidden, weight, bias, targets, row_weight, ignore_index, logit_scale, reduction)
+    dx = torch.empty(hidden.shape if wanted[0] else (0,), dtype=hidden.dtype, device=hidden.device)
+    dw = torch.empty(weight.shape if wanted[1] else (0,), dtype=weight.dtype, device=hidden.device)
+    db = torch.empty(bias.shape if wanted[2] else (0,), dtype=weight.dtype, device=hidden.device)
+    if a.N == 0:
+        return dx, dw.zero_(), db.zero_()
+    slopes = []
+    for name, g, like in (('grad_loss', grad_loss, () if reduction else targets.shape), ('grad_lse', grad_lse, targets.shape)):
+        if g is not None:
+            if g.shape != like:
+                raise _ffi.PmgError(f'pmg::linear_cross_entropy_bwd: {name} must be {tuple(like)}, got {tuple(g.shape)}')
+            g = g.to(torch.float32).contiguous()
+            slopes.append(g)
+            setattr(a, name, g.data_ptr())
+    if lse.dtype != torch.float32 or lse.shape != targets.shape or not lse.is_contiguous() or count.dtype != torch.float32:
+        raise _ffi.PmgError('pmg::linear_cross_entropy_bwd: lse and count must be those of the forward call')
+    _one_device([hidden, lse, count, *slopes])
+    a.lse, a.count = lse.data_ptr(), count.data_ptr()
+    if wanted[0]:
+        a.grad_hidden = dx.data_ptr()
+    if wanted[1]:
+        a.grad_weight = dw.data_ptr()
+    if wanted[2]:
+        a.grad_bias = db.data_ptr()
+    ws = _ce_workspace(a, 1, hidden.device)
+    with _on(index) as stream:
+        rc = _ffi.lib.pmg_linear_ce_bwd(C.byref(a), ws.data_ptr(), stream)
+    _ffi.check(rc, 'pmg_linear_ce_bwd')
+    return dx, dw, db
+
+
+def _ce_setup(ctx, inputs, output):
+    hidden, weight, bias, targets, row_weight, ctx.ignore_index, ctx.logit_scale, ctx.reduction = inputs
+    _, lse, count = output
+    ctx.set_materialize_grads(False)
+    ctx.save_for_backward(hidden, weight, bias, targets, row_weight, lse, count)
+
+
+def _ce_backward(ctx, g_loss, g_lse, g_count):
+    hidden, weight, bias, targets, row_weight, lse, count = ctx.saved_tensors
+    wanted = [ctx.needs_input_grad[0], ctx.needs_input_grad[1], bias is not None and ctx.needs_input_grad[2]]
+    if (g_loss is None and g_lse is None) or not any(wanted):
+        return (None,) * 8
+    got = torch.ops.pmg.linear_cross_entropy_bwd.default(g_loss, g_lse, hidden, weight, bias, targets, row_weight, lse, count,
+                                                         ctx.ignore_index, ctx.logit_scale, ctx.reduction, wanted)
+    return tuple(g if w else None for g, w in zip(got, wanted)) + (None,) * 5
+
+
+_lib.impl('linear_cross_entropy', _ce_fwd, 'CUDA')
+_lib.impl('linear_cross_entropy_bwd', _ce_bwd, 'CUDA')
+
+
+@torch.library.register_fake('pmg::linear_cross_entropy', lib=_lib)
+def _(hidden, weight, bias, targets, row_weight, ignore_index, logit_scale, reduction):
+    f32 = dict(dtype=torch.float32)
+    return (hidden.new_empty(targets.shape if reduction == 0 else (), **f32), hidden.new_empty(targets.shape, **f32),
+            hidden.new_empty(() if reduction else (0,), **f32))
+
+
+@torch.library.register_fake('pmg::linear_cross_entropy_bwd', lib=_lib)
+def _(grad_loss, grad_lse, hidden, weight, bias, targets, row_weight, lse, count, ignore_index, logit_scale, reduction, wanted):
+    return (hidden.new_empty(hidden.shape if wanted[0] else (0,)), weight.new_empty(weight.shape if wanted[1] else (0,)),
+            weight.new_empty((weight.shape[0],) if wanted[2] else (0,)))
+
+
+torch.library.register_autograd('pmg::linear_cross_entropy', _ce_backward, setup_context=_ce_setup, lib=_lib)
+
+
+def linear_cross_entropy(hidden: Tensor, weight: Tensor, targets: Tensor, bias: Optional[Tensor] = None,
+                         row_weight: Optional[Tensor] = None, ignore_index: int = -100, logit_scale: float = 1.0,
+                         reduction: str = 'mean', trusted_tokens: bool = False) -> Tuple[Tensor, Tensor]:
+    """(loss, lse) of ``logit_scale * (hidden @ weight.T + bias)`` against ``targets``, without keeping the logits.
+
+    ``hidden`` [..., H], ``weight`` [V, H] and ``bias`` [V] are all fp32 or all bf16; ``targets`` [...] int64 or int32.
+    The loss of a row is its negative log-probability times ``row_weight`` (fp32 [...], a reward say; it gets no
+    gradient) and 0 where the target is ``ignore_index``.  ``reduction``: 'none' ([...]), 'sum', or 'mean' over the rows
+    with a target (0 without any).  ``lse`` [...] is the log-sum-exp of every row's logits.  Differentiable through both
+    w.r.t. hidden, weight and bias: the logits are formed again, a piece of the vocabulary at a time.
+    ``trusted_tokens`` skips the range check of the targets, which synchronises (captured graphs need it skipped): a
+    target out of range then gives NaN."""
+    if reduction not in _ffi.PMG_REDUCE:
+        raise _ffi.PmgError(f'pmg::linear_cross_entropy: reduction must be none, sum or mean, got {reduction!r}')
+    _need_cuda([hidden, weight, targets, bias, row_weight])
+    if not trusted_tokens:
+        check_ids(targets, weight.shape[0], 'targets', ignore=int(ignore_index))
+    loss, lse, _ = torch.ops.pmg.linear_cross_entropy.default(hidden, weight, bias, targets, row_weight, int(ignore_index),
+                                                              float(logit_scale), _ffi.PMG_REDUCE[reduction])
+    return loss, lse
 
 
 # --------------------------------------------------------------------------------- norm and clipping

@@ -29,7 +29,7 @@ from torch import Tensor
 
 from . import _ffi
 from .lm_ops import (adamw_state, adamw_state_values, adamw_step, clip_grad_norm_, embedding,  # noqa: F401
-                     grad_norm)
+                     grad_norm, linear_cross_entropy)
 
 # Largest workspace one kernel call of the training pair may take; larger batches run as chunks whose
 # gradients accumulate (PMG_FLAG_ACCUMULATE).  At most 96 GiB of the 288 GB of HBM -- configs[3]
