@@ -100,6 +100,9 @@ int pmg_grad_norm_workspace(const int64_t* numel, int n, size_t* out);
 int pmg_grad_norm(const void* const* grads, const int64_t* numel, const int* dtype, int n, float* norm, void* ws,
                   pmg_stream stream);
 
+/* The refusals of pmg_grad_clip without its launch: 0 or a negative code. */
+int pmg_grad_clip_check(void* const* grads, const int64_t* numel, const int* dtype, int n, float max_norm);
+
 /* Every element of every tensor times min(1, max_norm / (norm[0] + 1e-6)), in place (what
  * clip_grad_norm_ of the reference's update does, reinforce_omics.py:336-340).  A NaN norm makes every
  * element NaN.  Tensors must not overlap. */

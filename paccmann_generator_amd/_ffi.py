@@ -22,6 +22,8 @@ PMG_ABI_VERSION = 3
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # PMG_LIB selects a tuning variant built by __graft_entry__.build(extra_flags=..., libname=...)
+# the PyTorch operators over include/pmg_lm.h (csrc/pmg_torch.cpp); links to lib/libpmg.so
+TORCH_LIB_PATH = os.path.join(_HERE, 'lib', 'libpmg_torch.so')
 LIB_PATH = os.environ.get('PMG_LIB') or os.path.join(_HERE, 'lib', 'libpmg.so')
 
 
@@ -98,6 +100,7 @@ LM_EXPORTS = {
     'pmg_linear_ce_bwd': [C.POINTER(PmgLinearCe), _P, _P],
     'pmg_grad_norm_workspace': [_P, _I, _SIZE],
     'pmg_grad_norm': [_P, _P, _P, _I, _P, _P, _P],
+    'pmg_grad_clip_check': [_P, _P, _P, _I, C.c_float],
     'pmg_grad_clip': [_P, _P, _P, _I, _P, C.c_float, _P],
     'pmg_adamw_step': [C.POINTER(PmgAdamw), _P, _P],
     'pmg_adamw_values': [_P, _P, _L, _I, _P, _P],
@@ -154,6 +157,9 @@ def _load():
 
 
 lib = _load()
+if not os.path.exists(TORCH_LIB_PATH):
+    raise ImportError(f'{TORCH_LIB_PATH} is missing: build it first (python -c "import __graft_entry__ as g; g.build()").')
+torch.ops.load_library(TORCH_LIB_PATH)
 
 
 class PmgError(RuntimeError):

@@ -441,23 +441,26 @@ extern "C" int pmg_grad_norm(const void* const* grads, const int64_t* numel, con
   return (int)hipGetLastError();
 }
 
-extern "C" int pmg_grad_clip(void* const* grads, const int64_t* numel, const int* dtype, int n, const float* norm,
-                             float max_norm, pmg_stream stream) {
-  if (!norm) return PMG_E_NULL;
+extern "C" int pmg_grad_clip_check(void* const* grads, const int64_t* numel, const int* dtype, int n, float max_norm) {
   if (!(max_norm > 0.0f)) return PMG_E_ARG;
   const int rc = grad_args_ok((const void* const*)grads, numel, dtype, n);
   if (rc) return rc;
   size_t need;
   if (const int e = pmg_grad_norm_workspace(numel, n, &need)) return e;  // chunks within a launch's reach
-  if (n > 0) {
-    Range* r = new (std::nothrow) Range[n];
-    if (!r) return PMG_E_ARG;
-    for (int i = 0; i < n; ++i)
-      r[i] = Range{(uintptr_t)grads[i], (uintptr_t)grads[i] + (size_t)numel[i] * pmg_elem_bytes(dtype[i]), numel[i] > 0};
-    const int ov = check_disjoint(r, n);
-    delete[] r;
-    if (ov) return ov;
-  }
+  if (n == 0) return PMG_OK;
+  Range* r = new (std::nothrow) Range[n];
+  if (!r) return PMG_E_ARG;
+  for (int i = 0; i < n; ++i)
+    r[i] = Range{(uintptr_t)grads[i], (uintptr_t)grads[i] + (size_t)numel[i] * pmg_elem_bytes(dtype[i]), numel[i] > 0};
+  const int ov = check_disjoint(r, n);
+  delete[] r;
+  return ov;
+}
+
+extern "C" int pmg_grad_clip(void* const* grads, const int64_t* numel, const int* dtype, int n, const float* norm,
+                             float max_norm, pmg_stream stream) {
+  if (!norm) return PMG_E_NULL;
+  if (const int rc = pmg_grad_clip_check(grads, numel, dtype, n, max_norm)) return rc;
   hipStream_t st = (hipStream_t)stream;
   const int chunk = norm_chunk(numel, n);
   batches<GradTable, GT_MAX>(

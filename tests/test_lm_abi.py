@@ -26,14 +26,14 @@ def test_header_compiles_as_plain_c_with_the_bound_layout(tmp_path):
     from paccmann_generator_amd import _ffi
     src = tmp_path / 't.c'
     src.write_text('#include "pmg_lm.h"\n#include <stdio.h>\n#include <stddef.h>\n'
-                   'int main(void){printf("%d %d %d\\n",(int)sizeof(pmg_adamw),(int)offsetof(pmg_adamw,step),'
+                   'int main(void){printf("%d %d %d %d %d\\n",(int)sizeof(pmg_linear_ce),(int)offsetof(pmg_linear_ce,grad_bias),(int)sizeof(pmg_adamw),(int)offsetof(pmg_adamw,step),'
                    '(int)offsetof(pmg_adamw,max_norm));return 0;}\n')
     exe = tmp_path / 't'
     subprocess.check_call(['gcc', '-std=c99', '-Wall', '-Werror', '-I', os.path.join(ROOT, 'include'), str(src), '-o',
                            str(exe)])
     got = [int(x) for x in subprocess.check_output([str(exe)]).split()]
-    a = _ffi.PmgAdamw
-    assert got == [C.sizeof(a), a.step.offset, a.max_norm.offset]
+    a, c = _ffi.PmgAdamw, _ffi.PmgLinearCe
+    assert got == [C.sizeof(c), c.grad_bias.offset, C.sizeof(a), a.step.offset, a.max_norm.offset]
 
 
 def test_embedding_refusals_and_workspace():
@@ -61,6 +61,39 @@ def test_embedding_refusals_and_workspace():
     assert lib.pmg_embedding_bwd_workspace(4, 9, 8, None) < 0
 
 
+def test_linear_ce_refusals_and_workspace():
+    from paccmann_generator_amd import _ffi
+    lib, size = _ffi.lib, C.c_size_t(0)
+
+    def args(**k):
+        a = _ffi.PmgLinearCe()
+        d = dict(N=40, V=90, H=16, dtype=0, id_bits=64, reduction=2, logit_scale=1.0, ignore_index=-100, ld_hidden=16, ld_weight=16,
+                 hidden=FAKE, weight=FAKE, targets=FAKE, loss=FAKE, lse=FAKE, count=FAKE, grad_loss=FAKE, grad_hidden=FAKE)
+        for name, x in {**d, **k}.items():
+            setattr(a, name, x)
+        return C.byref(a)
+
+    shapes = [dict(N=0), dict(V=0), dict(H=0), dict(H=1 << 17, ld_hidden=1 << 17, ld_weight=1 << 17), dict(dtype=2), dict(dtype=-1),
+              dict(id_bits=8), dict(ld_hidden=15), dict(ld_weight=3), dict(reduction=3), dict(hidden=FAKE + 2), dict(targets=FAKE + 4),
+              dict(row_weight=FAKE + 1), dict(bias=FAKE + 3)]
+    for k in shapes:
+        for rc in (lib.pmg_linear_ce_fwd(args(**k), FAKE, None), lib.pmg_linear_ce_bwd(args(**k), FAKE, None),
+                   lib.pmg_linear_ce_workspace(args(**k), 0, C.byref(size)), lib.pmg_linear_ce_workspace(args(**k), 1, C.byref(size))):
+            assert rc < 0 and len(lib.pmg_strerror(rc)) > 3, k
+    for k in (dict(hidden=None), dict(weight=None), dict(targets=None), dict(loss=None), dict(lse=None), dict(count=None), dict(loss=FAKE + 2)):
+        assert lib.pmg_linear_ce_fwd(args(**k), FAKE, None) < 0, k
+    for k in (dict(hidden=None), dict(lse=None), dict(count=None), dict(grad_bias=FAKE), dict(grad_weight=FAKE + 2), dict(grad_lse=FAKE + 2)):
+        assert lib.pmg_linear_ce_bwd(args(**k), FAKE, None) < 0, k
+    assert lib.pmg_linear_ce_fwd(args(), None, None) < 0 and lib.pmg_linear_ce_fwd(args(), FAKE + 8, None) < 0
+    assert lib.pmg_linear_ce_bwd(args(), FAKE + 4, None) < 0 and lib.pmg_linear_ce_workspace(None, 0, C.byref(size)) < 0
+    assert lib.pmg_linear_ce_bwd(args(grad_hidden=None), FAKE, None) == 0          # nothing wanted
+    # the backward's scratch holds a piece of the vocabulary, not all logits
+    for N, V, H in ((8192, 128000, 4096), (65536, 32000, 1024)):
+        k = dict(N=N, V=V, H=H, ld_hidden=H, ld_weight=H, dtype=1)
+        assert lib.pmg_linear_ce_workspace(args(**k), 1, C.byref(size)) == 0 and size.value < N * V
+        assert lib.pmg_linear_ce_workspace(args(**k), 0, C.byref(size)) == 0 and size.value < N * V // 8
+
+
 def test_norm_clip_and_update_refusals():
     from paccmann_generator_amd import _ffi
     lib, size = _ffi.lib, C.c_size_t(0)
@@ -73,8 +106,9 @@ def test_norm_clip_and_update_refusals():
     assert lib.pmg_grad_norm(ptr, numel, (C.c_int * 2)(0, 7), 2, FAKE, FAKE, None) < 0
     assert lib.pmg_grad_norm((C.c_void_p * 2)(FAKE, None), numel, dt, 2, FAKE, FAKE, None) < 0
     assert lib.pmg_grad_norm((C.c_void_p * 2)(FAKE + 2, FAKE), numel, dt, 2, FAKE, FAKE, None) < 0
+    assert lib.pmg_grad_clip_check(ptr, numel, dt, 2, 1.0) == 0 and lib.pmg_grad_clip(ptr, numel, dt, 2, None, 1.0, None) < 0
     for m in (0.0, -1.0, float('nan')):
-        assert lib.pmg_grad_clip(ptr, numel, dt, 2, FAKE, m, None) < 0
+        assert lib.pmg_grad_clip_check(ptr, numel, dt, 2, m) < 0 and lib.pmg_grad_clip(ptr, numel, dt, 2, FAKE, m, None) < 0
     rc = lib.pmg_grad_clip((C.c_void_p * 2)(FAKE, FAKE + 36), numel, dt, 2, FAKE, 1.0, None)
     assert rc < 0 and b'overlap' in lib.pmg_strerror(rc)
 
@@ -110,7 +144,7 @@ def test_norm_clip_and_update_refusals():
 def test_operators_are_registered_and_refuse_cpu_tensors():
     from torch._subclasses.fake_tensor import FakeTensorMode
     from paccmann_generator_amd import _ffi, ops
-    for name in ('embedding', 'embedding_bwd', 'grad_norm', 'clip_grad_norm_', 'adamw_step_', 'adamw_state_values'):
+    for name in ('embedding', 'embedding_bwd', 'linear_cross_entropy', 'linear_cross_entropy_bwd', 'grad_norm', 'clip_grad_norm_', 'adamw_step_', 'adamw_state_values'):
         assert str(getattr(torch.ops.pmg, name).default._schema).startswith(f'pmg::{name}(')
     p, g = torch.randn(6, 4), torch.randn(6, 4)
     m, v, _, _ = ops.adamw_state(p)
