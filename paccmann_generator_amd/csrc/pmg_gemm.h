@@ -50,10 +50,11 @@ __device__ __forceinline__ void pmg_load_lds16(const char* src, lds_char* dst) {
 
 // One operand's share of a stage: R rows of m (or n), 128 bytes of k.
 //   KC: k contiguous.  WAVES waves fill it, 1 KB an instruction.  LIST: rows by a list.
-template <typename T, int R, bool KC, int WAVES, bool LIST> struct pmg_operand {
+template <typename T, int R, bool KC, int WAVES, bool LIST, int KB> struct pmg_operand {
   static constexpr int E16 = 16 / sizeof(T);
-  static constexpr int KSTEP = 128 / sizeof(T);
-  static constexpr int BYTES = R * 128;
+  static constexpr int KSTEP = KB / sizeof(T);
+  static constexpr int BYTES = R * KB;
+  static constexpr int PER_ROW = KB / 16;         // 16-byte pieces of a row's k (k contiguous)
   static constexpr int CNT = BYTES / 1024 / WAVES;
   static constexpr int ROWB = R * sizeof(T);      // bytes of a row of k (m contiguous)
   static constexpr int PIECES = ROWB / 16;
@@ -65,30 +66,39 @@ template <typename T, int R, bool KC, int WAVES, bool LIST> struct pmg_operand {
     return (((k >> 2) & 3) << 2) & (PIECES - 1);
   }
 
+  static __device__ __forceinline__ int perm_k(int row) {  // of the pieces of a row (k contiguous)
+    return KB == 128 ? row & 7 : (row >> 2) & 3;
+  }
+
   const char* src[CNT];
   int64_t step;   // bytes from stage to stage
   int kofs[CNT];  // k of this lane's 16 bytes within a stage
-  // m contiguous with a list: the list's entries of the next stage, loaded a stage ahead
-  const int* list;
+  // m contiguous with a list: the entries of the rows that this wave fetches in the next stage
+  typedef const __attribute__((address_space(4))) int* scalar_list;
+  static constexpr int ROWS = KC ? 1 : CNT * 1024 / ROWB;  // of a wave
+  static constexpr int RPI = ROWS / CNT > 0 ? ROWS / CNT : 1;
+  scalar_list list;
   int64_t row_bytes;
-  int next[CNT];
+  int next[LIST && !KC ? ROWS : 1];
 
-  __device__ __forceinline__ void look_up(int64_t left) {
+  __device__ __forceinline__ void look_up() {
+    if constexpr (LIST && !KC) {
 #pragma unroll
-    for (int j = 0; j < CNT; ++j) next[j] = kofs[j] < left ? list[kofs[j]] : 0;
-    list += KSTEP;
+      for (int j = 0; j < ROWS; ++j) next[j] = list[j];
+      list += KSTEP;
+    }
   }
 
   // rows row0 .. of R_all (clamped: rows behind the end repeat the last one and are not stored), k from k0
-  __device__ __forceinline__ void init(const void* base, int64_t ld, const int* rows, int64_t row0, int64_t R_all, int64_t k0,
-                                       int64_t left) {
+  __device__ __forceinline__ void init(const void* base, int64_t ld, const int* rows, int64_t row0, int64_t R_all,
+                                       int64_t k0) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    step = KC ? 128 : (int64_t)KSTEP * ld * (int64_t)sizeof(T);
+    step = KC ? KB : (int64_t)KSTEP * ld * (int64_t)sizeof(T);
 #pragma unroll
     for (int j = 0; j < CNT; ++j) {
       const int byte = (wave * CNT + j) * 1024 + lane * 16;
       if (KC) {
-        const int row = byte >> 7, c = ((byte >> 4) & 7) ^ (row & 7);
+        const int row = byte / KB, c = ((byte >> 4) & (PER_ROW - 1)) ^ perm_k(row);
         int64_t r = row0 + row < R_all ? row0 + row : R_all - 1;
         if (LIST) r = rows[r];
         kofs[j] = c * E16;
@@ -103,31 +113,41 @@ template <typename T, int R, bool KC, int WAVES, bool LIST> struct pmg_operand {
     }
     if (LIST && !KC) {
       row_bytes = ld * (int64_t)sizeof(T);
-      list = rows + k0;
-      look_up(left);
+      list = (scalar_list)(rows + k0) + __builtin_amdgcn_readfirstlane(wave) * ROWS;
+      look_up();
     }
   }
 
-  // one stage into LDS at `dst`; `left`: k that remain (elements behind it read as zeros)
-  __device__ __forceinline__ void fetch(lds_char* dst, int64_t left) {
-    const int wave = threadIdx.x >> 6;
+  // one stage into LDS at `dst`.  PART: only `left` of its k exist (the others read as zeros), and the operand stays
+  // where it is; else it moves on by a stage.
+  template <bool PART> __device__ __forceinline__ void fetch(lds_char* dst, int left) {
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     lds_char* d = dst + wave * (CNT * 1024);
-    if (LIST && !KC) {
 #pragma unroll
-      for (int j = 0; j < CNT; ++j)
-        pmg_load_lds16(kofs[j] < left ? src[j] + next[j] * row_bytes : (const char*)&pmg_zero16, d + j * 1024);
-      look_up(left - KSTEP);
-      return;
-    }
-    if (left >= KSTEP) {
+    for (int j = 0; j < CNT; ++j) {
+      const char* from = src[j];
+      if constexpr (LIST && !KC) {
+        int64_t at = next[j * RPI] * row_bytes;
 #pragma unroll
-      for (int j = 0; j < CNT; ++j) {
-        pmg_load_lds16(src[j], d + j * 1024);
+        for (int r = 1; r < RPI; ++r) at = lane / (64 / RPI) == r ? next[j * RPI + r] * row_bytes : at;
+        from += at;
+      } else if (!PART) {
         src[j] += step;
       }
+      if (PART) from = kofs[j] < left ? from : (const char*)&pmg_zero16;
+      pmg_load_lds16(from, d + j * 1024);
+    }
+    if (LIST && !KC && !PART) look_up();
+  }
+
+  // behind a PART stage at the end of k: back by n stages
+  __device__ __forceinline__ void back(int64_t n) {
+    if constexpr (LIST && !KC) {
+      list -= (n + 1) * KSTEP;
+      look_up();
     } else {
 #pragma unroll
-      for (int j = 0; j < CNT; ++j) pmg_load_lds16(kofs[j] < left ? src[j] : (const char*)&pmg_zero16, d + j * 1024);
+      for (int j = 0; j < CNT; ++j) src[j] -= n * step;
     }
   }
 
@@ -137,7 +157,7 @@ template <typename T, int R, bool KC, int WAVES, bool LIST> struct pmg_operand {
     const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
     if (KC) {
       const int r = row + i;
-      return *(const __attribute__((address_space(3))) frag*)(s + r * 128 + (((kk * 4 + g) ^ (r & 7)) << 4));
+      return *(const __attribute__((address_space(3))) frag*)(s + r * KB + (((kk * 4 + g) ^ perm_k(r)) << 4));
     } else if constexpr (sizeof(T) == 2) {
       frag f;
 #pragma unroll
@@ -176,59 +196,113 @@ __device__ __forceinline__ void pmg_tile_of(int id, int tiles_m, int tiles_n, in
 }
 
 // acc[i][j]: the 16x16 tiles of wave (wm, wn)'s (BM / WM) x (BN / WN) part; k from k0 to k1 (k0 a multiple of the
-// stage).  Ends behind a barrier: LDS is free.
-template <typename T, int BM, int BN, int WM, int WN, bool AKC, bool BKC, bool ALIST, bool BLIST> struct pmg_tile {
+// stage).  Ends behind a barrier: LDS is free.  A list of rows of k may be read up to two stages beyond k1.
+template <typename T, int BM, int BN, int WM, int WN, bool AKC, bool BKC, bool ALIST, bool BLIST, int KB, int STAGES>
+struct pmg_tile {
   static constexpr int WAVES = WM * WN, THREADS = WAVES * 64;
   static constexpr int MI = BM / WM / 16, NI = BN / WN / 16;
-  typedef pmg_operand<T, BM, AKC, WAVES, ALIST> OpA;
-  typedef pmg_operand<T, BN, BKC, WAVES, BLIST> OpB;
+  typedef pmg_operand<T, BM, AKC, WAVES, ALIST, KB> OpA;
+  typedef pmg_operand<T, BN, BKC, WAVES, BLIST, KB> OpB;
   static constexpr int STAGE = OpA::BYTES + OpB::BYTES;
-  static constexpr int LDS = 2 * STAGE;
+  static constexpr int LDS = STAGES * STAGE;
   static constexpr int KSTEP = OpA::KSTEP;
+  static constexpr int LOADS = OpA::CNT + OpB::CNT;  // of a wave and stage
+  static constexpr int KK = KB / 64, HI = MI / 2;
+  static_assert(MI % 2 == 0, "two halves");
+
+  OpA a;
+  OpB b;
+  typename OpA::frag fa[2][HI];
+  typename OpB::frag fb[2][NI];
+  int rowA, rowB;
+
+  __device__ __forceinline__ void read_a(const lds_char* s, int half, int kk) {
+#pragma unroll
+    for (int i = 0; i < HI; ++i) fa[half][i] = OpA::read(s, rowA + (half * HI + i) * 16, kk);
+  }
+  __device__ __forceinline__ void read_b(const lds_char* s, int set, int kk) {
+#pragma unroll
+    for (int j = 0; j < NI; ++j) fb[set][j] = OpB::read(s + OpA::BYTES, rowB + j * 16, kk);
+  }
+  __device__ __forceinline__ void multiply(f32x4 (&acc)[MI][NI], int half, int set) {
+#pragma unroll
+    for (int i = 0; i < HI; ++i)
+#pragma unroll
+      for (int j = 0; j < NI; ++j) acc[half * HI + i][j] = pmg_frag<T>::mma(fa[half][i], fb[set][j], acc[half * HI + i][j]);
+  }
+
+  // One stage: it has landed (loads complete in order: those of the stages behind it may be under way), and every wave
+  // has read what it needs of the stage before, whose place (`put`) the next fetch takes.  The two places never are the
+  // same, which __restrict__ tells the compiler: else it would wait for the fetch before it reads.
+  // The fragments of a half are read while the half before them is multiplied: the first products here are those of the
+  // second half of the stage before.
+  template <bool FETCH>
+  __device__ __forceinline__ void stage(f32x4 (&acc)[MI][NI], lds_char* __restrict__ put, const lds_char* __restrict__ get) {
+    if (FETCH) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((STAGES - 2) * LOADS) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (FETCH) {
+      a.template fetch<false>(put, 0);
+      b.template fetch<false>(put + OpA::BYTES, 0);
+    }
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      read_b(get, 1, kk);
+      read_a(get, 0, kk);
+      multiply(acc, 1, 0);
+      read_a(get, 1, kk);
+      multiply(acc, 0, 1);
+#pragma unroll
+      for (int j = 0; j < NI; ++j) fb[0][j] = fb[1][j];
+    }
+  }
 
   static __device__ __forceinline__ void run(f32x4 (&acc)[MI][NI], lds_char* lds, const void* A, int64_t lda, const int* rows_a,
                                              int64_t m0, int64_t M, const void* B, int64_t ldb, const int* rows_b, int64_t n0,
                                              int64_t N, int64_t k0, int64_t k1) {
-    const int wave = threadIdx.x >> 6, rowA = (wave / WN) * (BM / WM), rowB = (wave % WN) * (BN / WN);
-    OpA a;
-    OpB b;
-    a.init(A, lda, rows_a, m0, M, k0, k1 - k0);
-    b.init(B, ldb, rows_b, n0, N, k0, k1 - k0);
+    const int wave = threadIdx.x >> 6;
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
       for (int j = 0; j < NI; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    int64_t left = k1 - k0;
-    if (left <= 0) return;
-    a.fetch(lds, left);
-    b.fetch(lds + OpA::BYTES, left);
-    int cur = 0;
-    while (left > 0) {
-      // this stage has landed, and every wave is done with the other one
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");
-      const lds_char* s = lds + cur * STAGE;
-      left -= KSTEP;
-      cur ^= 1;
-      if (left > 0) {
-        a.fetch(lds + cur * STAGE, left);
-        b.fetch(lds + cur * STAGE + OpA::BYTES, left);
-      }
-#pragma unroll
-      for (int kk = 0; kk < 2; ++kk) {
-        typename OpA::frag fa[MI];
-        typename OpB::frag fb[NI];
-#pragma unroll
-        for (int i = 0; i < MI; ++i) fa[i] = OpA::read(s, rowA + i * 16, kk);
-#pragma unroll
-        for (int j = 0; j < NI; ++j) fb[j] = OpB::read(s + OpA::BYTES, rowB + j * 16, kk);
-#pragma unroll
-        for (int i = 0; i < MI; ++i)
-#pragma unroll
-          for (int j = 0; j < NI; ++j) acc[i][j] = pmg_frag<T>::mma(fa[i], fb[j], acc[i][j]);
-      }
+    if (k1 <= k0) return;
+    pmg_tile t;
+    t.rowA = (wave / WN) * (BM / WM);
+    t.rowB = (wave % WN) * (BN / WN);
+    const int full = (int)((k1 - k0) / KSTEP), part = (int)((k1 - k0) - (int64_t)full * KSTEP);
+    const int steps = full + (part > 0);
+    // the stage that is not whole comes first: the loop below has whole ones only
+    t.a.init(A, lda, rows_a, m0, M, part ? k0 + (int64_t)full * KSTEP : k0);
+    t.b.init(B, ldb, rows_b, n0, N, part ? k0 + (int64_t)full * KSTEP : k0);
+    if (part) {
+      t.a.template fetch<true>(lds, part);
+      t.b.template fetch<true>(lds + OpA::BYTES, part);
+      t.a.back(full);
+      t.b.back(full);
     }
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s)
+      if (s < steps && (s > 0 || !part)) {
+        t.a.template fetch<false>(lds + s * STAGE, 0);
+        t.b.template fetch<false>(lds + s * STAGE + OpA::BYTES, 0);
+      }
+    __builtin_amdgcn_s_waitcnt(0);
+#pragma unroll
+    for (int i = 0; i < HI; ++i) t.fa[1][i] = typename OpA::frag{};
+#pragma unroll
+    for (int j = 0; j < NI; ++j) t.fb[0][j] = typename OpB::frag{};
+    int put = STAGES - 1, get = 0, s = 0;
+    for (; s < steps - (STAGES - 1); ++s) {
+      t.template stage<true>(acc, lds + put * STAGE, lds + get * STAGE);
+      put = put + 1 == STAGES ? 0 : put + 1;
+      get = get + 1 == STAGES ? 0 : get + 1;
+    }
+    for (; s < steps; ++s) {
+      t.template stage<false>(acc, lds, lds + get * STAGE);
+      get = get + 1 == STAGES ? 0 : get + 1;
+    }
+    t.multiply(acc, 1, 0);
     __syncthreads();
   }
 };

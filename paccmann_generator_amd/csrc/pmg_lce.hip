@@ -27,6 +27,27 @@ template <> __device__ __forceinline__ float exp_of<float>(float x) { return exp
 // behind bf16 operands the hardware's 2^x of a rounded product is exact enough: relative 2^-24 |x| log2(e)
 template <> __device__ __forceinline__ float exp_of<bf16_t>(float x) { return __builtin_amdgcn_exp2f(x * LOG2E); }
 
+// ------------------------------------------------------------------------------------------ tile shapes
+// Rows of m and n, waves along m and n, bytes of k a stage, stages, and workgroups that fit a CU.  Measured as plain
+// products with fp32 result, bf16 (operands with k / m and k / m contiguous), TFLOP/s: the large square 1152 / 1281 /
+// 1303 at 8192 x 8192 x 4096 (4096 x 8192 x 8192), the middle one 1067 / 1029 / 968; with two stages of 128 bytes the
+// large one gets 950 / 1007 / 1216, with four waves the middle one 906 / 989 / 929.  fp32: 142, of 157 the units give.
+struct Shape {
+  int BM, BN, WM, WN, KB, stages, per_cu;
+};
+enum { S256, S128, S64, SN64, SM64, SK16W, SK16, SK32, SK64 };  // S: square, SN / SM: 64 of n / m, SK: few tokens
+constexpr Shape SHAPES[] = {{256, 256, 2, 4, 64, 3, 1}, {128, 128, 2, 4, 128, 2, 2}, {64, 64, 2, 2, 128, 2, 5},
+                            {256, 64, 4, 1, 128, 2, 2}, {64, 256, 1, 4, 128, 2, 2},  {128, 16, 2, 1, 128, 2, 4},
+                            {64, 16, 2, 1, 128, 2, 8},  {128, 32, 2, 1, 128, 2, 4},  {128, 64, 2, 1, 128, 2, 3}};
+template <typename T, int S, bool AKC, bool BKC, bool ALIST, bool BLIST>
+using TileOf = pmg_tile<T, SHAPES[S].BM, SHAPES[S].BN, SHAPES[S].WM, SHAPES[S].WN, AKC, BKC, ALIST, BLIST, SHAPES[S].KB,
+                        SHAPES[S].stages>;
+template <int S> constexpr int THREADS_OF = SHAPES[S].WM * SHAPES[S].WN * 64;
+constexpr int LIST_SLACK = 256;  // entries behind the list of rows that a tile may read (and not use)
+
+// a value in memory that is the same for the whole launch, into a scalar register
+__device__ __forceinline__ int uniform_of(const int* p) { return *(const __attribute__((address_space(4))) int*)p; }
+
 // ------------------------------------------------------------------------------------------ arguments
 struct LogitArgs {
   const void *W, *X, *bias;
@@ -60,15 +81,16 @@ struct Row {
 };
 
 // ------------------------------------------------------------------------------------------ logits
-template <typename T, int BM, int BN, int WM, int WN, bool BACKWARD>
-__global__ __launch_bounds__(WM* WN * 64) void lce_logits_kernel(const LogitArgs a) {
-  typedef pmg_tile<T, BM, BN, WM, WN, true, true, false, BACKWARD> Tile;
+template <typename T, int S, bool BACKWARD>
+__global__ __launch_bounds__(THREADS_OF<S>) void lce_logits_kernel(const LogitArgs a) {
+  typedef TileOf<T, S, true, true, false, BACKWARD> Tile;
+  constexpr int BM = SHAPES[S].BM, BN = SHAPES[S].BN, WM = SHAPES[S].WM, WN = SHAPES[S].WN;
   constexpr int MI = Tile::MI, NI = Tile::NI;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   int tm, tn;
   pmg_tile_of(blockIdx.x, a.tiles_m, a.tiles_n, &tm, &tn);
   const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
-  const int64_t N = BACKWARD ? a.count[0] : a.N;
+  const int64_t N = BACKWARD ? uniform_of(a.count) : a.N;
   if (BACKWARD && n0 >= N) return;
   f32x4 acc[MI][NI];
   Tile::run(acc, (lds_char*)smem, a.W, a.ldw, nullptr, m0, a.V, a.X, a.ldx, a.list, n0, N, 0, a.K);
@@ -204,14 +226,15 @@ struct GradArgs {
   int add;               // add what acc holds
 };
 
-template <typename T, int BM, int BN, int WM, int WN, bool BKC>
-__global__ __launch_bounds__(WM* WN * 64) void lce_grad_kernel(const GradArgs a) {
-  typedef pmg_tile<T, BM, BN, WM, WN, false, BKC, !BKC, false> Tile;
+template <typename T, int S, bool BKC>
+__global__ __launch_bounds__(THREADS_OF<S>) void lce_grad_kernel(const GradArgs a) {
+  typedef TileOf<T, S, false, BKC, !BKC, false> Tile;
+  constexpr int BM = SHAPES[S].BM, BN = SHAPES[S].BN, WM = SHAPES[S].WM, WN = SHAPES[S].WN;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   int tm, tn;
   pmg_tile_of(blockIdx.x, a.tiles_m, a.tiles_n, &tm, &tn);
   const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
-  const int64_t rows = a.count[0], N = BKC ? rows : a.N, K = BKC ? a.K : rows;
+  const int64_t rows = uniform_of(a.count), N = BKC ? rows : a.N, K = BKC ? a.K : rows;
   if (n0 >= N) return;
   const int64_t steps = (K + Tile::KSTEP - 1) / Tile::KSTEP, per = (steps + a.splits - 1) / a.splits * Tile::KSTEP;
   const int64_t k0 = per * blockIdx.y, k1 = k0 + per < K ? k0 + per : K;
@@ -475,25 +498,19 @@ __global__ __launch_bounds__(256) void lce_pack_kernel(const T* __restrict__ src
 int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 int64_t div_up(int64_t x, int64_t by) { return (x + by - 1) / by; }
 
-struct Shape {
-  int BM, BN, per_cu;  // per_cu: workgroups a CU's LDS holds
-};
-enum { S256, S128, S64, SN64, SM64, SK16W, SK16, SK32, SK64 };  // S: square, SN / SM: 64 of n / m, SK: few tokens
-constexpr Shape SHAPES[] = {{256, 256, 1}, {128, 128, 2}, {64, 64, 5}, {256, 64, 2}, {64, 256, 2},
-                            {128, 16, 4},  {64, 16, 8},   {128, 32, 4}, {128, 64, 3}};
 constexpr int CUS = 256;
 
 int64_t tiles_of(int s, int64_t M, int64_t N) { return div_up(M, SHAPES[s].BM) * div_up(N, SHAPES[s].BN); }
 
-// The tile shape whose rounds over the chip cost least: a round runs per_cu tiles on every CU.  The two larger
-// squares reach the same rate when they fill the chip, the small one about 0.6 of it.
+// The square whose rounds over the chip cost least: a round runs per_cu tiles on every CU; against the large one's
+// rate the middle one has 0.85 of it, the small one 0.6.
 int best_square(int64_t M, int64_t N) {
   int best = S256;
   double least = 0;
   for (int s = S256; s <= S64; ++s) {
     const int64_t t = tiles_of(s, M, N);
     const double rounds = (double)div_up(t, (int64_t)CUS * SHAPES[s].per_cu);
-    const double cost = rounds * SHAPES[s].per_cu * SHAPES[s].BM * SHAPES[s].BN * (s == S64 ? 1.6 : 1.0);
+    const double cost = rounds * SHAPES[s].per_cu * SHAPES[s].BM * SHAPES[s].BN * (s == S256 ? 1.0 : s == S128 ? 1 / 0.85 : 1 / 0.6);
     if (s == S256 || cost < least) {
       best = s;
       least = cost;
@@ -612,7 +629,7 @@ Layout bwd_layout(const Problem& p, const BwdPlan& b) {
   L.xp = take(p.pack_x ? (size_t)p.N * p.Hp * p.eb : 0);
   L.wp = take(p.pack_w ? (size_t)p.V * p.Hp * p.eb : 0);
   L.row = take((size_t)p.N * sizeof(Row));
-  L.list = take((size_t)p.N * 4);
+  L.list = take(((size_t)p.N + LIST_SLACK) * 4);
   L.total = take(4);
   L.first = take((size_t)div_up(p.N, 1024) * 4);
   L.used = take((size_t)p.N);
@@ -645,13 +662,11 @@ int problem_of(const pmg_linear_ce* a, Problem* p) {
   return PMG_OK;
 }
 
-template <typename T, int BM, int BN, int WM, int WN, bool BACKWARD>
-int launch_logits(const LogitArgs& a, hipStream_t st) {
-  typedef pmg_tile<T, BM, BN, WM, WN, true, true, false, BACKWARD> Tile;
+template <typename T, int S, bool BACKWARD> int launch_logits(const LogitArgs& a, hipStream_t st) {
   static std::atomic<unsigned long long> done{0};
-  if (const hipError_t e = pmg_full_lds_once((const void*)&lce_logits_kernel<T, BM, BN, WM, WN, BACKWARD>, &done)) return (int)e;
-  hipLaunchKernelGGL((lce_logits_kernel<T, BM, BN, WM, WN, BACKWARD>), dim3((unsigned)((int64_t)a.tiles_m * a.tiles_n)),
-                     dim3(Tile::THREADS), Tile::LDS, st, a);
+  if (const hipError_t e = pmg_full_lds_once((const void*)&lce_logits_kernel<T, S, BACKWARD>, &done)) return (int)e;
+  hipLaunchKernelGGL((lce_logits_kernel<T, S, BACKWARD>), dim3((unsigned)((int64_t)a.tiles_m * a.tiles_n)), dim3(THREADS_OF<S>),
+                     (TileOf<T, S, true, true, false, BACKWARD>::LDS), st, a);
   return (int)hipGetLastError();
 }
 
@@ -660,26 +675,25 @@ template <typename T, bool BACKWARD> int logits(int s, LogitArgs a, hipStream_t 
   a.tiles_n = (int)div_up(a.N, SHAPES[s].BN);
   if ((int64_t)a.tiles_m * a.tiles_n > 0x7fffffff) return PMG_E_ARG;
   switch (s) {
-    case S256: return launch_logits<T, 256, 256, 2, 4, BACKWARD>(a, st);
-    case S128: return launch_logits<T, 128, 128, 2, 2, BACKWARD>(a, st);
-    case S64: return launch_logits<T, 64, 64, 2, 2, BACKWARD>(a, st);
-    case SM64: return launch_logits<T, 64, 256, 1, 4, BACKWARD>(a, st);
+    case S256: return launch_logits<T, S256, BACKWARD>(a, st);
+    case S128: return launch_logits<T, S128, BACKWARD>(a, st);
+    case S64: return launch_logits<T, S64, BACKWARD>(a, st);
+    case SM64: return launch_logits<T, SM64, BACKWARD>(a, st);
   }
   if constexpr (!BACKWARD) switch (s) {
-      case SK16W: return launch_logits<T, 128, 16, 2, 1, false>(a, st);
-      case SK16: return launch_logits<T, 64, 16, 2, 1, false>(a, st);
-      case SK32: return launch_logits<T, 128, 32, 2, 1, false>(a, st);
-      case SK64: return launch_logits<T, 128, 64, 2, 1, false>(a, st);
+      case SK16W: return launch_logits<T, SK16W, false>(a, st);
+      case SK16: return launch_logits<T, SK16, false>(a, st);
+      case SK32: return launch_logits<T, SK32, false>(a, st);
+      case SK64: return launch_logits<T, SK64, false>(a, st);
     }
   return PMG_E_ARG;
 }
 
-template <typename T, int BM, int BN, int WM, int WN, bool BKC> int launch_grad(const GradArgs& a, hipStream_t st) {
-  typedef pmg_tile<T, BM, BN, WM, WN, false, BKC, !BKC, false> Tile;
+template <typename T, int S, bool BKC> int launch_grad(const GradArgs& a, hipStream_t st) {
   static std::atomic<unsigned long long> done{0};
-  if (const hipError_t e = pmg_full_lds_once((const void*)&lce_grad_kernel<T, BM, BN, WM, WN, BKC>, &done)) return (int)e;
-  hipLaunchKernelGGL((lce_grad_kernel<T, BM, BN, WM, WN, BKC>), dim3((unsigned)((int64_t)a.tiles_m * a.tiles_n), a.splits),
-                     dim3(Tile::THREADS), Tile::LDS, st, a);
+  if (const hipError_t e = pmg_full_lds_once((const void*)&lce_grad_kernel<T, S, BKC>, &done)) return (int)e;
+  hipLaunchKernelGGL((lce_grad_kernel<T, S, BKC>), dim3((unsigned)((int64_t)a.tiles_m * a.tiles_n), a.splits), dim3(THREADS_OF<S>),
+                     (TileOf<T, S, false, BKC, !BKC, false>::LDS), st, a);
   return (int)hipGetLastError();
 }
 
@@ -692,11 +706,11 @@ template <typename T, bool BKC> int grad(int s, GradArgs a, hipStream_t st) {
   if (a.splits > 1) a.out = nullptr;
   int rc = PMG_E_ARG;
   switch (s) {
-    case S256: rc = launch_grad<T, 256, 256, 2, 4, BKC>(a, st); break;
-    case S128: rc = launch_grad<T, 128, 128, 2, 2, BKC>(a, st); break;
-    case S64: rc = launch_grad<T, 64, 64, 2, 2, BKC>(a, st); break;
+    case S256: rc = launch_grad<T, S256, BKC>(a, st); break;
+    case S128: rc = launch_grad<T, S128, BKC>(a, st); break;
+    case S64: rc = launch_grad<T, S64, BKC>(a, st); break;
     case SN64:
-      if constexpr (!BKC) rc = launch_grad<T, 256, 64, 4, 1, BKC>(a, st);
+      if constexpr (!BKC) rc = launch_grad<T, SN64, BKC>(a, st);
       break;
   }
   if (rc || a.splits == 1) return rc;
