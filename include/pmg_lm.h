@@ -36,7 +36,7 @@ int pmg_embedding_fwd(const void* weight, int64_t ld_weight, const void* ids, in
                       int dtype, float scale, void* out, pmg_stream stream);
 
 /* Bytes of scratch for pmg_embedding_bwd. */
-int pmg_embedding_bwd_workspace(int64_t N, int64_t V, int64_t E, size_t* out);
+int pmg_embedding_bwd_workspace(int64_t N, int64_t V, int64_t E, int dtype, size_t* out);
 
 /* grad_weight[v] = scale * (sum of grad[n] over the n with ids[n] == v), summed in fp32, rounded once; zero
  * for tokens that do not occur and for padding_idx (-1: none).  Every row is written; ids outside [0,V) add

@@ -93,7 +93,7 @@ EXPORTS = (
 _P, _I, _L, _SIZE = C.c_void_p, C.c_int, C.c_int64, C.POINTER(C.c_size_t)
 LM_EXPORTS = {
     'pmg_embedding_fwd': [_P, _L, _P, _I, _L, _L, _L, _I, C.c_float, _P, _P],
-    'pmg_embedding_bwd_workspace': [_L, _L, _L, _SIZE],
+    'pmg_embedding_bwd_workspace': [_L, _L, _L, _I, _SIZE],
     'pmg_embedding_bwd': [_P, _L, _P, _I, _L, _L, _L, _I, C.c_float, _L, _P, _P, _P],
     'pmg_linear_ce_workspace': [C.POINTER(PmgLinearCe), _I, _SIZE],
     'pmg_linear_ce_fwd': [C.POINTER(PmgLinearCe), _P, _P],

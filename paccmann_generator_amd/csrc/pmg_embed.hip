@@ -18,11 +18,12 @@ namespace {
 
 constexpr int THREADS = 256;
 constexpr int SMALL_N = 2048;   // one-workgroup sort: 66 steps in LDS, less than the radix passes' launches
-constexpr int TILE = 2048;      // keys a workgroup of the radix sort takes: 4 waves x 8 rounds x 64
+constexpr int ROUND = 256;      // keys a workgroup of the radix sort takes at a time: 4 waves x 64
 constexpr int MAX_BITS = 9;     // digit bits a pass: 17 bits of ids (128 k tokens) in two passes
 constexpr int MAX_BINS = 1 << MAX_BITS;
 constexpr int FILL_ROWS = 64;   // table rows a workgroup checks and zeroes
-constexpr int JOIN_THREADS = 1024;
+constexpr int JOIN_THREADS = 256;
+constexpr int HELD = 2048;      // sorted keys and positions that a workgroup of the reduction holds in LDS
 
 // ids outside [0, V) and the padding id sort behind all tokens and take no part
 template <typename I> __device__ __forceinline__ uint32_t key_of(I id, int64_t V, int64_t pad) {
@@ -104,16 +105,16 @@ struct FromKeys {
 };
 
 // count[digit * tiles + tile]
-template <typename Src>
+template <typename Src, int ROUNDS>
 __global__ __launch_bounds__(THREADS) void embed_count_kernel(const Src src, int64_t N, int shift, int bits, int tiles,
                                                               int* __restrict__ count) {
   __shared__ int bin[MAX_BINS];
   const int bins = 1 << bits;
   for (int b = threadIdx.x; b < bins; b += THREADS) bin[b] = 0;
   __syncthreads();
-  const int64_t base = (int64_t)blockIdx.x * TILE;
+  const int64_t base = (int64_t)blockIdx.x * (ROUNDS * ROUND);
 #pragma unroll
-  for (int r = 0; r < TILE / THREADS; ++r) {
+  for (int r = 0; r < ROUNDS; ++r) {
     const int64_t i = base + r * THREADS + threadIdx.x;
     if (i < N) atomicAdd(&bin[(src.key(i) >> shift) & (bins - 1)], 1);  // integers: any order, one result
   }
@@ -156,9 +157,9 @@ __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_wave_barrier();
 }
 
-// Stable: a wave takes 512 consecutive keys in rounds of 64; keys of one digit in a round are ranked by
+// Stable: a wave takes ROUNDS x 64 consecutive keys in rounds of 64; keys of one digit in a round are ranked by
 // lane, rounds and waves by running counts.
-template <typename Src>
+template <typename Src, int ROUNDS>
 __global__ __launch_bounds__(THREADS) void embed_scatter_kernel(const Src src, int64_t N, int shift, int bits, int tiles,
                                                                 const int* __restrict__ count,
                                                                 const int* __restrict__ total,
@@ -166,7 +167,6 @@ __global__ __launch_bounds__(THREADS) void embed_scatter_kernel(const Src src, i
   __shared__ int place[THREADS / 64][MAX_BINS];  // counts of a wave's keys, then where its next key of a digit goes
   __shared__ int start[MAX_BINS];
   __shared__ int wsum[THREADS / 64];
-  constexpr int ROUNDS = TILE / THREADS;
   const int bins = 1 << bits, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   for (int b = lane; b < bins; b += 64) place[wave][b] = 0;
   // first position of every digit: exclusive scan of the totals
@@ -183,7 +183,7 @@ __global__ __launch_bounds__(THREADS) void embed_scatter_kernel(const Src src, i
     carry += (wsum[0] + wsum[1]) + (wsum[2] + wsum[3]);
     __syncthreads();
   }
-  const int64_t base = (int64_t)blockIdx.x * TILE + wave * (ROUNDS * 64) + lane;
+  const int64_t base = (int64_t)blockIdx.x * (ROUNDS * ROUND) + wave * (ROUNDS * 64) + lane;
   uint32_t key[ROUNDS];
   uint64_t same[ROUNDS];
 #pragma unroll
@@ -267,16 +267,29 @@ __global__ __launch_bounds__(THREADS) void embed_reduce_kernel(const ReduceArgs 
         for (int64_t c = lane * VEC; c < a.E; c += 64 * VEC) z.store(dW + (v0 + r) * a.E + c, alo, a.E - c);
     return;
   }
+  // the workgroup's keys and positions, and the keys next to them
+  __shared__ uint32_t key[HELD + 2], pos[HELD];
+  const int per = THREADS / a.tpr * a.chunk;
+  const int64_t first = (int64_t)blockIdx.x * per;
+  for (int i = threadIdx.x; i < per + 2; i += THREADS) {
+    const int64_t p = first + i - 1;
+    key[i] = p >= 0 && p < a.N ? a.keys[p] : ~0u;
+    if (i >= 1 && i <= per && p < a.N) pos[i - 1] = a.pos[p];
+  }
+  __syncthreads();
   const int64_t c = ((int64_t)blockIdx.y * a.tpr + (threadIdx.x & (a.tpr - 1))) * VEC;
-  const int64_t ch = (int64_t)blockIdx.x * (THREADS / a.tpr) + threadIdx.x / a.tpr;
+  const int grp = threadIdx.x / a.tpr;
+  const int64_t ch = (int64_t)blockIdx.x * (THREADS / a.tpr) + grp;
   if (c >= a.E || ch >= a.chunks) return;
   const bool ali = pmg_rows_aligned16(g, a.ldg), alp = (a.E & 3) == 0;
-  const int64_t lo = ch * a.chunk, hi = lo + a.chunk < a.N ? lo + a.chunk : a.N;
+  const int lo = grp * a.chunk, n = (int)(a.N - ch * a.chunk < a.chunk ? a.N - ch * a.chunk : a.chunk);
+  const uint32_t* k = key + 1 + lo;  // k[-1] and k[n]: the neighbours
+  const uint32_t* at = pos + lo;
   float acc[VEC];
 #pragma unroll
   for (int j = 0; j < VEC; ++j) acc[j] = 0.0f;
-  uint32_t cur = a.keys[lo];
-  bool before = lo > 0 && a.keys[lo - 1] == cur;
+  uint32_t cur = k[0];
+  bool before = k[-1] == cur;
   auto put_part = [&](int slot) {
     float* p = a.part + (ch * 2 + slot) * a.E + c;
 #pragma unroll
@@ -290,37 +303,48 @@ __global__ __launch_bounds__(THREADS) void embed_reduce_kernel(const ReduceArgs 
     for (int j = 0; j < VEC; ++j) y.x[j] = acc[j] * a.scale;
     y.store(dW + (int64_t)cur * a.E + c, alo, a.E - c);
   };
-  for (int64_t i = lo; i < hi; i += U) {
-    pmg_vec16<T> x[U];
-    uint32_t k[U];
+  typedef typename pmg_vec16<T>::vec vec;
+  vec x[2][U];
+  auto load = [&](vec(&v)[U], int i) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (i + u < n && k[i + u] < (uint32_t)a.V) v[u] = pmg_vec16<T>::raw(g + (int64_t)at[i + u] * a.ldg + c, ali, a.E - c);
+  };
+  // false: what follows takes no part (dropped positions sort last)
+  auto add = [&](const vec(&v)[U], int i) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      k[u] = i + u < hi ? a.keys[i + u] : (uint32_t)a.V;
-      if (k[u] < (uint32_t)a.V) x[u].load(g + (int64_t)a.pos[i + u] * a.ldg + c, ali, a.E - c);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (i + u < hi) {
-        if (k[u] != cur) {
+      if (i + u < n) {
+        const uint32_t q = k[i + u];
+        if (q != cur) {
           if (before) put_part(0);
           else put_row();
           before = false;
-          cur = k[u];
+          cur = q;
 #pragma unroll
           for (int j = 0; j < VEC; ++j) acc[j] = 0.0f;
         }
-        if (cur >= (uint32_t)a.V) return;  // dropped positions sort last
+        if (cur >= (uint32_t)a.V) return false;
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) acc[j] += x[u].x[j];
+        for (int j = 0; j < VEC; ++j) acc[j] += (float)v[u][j];
       }
     }
+    return true;
+  };
+  load(x[0], 0);
+  for (int i = 0; i < n; i += 2 * U) {  // the rows of one set are under way while the other is added up
+    load(x[1], i + U);
+    if (!add(x[0], i)) return;
+    load(x[0], i + 2 * U);
+    if (!add(x[1], i + U)) return;
   }
   if (before) put_part(0);
-  else if (hi < a.N && a.keys[hi] == cur) put_part(1);
+  else if (k[n] == cur) put_part(1);
   else put_row();
 }
 
-// One workgroup a chunk and column block; only a chunk whose last run begins in it and goes on has work: the
+// One workgroup a chunk and column block; only a chunk whose last run begins in it and goes on has work (most do where
+// tokens are frequent, with two or three parts each: small workgroups, 43 us with 1024 threads at 32767 x 2048): the
 // parts of the run are dealt to the workgroup's groups of tpr threads in turn, and the groups' sums are
 // added in order.
 template <typename T>
@@ -332,14 +356,20 @@ __global__ __launch_bounds__(JOIN_THREADS) void embed_join_kernel(const ReduceAr
   const uint32_t cur = a.keys[hi];
   if (cur >= (uint32_t)a.V || a.keys[hi - 1] != cur) return;
   if (a.keys[lo] == cur && lo > 0 && a.keys[lo - 1] == cur) return;  // began earlier: another chunk's run
-  // first position behind the run
-  int64_t l = hi, h = a.N;
-  while (l < h) {
-    const int64_t mid = (l + h) >> 1;
-    if (a.keys[mid] <= cur) l = mid + 1;
-    else h = mid;
+  // the last chunk that begins inside the run: all threads look at the chunks behind this one
+  __shared__ int ends;
+  int64_t last = ch + 1;
+  for (int64_t base = ch + 1;; base += JOIN_THREADS) {
+    if (threadIdx.x == 0) ends = JOIN_THREADS;
+    __syncthreads();
+    const int64_t k = base + threadIdx.x;
+    if (k >= a.chunks || a.keys[k * a.chunk] != cur) atomicMin(&ends, (int)threadIdx.x);
+    __syncthreads();
+    const int e = ends;
+    last = base + e - 1;
+    if (e < JOIN_THREADS) break;
+    __syncthreads();
   }
-  const int64_t last = (l - 1) / a.chunk;  // chunk of the run's last position
   const int groups = JOIN_THREADS / a.tpr, grp = threadIdx.x / a.tpr, t = threadIdx.x & (a.tpr - 1);
   const int64_t c = ((int64_t)blockIdx.y * a.tpr + t) * VEC;
   const bool alp = (a.E & 3) == 0;
@@ -347,8 +377,8 @@ __global__ __launch_bounds__(JOIN_THREADS) void embed_join_kernel(const ReduceAr
 #pragma unroll
   for (int j = 0; j < VEC; ++j) acc[j] = 0.0f;
   if (c < a.E) {
-#pragma unroll 4
-    for (int64_t k = ch + grp; k <= last; k += groups) {
+#pragma unroll 16
+    for (int64_t k = ch + grp; k <= last; k += groups) {  // long runs: many loads under way
       const float* p = a.part + (k * 2 + (k == ch ? 1 : 0)) * a.E + c;
 #pragma unroll
       for (int j = 0; j < VEC; j += 4) {
@@ -384,9 +414,9 @@ int threads_per_row(int64_t E, int vec) {  // a power of two up to a wave
 
 // Sorted positions a chunk: short where there are few positions, so that a thousand chunks share the work;
 // 64 at most, so that the partial rows stay a small part of what is read.
-int chunk_of(int64_t N) {
+int chunk_of(int64_t N, int tpr) {
   int c = 8;
-  while (c < 64 && N / c > 1024) c <<= 1;
+  while (c < 64 && N / c > 1024 && c * 2 * (THREADS / tpr) <= HELD) c <<= 1;
   return c;
 }
 
@@ -399,10 +429,10 @@ int key_bits(int64_t V) {  // keys 0 .. V
 struct BwdLayout {
   size_t keys[2], pos[2], count, total, part, bytes;
   int64_t tiles, chunks;
-  int chunk;
+  int chunk, tpr, rounds;
 };
 
-BwdLayout bwd_layout(int64_t N, int64_t V, int64_t E) {
+BwdLayout bwd_layout(int64_t N, int64_t E, int dtype) {
   BwdLayout L;
   size_t at = 0;
   auto take = [&](size_t bytes) {
@@ -410,8 +440,11 @@ BwdLayout bwd_layout(int64_t N, int64_t V, int64_t E) {
     at += (bytes + 255) & ~(size_t)255;
     return p;
   };
-  L.tiles = (N + TILE - 1) / TILE;
-  L.chunk = chunk_of(N);
+  // rounds of 256 keys a workgroup of the sort: fewer where there would be few workgroups
+  L.rounds = N >= 256 * 2048 ? 8 : 2;
+  L.tiles = (N + L.rounds * ROUND - 1) / (L.rounds * ROUND);
+  L.tpr = threads_per_row(E, 16 / (int)pmg_elem_bytes(dtype));
+  L.chunk = chunk_of(N, L.tpr);
   L.chunks = (N + L.chunk - 1) / L.chunk;
   const bool small = N <= SMALL_N;
   for (int i = 0; i < 2; ++i) {
@@ -422,12 +455,11 @@ BwdLayout bwd_layout(int64_t N, int64_t V, int64_t E) {
   L.total = take(small ? 0 : MAX_BINS * 4);
   L.part = take((size_t)L.chunks * 2 * (size_t)E * 4);
   L.bytes = at ? at : 256;
-  (void)V;
   return L;
 }
 
 int embed_args_ok(int64_t N, int64_t V, int64_t E, int dtype, int id_bits) {
-  if (N < 0 || V < 1 || E < 1 || N > 0x7fffffff - TILE || V > 0x7ffffffe || E > ((int64_t)1 << 22)) return PMG_E_ARG;
+  if (N < 0 || V < 1 || E < 1 || N > 0x7fffffff - 8 * ROUND || V > 0x7ffffffe || E > ((int64_t)1 << 22)) return PMG_E_ARG;
   if (!pmg_dtype_ok(dtype)) return PMG_E_DTYPE;
   if (id_bits != 32 && id_bits != 64) return PMG_E_DTYPE;
   return PMG_OK;
@@ -448,14 +480,19 @@ int fwd(const void* W, int64_t ldw, const void* ids, int64_t N, int64_t V, int64
   return (int)hipGetLastError();
 }
 
-template <typename Src>
-void radix_pass(const Src& src, int64_t N, int shift, int bits, const BwdLayout& L, char* ws, int to, hipStream_t st) {
+template <typename Src, int ROUNDS>
+void radix_pass_of(const Src& src, int64_t N, int shift, int bits, const BwdLayout& L, char* ws, int to, hipStream_t st) {
   int *count = (int*)(ws + L.count), *total = (int*)(ws + L.total);
   const dim3 grid((unsigned)L.tiles), block(THREADS);
-  hipLaunchKernelGGL(embed_count_kernel<Src>, grid, block, 0, st, src, N, shift, bits, (int)L.tiles, count);
+  hipLaunchKernelGGL((embed_count_kernel<Src, ROUNDS>), grid, block, 0, st, src, N, shift, bits, (int)L.tiles, count);
   hipLaunchKernelGGL(embed_scan_kernel, dim3(1u << bits), block, 0, st, count, (int)L.tiles, total);
-  hipLaunchKernelGGL(embed_scatter_kernel<Src>, grid, block, 0, st, src, N, shift, bits, (int)L.tiles, count, total,
+  hipLaunchKernelGGL((embed_scatter_kernel<Src, ROUNDS>), grid, block, 0, st, src, N, shift, bits, (int)L.tiles, count, total,
                      (uint32_t*)(ws + L.keys[to]), (uint32_t*)(ws + L.pos[to]));
+}
+template <typename Src>
+void radix_pass(const Src& src, int64_t N, int shift, int bits, const BwdLayout& L, char* ws, int to, hipStream_t st) {
+  if (L.rounds == 8) radix_pass_of<Src, 8>(src, N, shift, bits, L, ws, to, st);
+  else radix_pass_of<Src, 2>(src, N, shift, bits, L, ws, to, st);
 }
 
 // Returns which of the two key buffers holds the sorted keys.
@@ -481,8 +518,9 @@ int sort_ids(const I* ids, int64_t N, int64_t V, int64_t pad, const BwdLayout& L
 template <typename T>
 int bwd(const void* g, int64_t ldg, const void* ids, int id_bits, int64_t N, int64_t V, int64_t E, float scale, int64_t pad,
         void* dW, char* ws, hipStream_t st) {
-  const BwdLayout L = bwd_layout(N, V, E);
-  const int tpr = threads_per_row(E, pmg_vec16<T>::N);
+  const int dtype = sizeof(T) == 4 ? PMG_F32 : PMG_BF16;
+  const BwdLayout L = bwd_layout(N, E, dtype);
+  const int tpr = L.tpr;
   const int64_t cols = (E + (int64_t)tpr * pmg_vec16<T>::N - 1) / ((int64_t)tpr * pmg_vec16<T>::N);
   if (cols > 65535) return PMG_E_ARG;
   int at = 0;
@@ -519,11 +557,11 @@ extern "C" int pmg_embedding_fwd(const void* weight, int64_t ld_weight, const vo
   return w ? fwd<f16_t, int64_t>(weight, ld_weight, ids, N, V, E, scale, out, st) : fwd<f16_t, int32_t>(weight, ld_weight, ids, N, V, E, scale, out, st);
 }
 
-extern "C" int pmg_embedding_bwd_workspace(int64_t N, int64_t V, int64_t E, size_t* out) {
+extern "C" int pmg_embedding_bwd_workspace(int64_t N, int64_t V, int64_t E, int dtype, size_t* out) {
   if (!out) return PMG_E_NULL;
-  const int rc = embed_args_ok(N, V, E, PMG_F32, 64);
+  const int rc = embed_args_ok(N, V, E, dtype, 64);
   if (rc) return rc;
-  *out = bwd_layout(N, V, E).bytes;
+  *out = bwd_layout(N, E, dtype).bytes;
   return PMG_OK;
 }
 

@@ -235,8 +235,8 @@ struct pmg_tile {
   // has read what it needs of the stage before, whose place (`put`) the next fetch takes.  The two places never are the
   // same, which __restrict__ tells the compiler: else it would wait for the fetch before it reads.
   // The fragments of a half are read while the half before them is multiplied: the first products here are those of the
-  // second half of the stage before.
-  template <bool FETCH>
+  // second half of the stage before (none in the FIRST one).
+  template <bool FETCH, bool FIRST>
   __device__ __forceinline__ void stage(f32x4 (&acc)[MI][NI], lds_char* __restrict__ put, const lds_char* __restrict__ get) {
     if (FETCH) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((STAGES - 2) * LOADS) : "memory");
     else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
@@ -250,7 +250,7 @@ struct pmg_tile {
     for (int kk = 0; kk < KK; ++kk) {
       read_b(get, 1, kk);
       read_a(get, 0, kk);
-      multiply(acc, 1, 0);
+      if (!FIRST || kk > 0) multiply(acc, 1, 0);
       read_a(get, 1, kk);
       multiply(acc, 0, 1);
 #pragma unroll
@@ -288,18 +288,20 @@ struct pmg_tile {
         t.b.template fetch<false>(lds + s * STAGE + OpA::BYTES, 0);
       }
     __builtin_amdgcn_s_waitcnt(0);
-#pragma unroll
-    for (int i = 0; i < HI; ++i) t.fa[1][i] = typename OpA::frag{};
-#pragma unroll
-    for (int j = 0; j < NI; ++j) t.fb[0][j] = typename OpB::frag{};
-    int put = STAGES - 1, get = 0, s = 0;
+    int put = STAGES - 1, get = 1 % STAGES, s = 1;
+    if (steps > STAGES - 1) {
+      t.template stage<true, true>(acc, lds + put * STAGE, lds);
+      put = 0;
+    } else {
+      t.template stage<false, true>(acc, lds, lds);
+    }
     for (; s < steps - (STAGES - 1); ++s) {
-      t.template stage<true>(acc, lds + put * STAGE, lds + get * STAGE);
+      t.template stage<true, false>(acc, lds + put * STAGE, lds + get * STAGE);
       put = put + 1 == STAGES ? 0 : put + 1;
       get = get + 1 == STAGES ? 0 : get + 1;
     }
     for (; s < steps; ++s) {
-      t.template stage<false>(acc, lds, lds + get * STAGE);
+      t.template stage<false, false>(acc, lds, lds + get * STAGE);
       get = get + 1 == STAGES ? 0 : get + 1;
     }
     t.multiply(acc, 1, 0);

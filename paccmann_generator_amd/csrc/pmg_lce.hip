@@ -35,10 +35,11 @@ template <> __device__ __forceinline__ float exp_of<bf16_t>(float x) { return __
 struct Shape {
   int BM, BN, WM, WN, KB, stages, per_cu;
 };
-enum { S256, S128, S64, SN64, SM64, SK16W, SK16, SK32, SK64 };  // S: square, SN / SM: 64 of n / m, SK: few tokens
+enum { S256, S128, S64, SN64, SM64, SK16W, SK16, SK32, SK64, SD64 };  // S: square, SN / SM / SD: 64 of n or m, SK: few tokens
 constexpr Shape SHAPES[] = {{256, 256, 2, 4, 64, 3, 1}, {128, 128, 2, 4, 128, 2, 2}, {64, 64, 2, 2, 128, 2, 5},
-                            {256, 64, 4, 1, 128, 2, 2}, {64, 256, 1, 4, 128, 2, 2},  {128, 16, 2, 1, 128, 2, 4},
-                            {64, 16, 2, 1, 128, 2, 8},  {128, 32, 2, 1, 128, 2, 4},  {128, 64, 2, 1, 128, 2, 3}};
+                            {128, 64, 2, 2, 128, 2, 3}, {64, 128, 2, 2, 128, 2, 3},  {128, 16, 2, 1, 128, 2, 4},
+                            {64, 16, 2, 1, 128, 2, 8},  {128, 32, 2, 1, 128, 2, 4},  {128, 64, 2, 1, 128, 2, 3},
+                            {128, 64, 2, 2, 64, 2, 6}};
 template <typename T, int S, bool AKC, bool BKC, bool ALIST, bool BLIST>
 using TileOf = pmg_tile<T, SHAPES[S].BM, SHAPES[S].BN, SHAPES[S].WM, SHAPES[S].WN, AKC, BKC, ALIST, BLIST, SHAPES[S].KB,
                         SHAPES[S].stages>;
@@ -238,17 +239,22 @@ __global__ __launch_bounds__(THREADS_OF<S>) void lce_grad_kernel(const GradArgs 
   if (n0 >= N) return;
   const int64_t steps = (K + Tile::KSTEP - 1) / Tile::KSTEP, per = (steps + a.splits - 1) / a.splits * Tile::KSTEP;
   const int64_t k0 = per * blockIdx.y, k1 = k0 + per < K ? k0 + per : K;
-  f32x4 acc[Tile::MI][Tile::NI];
-  Tile::run(acc, (lds_char*)smem, a.A, a.lda, a.list, m0, a.M, a.B, a.ldb, nullptr, n0, N, k0, k1);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t mw = m0 + (wave / WN) * (BM / WM) + 4 * (lane >> 4), nw = n0 + (wave % WN) * (BN / WN) + (lane & 15);
+  int place[Tile::NI];  // of this lane's rows of the result
+  if (BKC) {
+#pragma unroll
+    for (int j = 0; j < Tile::NI; ++j) place[j] = nw + j * 16 < N ? a.list[nw + j * 16] : 0;
+  }
+  f32x4 acc[Tile::MI][Tile::NI];
+  Tile::run(acc, (lds_char*)smem, a.A, a.lda, a.list, m0, a.M, a.B, a.ldb, nullptr, n0, N, k0, k1);
   float* sums = a.acc ? a.acc + (int64_t)blockIdx.y * a.N * a.M : nullptr;
   const bool als = (a.M & 3) == 0, alo = ((a.ldo & 3) == 0) && pmg_aligned4((const T*)a.out);
 #pragma unroll
   for (int j = 0; j < Tile::NI; ++j) {
     const int64_t n = nw + j * 16;
     if (n >= N) continue;
-    const int64_t o = BKC && a.out ? a.list[n] : n;
+    const int64_t o = BKC ? place[j] : n;
 #pragma unroll
     for (int i = 0; i < Tile::MI; ++i) {
       const int64_t m = mw + i * 16;
@@ -256,7 +262,8 @@ __global__ __launch_bounds__(THREADS_OF<S>) void lce_grad_kernel(const GradArgs 
       f32x4 x = acc[i][j];
       float* s = sums + n * a.M + m;
       if (a.add) x += pmg_load4(s, als, a.M - m);
-      if (a.out) pmg_store4((T*)a.out + o * a.ldo + m, x, alo, a.M - m);
+      if (a.out && S == SD64) pmg_store4_nt((T*)a.out + o * a.ldo + m, x, alo, a.M - m);
+      else if (a.out) pmg_store4((T*)a.out + o * a.ldo + m, x, alo, a.M - m);
       else pmg_store4(s, x, als, a.M - m);
     }
   }
@@ -275,17 +282,26 @@ __global__ __launch_bounds__(256) void lce_join_kernel(const float* __restrict__
   out[(list ? list[r] : r) * ldo + (i - r * M)] = (T)s;
 }
 
-// db[v] = sum over the tiles of BN tokens
+// db[v] = sum over the tiles of BN tokens; 64 entries by 16 groups that take the tiles in turn, joined in order
 template <typename T>
-__global__ __launch_bounds__(256) void lce_dbias_kernel(const float* __restrict__ part, int BN, const int* count, int64_t ldl,
-                                                        int64_t V, T* __restrict__ db) {
-  const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (v >= V) return;
-  const int tiles = (count[0] + BN - 1) / BN;
+__global__ __launch_bounds__(1024) void lce_dbias_kernel(const float* __restrict__ part, int BN, const int* count, int64_t ldl,
+                                                         int64_t V, T* __restrict__ db) {
+  __shared__ float red[16][64];
+  const int c = threadIdx.x & 63, grp = threadIdx.x >> 6, tiles = (uniform_of(count) + BN - 1) / BN;
+  const int64_t v = (int64_t)blockIdx.x * 64 + c;
   float s = 0.0f;
+  if (v < V) {
 #pragma unroll 8
-  for (int k = 0; k < tiles; ++k) s += part[(int64_t)k * ldl + v];
-  db[v] = (T)s;
+    for (int k = grp; k < tiles; k += 16) s += part[(int64_t)k * ldl + v];
+  }
+  red[grp][c] = s;
+  __syncthreads();
+  if (grp == 0 && v < V) {
+    s = 0.0f;
+#pragma unroll
+    for (int g = 0; g < 16; ++g) s += red[g][c];
+    db[v] = (T)s;
+  }
 }
 
 // ------------------------------------------------------------------------------------------ rows
@@ -474,14 +490,20 @@ __global__ __launch_bounds__(1024) void lce_scan_kernel(int* __restrict__ first,
   }
 }
 
-// zero rows of the gradient of hidden for the rows without a slope; a wave a row
+// zero rows of the gradient of hidden for the rows without a slope; a workgroup looks at 64 rows, a wave takes every
+// fourth of those it finds
 template <typename T>
 __global__ __launch_bounds__(256) void lce_zero_rows_kernel(const uint8_t* __restrict__ used, int64_t N, int64_t H,
                                                             T* __restrict__ dx) {
-  const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (n >= N || used[n]) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t n0 = (int64_t)blockIdx.x * 64;
+  uint64_t left = __ballot(n0 + lane < N && !used[n0 + lane]);
   const bool al = (H & 3) == 0 && pmg_aligned4(dx);
-  for (int64_t c = (threadIdx.x & 63) * 4; c < H; c += 256) pmg_store4(dx + n * H + c, f32x4{0.f, 0.f, 0.f, 0.f}, al, H - c);
+  for (int k = 0; left; ++k, left &= left - 1) {
+    if ((k & 3) != wave) continue;
+    T* row = dx + (n0 + __ffsll((unsigned long long)left) - 1) * H;
+    for (int64_t c = lane * 4; c < H; c += 256) pmg_store4(row + c, f32x4{0.f, 0.f, 0.f, 0.f}, al, H - c);
+  }
 }
 
 // rows of `width` elements, `ld` apart, into rows of `wide` (a multiple of 16 bytes), zero behind the end
@@ -524,14 +546,17 @@ int logits_shape(int64_t V, int64_t N, bool backward) {
     if (N <= 16) return div_up(V, 128) >= 3 * CUS ? SK16W : SK16;
     return N <= 32 ? SK32 : SK64;
   }
-  if (V <= 64) return div_up(N, 256) >= CUS ? SM64 : S64;
+  if (V <= 64) return div_up(N, 128) >= CUS ? SM64 : S64;
   return best_square(V, N);
 }
 
-int dx_shape(int64_t H, int64_t N) { return best_square(H, N); }
+// A short sum (few vocabulary entries) is bound by writing dx: small tiles, several a CU, so that some write while
+// others multiply, and stores that pass the caches by (fp32, 524288 x 512 over 60: 380 us; 410 us with plain stores, 478
+// us with 64 x 256, 506 us with the large square).
+int dx_shape(int64_t H, int64_t N, int64_t K) { return K <= 256 && H > 64 ? SD64 : best_square(H, N); }
 
 int dw_shape(int64_t H, int64_t V) {
-  if (V <= 64 && H >= 256) return SN64;
+  if (V <= 64 && H > 64) return SN64;
   return best_square(H, V);
 }
 
@@ -554,9 +579,9 @@ struct Problem {
   int kstep;
 };
 
-// Vocabulary entries of a backward piece: dl of a piece stays around 128 MB, which the chip's last-level cache
-// holds between the product that writes it and the two that read it.
-constexpr int64_t PIECE_BYTES = 128 << 20;
+// Vocabulary entries of a backward piece: dl of a piece takes about 256 MB.  8192 tokens over 128000 (2 GB in one piece):
+// 27.4 ms a step with 256 MB, 27.2 with 128, 27.7 with 1024; 4095 over 32001 (250 MB): 1.80 ms, 1.90 in pieces of 128 MB.
+constexpr int64_t PIECE_BYTES = 256 << 20;
 int64_t piece_of(const Problem& p) {
   if (p.V <= 256) return p.V;
   int64_t v = PIECE_BYTES / (p.N * (int64_t)p.eb) / 256 * 256;
@@ -616,7 +641,7 @@ BwdPlan bwd_plan(const Problem& p) {
   b.pieces = div_up(p.V, b.piece);
   b.ldl = up(b.piece, 64);
   b.s_dl = logits_shape(b.piece, p.N, true);
-  b.s_dx = dx_shape(p.H, p.N);
+  b.s_dx = dx_shape(p.H, p.N, b.piece);
   b.s_dw = dw_shape(p.H, b.piece);
   b.split_dx = b.pieces == 1 ? splits_of(b.s_dx, p.H, p.N, b.piece, p.kstep) : 1;
   b.split_dw = splits_of(b.s_dw, p.H, b.piece, p.N, p.kstep);
@@ -712,6 +737,9 @@ template <typename T, bool BKC> int grad(int s, GradArgs a, hipStream_t st) {
     case SN64:
       if constexpr (!BKC) rc = launch_grad<T, SN64, BKC>(a, st);
       break;
+    case SD64:
+      if constexpr (BKC) rc = launch_grad<T, SD64, BKC>(a, st);
+      break;
   }
   if (rc || a.splits == 1) return rc;
   const int64_t total = a.N * a.M;
@@ -800,7 +828,7 @@ template <typename T> int backward(const pmg_linear_ce* a, const Problem& p, cha
   }
   hipLaunchKernelGGL(lce_slopes_kernel<true>, dim3(sl.groups), dim3(1024), 0, st, sl);
   if (a->grad_hidden)
-    hipLaunchKernelGGL(lce_zero_rows_kernel<T>, dim3((unsigned)div_up(p.N, 4)), dim3(256), 0, st, sl.used, p.N, p.H,
+    hipLaunchKernelGGL(lce_zero_rows_kernel<T>, dim3((unsigned)div_up(p.N, 64)), dim3(256), 0, st, sl.used, p.N, p.H,
                        (T*)a->grad_hidden);
   l.row = sl.row;
   l.list = sl.list;
@@ -818,7 +846,7 @@ template <typename T> int backward(const pmg_linear_ce* a, const Problem& p, cha
     l.bias = bias ? bias + v0 * (int64_t)p.eb : nullptr;
     if (const int rc = logits<T, true>(b.s_dl, l, st)) return rc;
     if (a->grad_bias)
-      hipLaunchKernelGGL(lce_dbias_kernel<T>, dim3((unsigned)div_up(v, 256)), dim3(256), 0, st, l.dbias,
+      hipLaunchKernelGGL(lce_dbias_kernel<T>, dim3((unsigned)div_up(v, 64)), dim3(1024), 0, st, l.dbias,
                          SHAPES[b.s_dl].BN, sl.total, b.ldl, v, (T*)a->grad_bias + v0);
     if (a->grad_hidden) {
       GradArgs g = {};

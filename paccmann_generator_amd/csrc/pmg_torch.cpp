@@ -111,7 +111,7 @@ Tensor embedding_bwd(const Tensor& grad, const Tensor& ids, int64_t vocab_size, 
   int64_t ld;
   const Tensor g = rows_of(grad, E, &ld), flat = ids.contiguous();
   size_t need = 0;
-  check(pmg_embedding_bwd_workspace(flat.numel(), vocab_size, E, &need), "pmg_embedding_bwd_workspace");
+  check(pmg_embedding_bwd_workspace(flat.numel(), vocab_size, E, dtype, &need), "pmg_embedding_bwd_workspace");
   const Tensor ws = bytes(need, grad);
   Tensor out = at::empty({vocab_size, E}, grad.options().requires_grad(false));
   On on(grad.device());

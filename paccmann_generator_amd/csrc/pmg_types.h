@@ -39,6 +39,13 @@ template <typename T> __device__ __forceinline__ void pmg_store4(T* p, f32x4 x, 
   for (int j = 0; j < 4; ++j)
     if (j < left) p[j] = (T)x[j];
 }
+// past the caches: for results that nobody reads soon
+template <typename T> __device__ __forceinline__ void pmg_store4_nt(T* p, f32x4 x, bool aligned, int64_t left) {
+  if (!aligned || left < 4) return pmg_store4(p, x, aligned, left);
+  typename pmg_vec4<T>::type v;
+  v.x = (T)x.x; v.y = (T)x.y; v.z = (T)x.z; v.w = (T)x.w;
+  __builtin_nontemporal_store(v, reinterpret_cast<typename pmg_vec4<T>::type*>(p));
+}
 template <typename T> __device__ __forceinline__ bool pmg_aligned4(const T* p) {
   return ((uintptr_t)p & (4 * sizeof(T) - 1)) == 0;
 }
@@ -49,10 +56,18 @@ static inline bool pmg_dtype_ok(int dtype) { return dtype == PMG_F32 || dtype ==
 // 16 bytes of a row: 4 fp32 or 8 bf16 / fp16 elements, in fp32 registers.
 template <typename T> struct pmg_vec16 {
   static constexpr int N = 16 / sizeof(T);
+  typedef T vec __attribute__((ext_vector_type(N)));
   float x[N];
+  // the 16 bytes as they lie in memory: a load whose conversion (unpack) waits until they are needed
+  static __device__ __forceinline__ vec raw(const T* p, bool aligned, int64_t left) {
+    if (aligned && left >= N) return *reinterpret_cast<const vec*>(p);
+    vec v;
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = j < left ? p[j] : (T)0.0f;
+    return v;
+  }
   // `left` elements remain at p (>= 1); aligned: p is a multiple of 16 bytes
   __device__ __forceinline__ void load(const T* p, bool aligned, int64_t left) {
-    typedef T vec __attribute__((ext_vector_type(N)));
     if (aligned && left >= N) {
       const vec v = *reinterpret_cast<const vec*>(p);
 #pragma unroll
@@ -63,7 +78,6 @@ template <typename T> struct pmg_vec16 {
     }
   }
   __device__ __forceinline__ void store(T* p, bool aligned, int64_t left) const {
-    typedef T vec __attribute__((ext_vector_type(N)));
     if (aligned && left >= N) {
       vec v;
 #pragma unroll

@@ -54,11 +54,11 @@ def test_embedding_refusals_and_workspace():
         assert bwd(**bad) < 0, bad
     last = 0
     for n in (0, 1, 2048, 2049, 100000, 1 << 20):
-        assert lib.pmg_embedding_bwd_workspace(n, 32000, 512, C.byref(size)) == 0
+        assert lib.pmg_embedding_bwd_workspace(n, 32000, 512, 1, C.byref(size)) == 0
         assert size.value >= last and size.value >= 8 * n
         last = size.value
-    assert lib.pmg_embedding_bwd_workspace(-1, 9, 8, C.byref(size)) < 0
-    assert lib.pmg_embedding_bwd_workspace(4, 9, 8, None) < 0
+    assert lib.pmg_embedding_bwd_workspace(-1, 9, 8, 0, C.byref(size)) < 0
+    assert lib.pmg_embedding_bwd_workspace(4, 9, 8, 0, None) < 0 and lib.pmg_embedding_bwd_workspace(4, 9, 8, 3, C.byref(size)) < 0
 
 
 def test_linear_ce_refusals_and_workspace():
