@@ -7,7 +7,8 @@ from . import _ffi  # noqa: F401  (fails loudly when the HIP library is missing)
 from .decoder import Generator, GreedySearch, SamplingSearch, StackGRUDecoder  # noqa: F401
 from . import ops  # noqa: F401
 from .hostpool import HostPool  # noqa: F401
+from .optim import AdamW  # noqa: F401
 from .reinforce import Reinforce, ReinforceMultiModalSets, ReinforceOmic, ReinforceProtein  # noqa: F401
 
-__all__ = ['Generator', 'GreedySearch', 'SamplingSearch', 'StackGRUDecoder', 'ops', 'Reinforce', 'ReinforceOmic',
+__all__ = ['AdamW', 'Generator', 'GreedySearch', 'SamplingSearch', 'StackGRUDecoder', 'ops', 'Reinforce', 'ReinforceOmic',
            'ReinforceProtein', 'ReinforceMultiModalSets', 'HostPool']

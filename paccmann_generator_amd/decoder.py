@@ -81,6 +81,22 @@ class StackGRUDecoder(nn.Module):
         h_out, s_out, _ = ops.step(self.weights(), input_token, hidden, stack, want_logits=False)
         return h_out[-1:].clone(), h_out, s_out
 
+    # -- the vocabulary's two ends, differentiable (pre-training, scoring with other recurrences) -----------------
+    def embed(self, tokens, trusted_tokens: bool = False):
+        """Embedded tokens [..., E]: the lookup of ``embedding``, whose gradient is summed by sorted tokens."""
+        return ops.embedding(self.embedding.weight, tokens, padding_idx=self.embedding.padding_idx,
+                             trusted_tokens=trusted_tokens)
+
+    def token_loss(self, hidden, targets, reward=None, ignore_index: int = -100, temperature: float = 1.0,
+                   reduction: str = 'mean', trusted_tokens: bool = False):
+        """Negative log-probability of ``targets`` [...] under ``output_layer(hidden [..., H]) / temperature``, times
+        ``reward`` [...] where given: output_layer, log_softmax, gather and the reward-weighted mean of
+        reinforce_omics.py:326-332 without keeping the logits, for a vocabulary of any size."""
+        loss, _ = ops.linear_cross_entropy(hidden, self.output_layer.weight, targets, bias=self.output_layer.bias,
+                                           row_weight=reward, ignore_index=ignore_index, logit_scale=1.0 / temperature,
+                                           reduction=reduction, trusted_tokens=trusted_tokens)
+        return loss
+
 
 class _CroppedRows:
     """Iterable of variable-length 1-D token tensors (what TeacherVAE.generate yields,

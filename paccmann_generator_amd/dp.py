@@ -127,7 +127,7 @@ def _scatter_grads(params, flat, take) -> None:
 
 def data_parallel_step(dec_params: Sequence[torch.nn.Parameter], enc_params: Sequence[torch.nn.Parameter],
                        optimizer, backward_fn: Callable[[], object], num_mols: int, reward_sum,
-                       grad_clipping: Optional[float], group=None):
+                       grad_clipping: Optional[float], group=None, clip_fn: Callable = torch.nn.utils.clip_grad_norm_):
     """One data-parallel REINFORCE update on this rank's shard (reinforce_omics.py:289-341 with the
     mean over valid molecules taken over ALL ranks).  Device-agnostic: the HIP operator (or, in the
     CPU tests, the oracle) comes in through ``backward_fn``.
@@ -149,6 +149,8 @@ def data_parallel_step(dec_params: Sequence[torch.nn.Parameter], enc_params: Seq
     reference never zeroes them and they carry over from step to step.  Only THIS step's
     contribution is summed over the ranks; the carried part is set aside before the backward pass
     and added back afterwards (summing it too would multiply it by the world size every step).
+
+    ``clip_fn(parameters, max_norm)`` clips their gradients in place.
 
     Returns (mean reward, loss) as 0-dim tensors on the parameters' device -- (0, 0) when the update
     was skipped -- and the global valid count (a 0-dim tensor, or the int 0)."""
@@ -182,6 +184,6 @@ def data_parallel_step(dec_params: Sequence[torch.nn.Parameter], enc_params: Seq
         if g is not None:
             p.grad = g if p.grad is None else g.add_(p.grad)
     if grad_clipping is not None:
-        torch.nn.utils.clip_grad_norm_(params, grad_clipping)
+        clip_fn(params, grad_clipping)
     optimizer.step()
     return tail[-2].clone(), tail[-3].clone(), n_glob

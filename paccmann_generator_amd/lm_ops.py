@@ -160,6 +160,11 @@ def clip_grad_norm_(grads: Sequence[Tensor], max_norm: float) -> Tensor:
         return _ops.clip_grad_norm_.default(grads, float(max_norm))
 
 
+def clip_param_grads_(params: Sequence[Tensor], max_norm: float) -> Tensor:
+    """``clip_grad_norm_`` of the gradients of ``params`` that have one."""
+    return clip_grad_norm_([p.grad for p in params if p.grad is not None], max_norm)
+
+
 # ------------------------------------------------------------------------------------------- AdamW
 @torch.library.register_fake('pmg::adamw_step_')
 def _(*args):

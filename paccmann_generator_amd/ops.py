@@ -28,8 +28,8 @@ import torch
 from torch import Tensor
 
 from . import _ffi
-from .lm_ops import (adamw_state, adamw_state_values, adamw_step, clip_grad_norm_, embedding,  # noqa: F401
-                     grad_norm, linear_cross_entropy)
+from .lm_ops import (adamw_state, adamw_state_values, adamw_step, clip_grad_norm_, clip_param_grads_,  # noqa: F401
+                     embedding, grad_norm, linear_cross_entropy)
 
 # Largest workspace one kernel call of the training pair may take; larger batches run as chunks whose
 # gradients accumulate (PMG_FLAG_ACCUMULATE).  At most 96 GiB of the 288 GB of HBM -- configs[3]

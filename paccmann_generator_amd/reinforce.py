@@ -26,6 +26,7 @@ import torch
 
 from . import _ffi, dp, ops
 from .decoder import SamplingSearch
+from .optim import AdamW
 
 
 def _rdkit_validity():
@@ -49,6 +50,8 @@ class Reinforce(object):
         reward_fn:     host reward ``f(smiles, target) -> array`` (reinforce_omics.py:209-222)
         score_fn:      host scoring used by generate_compounds_and_evaluate (defaults to reward_fn)
         process_group: torch.distributed group for data-parallel latent sharding
+        params['optimizer']: 'adam' (torch.optim.Adam, the default) or 'fused_adam' (optim.AdamW: the same update, and
+                       the clipping, in a few launches over all parameters; params['optimizer_state_bits'] 32 or 8)
         micro_batches: k > 1 runs the reward scoring of a step under its teacher-forced pass and the
                        backward passes of earlier slices (_policy_gradient_pipelined); also read from
                        params['micro_batches']; default 1 (the reference's serial order)
@@ -65,12 +68,17 @@ class Reinforce(object):
             raise RuntimeError('paccmann_generator_amd needs the decoder on a GPU: there is no CPU path')
 
         # reinforce.py:44-49: Adam over decoder parameters only
-        self.optimizer = torch.optim.Adam(
-            list(self.generator.decoder.parameters()),
-            lr=params.get('learning_rate', 0.0001),
-            eps=params.get('eps', 0.0001),
-            weight_decay=params.get('weight_decay', 0.00001),
-        )
+        hyper = dict(lr=params.get('learning_rate', 0.0001), eps=params.get('eps', 0.0001),
+                     weight_decay=params.get('weight_decay', 0.00001))
+        kind = params.get('optimizer', 'adam')
+        if kind == 'adam':
+            self.optimizer = torch.optim.Adam(list(self.generator.decoder.parameters()), **hyper)
+        elif kind == 'fused_adam':
+            self.optimizer = AdamW(list(self.generator.decoder.parameters()), decoupled=False,
+                                   state_bits=params.get('optimizer_state_bits', 32), **hyper)
+        else:
+            raise ValueError(f"params['optimizer'] must be 'adam' or 'fused_adam', got {kind!r}")
+        self._clip = ops.clip_param_grads_ if kind == 'fused_adam' else torch.nn.utils.clip_grad_norm_
         self.model_name = model_name
         self.model_path = os.path.join(params.get('model_folder', 'biased_models'), model_name)
         self.weights_path = os.path.join(self.model_path, 'weights/{}')
@@ -244,13 +252,13 @@ class Reinforce(object):
         if ddp:
             r, l, _ = dp.data_parallel_step(dec_params, enc_params, self.optimizer, lambda: run(1.0), num_mols,
                                             rewards_t.sum() if num_mols > 0 else 0.0, self.grad_clipping,
-                                            group=self.process_group)
+                                            group=self.process_group, clip_fn=self._clip)
             return r, l
         self.optimizer.zero_grad()
         loss = run(1.0 / num_mols)
         summed_reward = torch.mean(rewards_t.float())
         if self.grad_clipping is not None:
-            torch.nn.utils.clip_grad_norm_(dec_params + enc_params, self.grad_clipping)
+            self._clip(dec_params + enc_params, self.grad_clipping)
         self.optimizer.step()
         return summed_reward, loss
 
@@ -385,13 +393,13 @@ class Reinforce(object):
         if ddp:
             r, loss, _ = dp.data_parallel_step(dec_params, enc_params, self.optimizer, lambda: run(1.0), n_valid,
                                                lambda: float(sum(float(x.sum(dtype=np.float64)) for x in rewards_all)),
-                                               self.grad_clipping, group=self.process_group)
+                                               self.grad_clipping, group=self.process_group, clip_fn=self._clip)
             return r, _loss_value(loss)
         self.optimizer.zero_grad()
         loss = run(1.0 / n_valid)
         r = torch.mean(torch.from_numpy(np.concatenate(rewards_all)).float())
         if self.grad_clipping is not None:
-            torch.nn.utils.clip_grad_norm_(dec_params + enc_params, self.grad_clipping)
+            self._clip(dec_params + enc_params, self.grad_clipping)
         self.optimizer.step()
         return r, _loss_value(loss)
 
