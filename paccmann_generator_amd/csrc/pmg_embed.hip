@@ -42,23 +42,23 @@ __global__ __launch_bounds__(THREADS) void embed_fwd_kernel(const T* __restrict_
   const int64_t c = ((int64_t)blockIdx.y * tpr + (threadIdx.x & (tpr - 1))) * VEC;
   if (c >= E) return;
   const int64_t row0 = (int64_t)blockIdx.x * rpw * ROWS + threadIdx.x / tpr;
-  const bool ali = pmg_rows_aligned16(W, ldw), alo = pmg_rows_aligned16(out, E);
-  pmg_vec16<T> x[ROWS];
+  typename pmg_vec16<T>::vec x[ROWS];
   bool ok[ROWS];
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
     const int64_t n = row0 + (int64_t)r * rpw;
     const int64_t id = n < N ? (int64_t)ids[n] : 0;
     ok[r] = id >= 0 && id < V;
-    if (n < N) x[r].load(W + (ok[r] ? id : 0) * ldw + c, ali, E - c);
+    if (n < N) x[r] = pmg_vec16<T>::load(W + (ok[r] ? id : 0) * ldw + c, E - c);
   }
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
     const int64_t n = row0 + (int64_t)r * rpw;
     if (n >= N) break;
+    float y[VEC];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) x[r].x[j] = ok[r] ? x[r].x[j] * scale : __builtin_nanf("");
-    x[r].store(out + n * E + c, alo, E - c);
+    for (int j = 0; j < VEC; ++j) y[j] = ok[r] ? (float)x[r][j] * scale : __builtin_nanf("");
+    pmg_vec16<T>::store(out + n * E + c, y, E - c);
   }
 }
 
@@ -241,7 +241,6 @@ __global__ __launch_bounds__(THREADS) void embed_reduce_kernel(const ReduceArgs 
                                                                T* __restrict__ dW) {
   constexpr int VEC = pmg_vec16<T>::N;
   constexpr int U = 8;  // rows loaded ahead of their sum
-  const bool alo = pmg_rows_aligned16(dW, a.E);
   if ((int64_t)blockIdx.x >= a.reduce_blocks) {
     // rows of tokens that do not occur
     __shared__ int absent[FILL_ROWS];
@@ -258,13 +257,11 @@ __global__ __launch_bounds__(THREADS) void embed_reduce_kernel(const ReduceArgs 
       absent[threadIdx.x] = v < a.V && !(lo < a.N && (int64_t)a.keys[lo] == v);
     }
     __syncthreads();
-    pmg_vec16<T> z;
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) z.x[j] = 0.0f;
+    const float zero[VEC] = {};
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     for (int r = wave; r < FILL_ROWS; r += THREADS / 64)
       if (absent[r])
-        for (int64_t c = lane * VEC; c < a.E; c += 64 * VEC) z.store(dW + (v0 + r) * a.E + c, alo, a.E - c);
+        for (int64_t c = lane * VEC; c < a.E; c += 64 * VEC) pmg_vec16<T>::store(dW + (v0 + r) * a.E + c, zero, a.E - c);
     return;
   }
   // the workgroup's keys and positions, and the keys next to them
@@ -281,7 +278,6 @@ __global__ __launch_bounds__(THREADS) void embed_reduce_kernel(const ReduceArgs 
   const int grp = threadIdx.x / a.tpr;
   const int64_t ch = (int64_t)blockIdx.x * (THREADS / a.tpr) + grp;
   if (c >= a.E || ch >= a.chunks) return;
-  const bool ali = pmg_rows_aligned16(g, a.ldg), alp = (a.E & 3) == 0;
   const int lo = grp * a.chunk, n = (int)(a.N - ch * a.chunk < a.chunk ? a.N - ch * a.chunk : a.chunk);
   const uint32_t* k = key + 1 + lo;  // k[-1] and k[n]: the neighbours
   const uint32_t* at = pos + lo;
@@ -294,21 +290,21 @@ __global__ __launch_bounds__(THREADS) void embed_reduce_kernel(const ReduceArgs 
     float* p = a.part + (ch * 2 + slot) * a.E + c;
 #pragma unroll
     for (int j = 0; j < VEC; j += 4) {
-      if (c + j < a.E) pmg_store4(p + j, f32x4{acc[j], acc[j + 1], acc[j + 2], acc[j + 3]}, alp, a.E - c - j);
+      if (c + j < a.E) pmg_store4(p + j, f32x4{acc[j], acc[j + 1], acc[j + 2], acc[j + 3]}, a.E - c - j);
     }
   };
   auto put_row = [&]() {
-    pmg_vec16<T> y;
+    float y[VEC];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) y.x[j] = acc[j] * a.scale;
-    y.store(dW + (int64_t)cur * a.E + c, alo, a.E - c);
+    for (int j = 0; j < VEC; ++j) y[j] = acc[j] * a.scale;
+    pmg_vec16<T>::store(dW + (int64_t)cur * a.E + c, y, a.E - c);
   };
   typedef typename pmg_vec16<T>::vec vec;
   vec x[2][U];
   auto load = [&](vec(&v)[U], int i) {
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (i + u < n && k[i + u] < (uint32_t)a.V) v[u] = pmg_vec16<T>::raw(g + (int64_t)at[i + u] * a.ldg + c, ali, a.E - c);
+      if (i + u < n && k[i + u] < (uint32_t)a.V) v[u] = pmg_vec16<T>::load(g + (int64_t)at[i + u] * a.ldg + c, a.E - c);
   };
   // false: what follows takes no part (dropped positions sort last)
   auto add = [&](const vec(&v)[U], int i) {
@@ -372,7 +368,6 @@ __global__ __launch_bounds__(JOIN_THREADS) void embed_join_kernel(const ReduceAr
   }
   const int groups = JOIN_THREADS / a.tpr, grp = threadIdx.x / a.tpr, t = threadIdx.x & (a.tpr - 1);
   const int64_t c = ((int64_t)blockIdx.y * a.tpr + t) * VEC;
-  const bool alp = (a.E & 3) == 0;
   float acc[VEC];
 #pragma unroll
   for (int j = 0; j < VEC; ++j) acc[j] = 0.0f;
@@ -383,7 +378,7 @@ __global__ __launch_bounds__(JOIN_THREADS) void embed_join_kernel(const ReduceAr
 #pragma unroll
       for (int j = 0; j < VEC; j += 4) {
         if (c + j < a.E) {
-          const f32x4 x = pmg_load4(p + j, alp, a.E - c - j);
+          const f32x4 x = pmg_load4(p + j, a.E - c - j);
           acc[j] += x.x; acc[j + 1] += x.y; acc[j + 2] += x.z; acc[j + 3] += x.w;
         }
       }
@@ -393,14 +388,14 @@ __global__ __launch_bounds__(JOIN_THREADS) void embed_join_kernel(const ReduceAr
   for (int j = 0; j < VEC; ++j) sum[j * JOIN_THREADS + threadIdx.x] = acc[j];
   __syncthreads();
   if (grp == 0 && c < a.E) {
-    pmg_vec16<T> y;
+    float y[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
       float s = 0.0f;
       for (int q = 0; q < groups; ++q) s += sum[j * JOIN_THREADS + q * a.tpr + t];
-      y.x[j] = s * a.scale;
+      y[j] = s * a.scale;
     }
-    y.store(dW + (int64_t)cur * a.E + c, pmg_rows_aligned16(dW, a.E), a.E - c);
+    pmg_vec16<T>::store(dW + (int64_t)cur * a.E + c, y, a.E - c);
   }
 }
 

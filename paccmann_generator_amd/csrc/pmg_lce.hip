@@ -2,15 +2,17 @@
 // never kept.
 //
 //   l = s (x W^T + b)     lse_n = log sum_v exp l_nv     nll_n = lse_n - l_{n,t_n}
-//   dl_nv = s (a_n exp(l_nv - lse_n) - c_n [v = t_n])    dx = dl W    dW = dl^T x    db = sum_n dl_n
-// where c_n is the slope of the loss in nll_n and a_n that plus the slope in lse_n.
+//   dl_nv = a_n exp(l_nv - lse_n) - c_n [v = t_n]    dx = f dl W    dW = f dl^T x    db = f sum_n dl_n
+// where f c_n / s is the slope of the loss in nll_n, f a_n / s that plus the slope in lse_n, and f what all rows have
+// in common (the logits' scale, and of a reduced loss its slope and the mean's 1 / count).
 //
 // Forward: the tile product of pmg_gemm.h (m = vocabulary, n = tokens) whose epilogue leaves per token and
 // vocabulary tile the largest logit and the sum of exponentials below it, and the target's logit: 8 bytes
 // for 256 logits.  A second kernel joins them.  Few tokens (serving) take narrow tiles: W is streamed once.
 // Backward: the vocabulary goes in pieces; of each piece the logits are formed again, dl is written in the
-// operands' type (bf16: one rounding, relative 2^-9 like the operands themselves; the products sum in
-// fp32) and read by the two products for dx and dW.  dx is summed over the pieces in fp32.  Long sums with
+// operands' type (bf16: one rounding, relative 2^-9 at most, like the operands themselves; without f, so
+// that the targets' -1 and the zeros stay exact and the roundings of the rows are not all the same; the products sum
+// in fp32) and read by the two products for dx and dW.  dx is summed over the pieces in fp32.  Long sums with
 // few result tiles are split and joined in a fixed order.  No atomics: equal inputs give equal bits.
 // Rows without a slope (ignored targets, zero weights) take no part in the backward: the others are listed, the
 // products run over the list, and the rows left out get a zero gradient whatever they hold.
@@ -66,6 +68,7 @@ struct LogitArgs {
   const struct Row* row; // [count]
   const int* list;       // [count] their places in X
   const int* count;
+  const float* factor;   // f
   void* dl;              // [count][ldl], columns V .. ldl zero
   int64_t ldl;
   float* dbias;          // [tiles_n][ldl] or null
@@ -170,7 +173,6 @@ __global__ __launch_bounds__(THREADS_OF<S>) void lce_logits_kernel(const LogitAr
       const int64_t n = n0 + wn * (BN / WN) + j * 16 + col;
       if (n < N) {
         const Row r = a.row[n];
-        const float as = r.a * a.scale, cs = r.c * a.scale;
         const int64_t t = (int64_t)r.target - a.v0;
 #pragma unroll
         for (int i = 0; i < MI; ++i) {
@@ -178,8 +180,8 @@ __global__ __launch_bounds__(THREADS_OF<S>) void lce_logits_kernel(const LogitAr
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int64_t v = mw + i * 16 + e;
-            float x = v < a.V ? as * exp_of<T>(acc[i][j][e] - r.lse) : 0.0f;  // entries behind the end are zero
-            if (v == t && v < a.V) x -= cs;
+            float x = v < a.V ? r.a * exp_of<T>(acc[i][j][e] - r.lse) : 0.0f;  // entries behind the end are zero
+            if (v == t && v < a.V) x -= r.c;
             d[e] = x;
             db[i][e] += x;
           }
@@ -206,7 +208,7 @@ __global__ __launch_bounds__(THREADS_OF<S>) void lce_logits_kernel(const LogitAr
         float s = 0.0f;
 #pragma unroll
         for (int w = 0; w < WN; ++w) s += red[w * BM + r];
-        if (m0 + r < a.ldl) a.dbias[(int64_t)tn * a.ldl + m0 + r] = s;
+        if (m0 + r < a.ldl) a.dbias[(int64_t)tn * a.ldl + m0 + r] = s * a.factor[0];
       }
     }
   }
@@ -220,6 +222,7 @@ struct GradArgs {
   int64_t M, N, K;
   const int* list;       // of the rows that the backward takes, and their number:
   const int* count;      // dx: row n of the result is row list[n] of out, N = count; dW: rows k of A, K = count
+  const float* factor;   // f
   int tiles_m, tiles_n, splits;
   void* out;             // of T, row stride ldo; or null: the fp32 sums go to acc
   int64_t ldo;
@@ -248,8 +251,8 @@ __global__ __launch_bounds__(THREADS_OF<S>) void lce_grad_kernel(const GradArgs 
   }
   f32x4 acc[Tile::MI][Tile::NI];
   Tile::run(acc, (lds_char*)smem, a.A, a.lda, a.list, m0, a.M, a.B, a.ldb, nullptr, n0, N, k0, k1);
+  const float f = a.factor[0];
   float* sums = a.acc ? a.acc + (int64_t)blockIdx.y * a.N * a.M : nullptr;
-  const bool als = (a.M & 3) == 0, alo = ((a.ldo & 3) == 0) && pmg_aligned4((const T*)a.out);
 #pragma unroll
   for (int j = 0; j < Tile::NI; ++j) {
     const int64_t n = nw + j * 16;
@@ -259,12 +262,12 @@ __global__ __launch_bounds__(THREADS_OF<S>) void lce_grad_kernel(const GradArgs 
     for (int i = 0; i < Tile::MI; ++i) {
       const int64_t m = mw + i * 16;
       if (m >= a.M) continue;
-      f32x4 x = acc[i][j];
+      f32x4 x = acc[i][j] * f;
       float* s = sums + n * a.M + m;
-      if (a.add) x += pmg_load4(s, als, a.M - m);
-      if (a.out && S == SD64) pmg_store4_nt((T*)a.out + o * a.ldo + m, x, alo, a.M - m);
-      else if (a.out) pmg_store4((T*)a.out + o * a.ldo + m, x, alo, a.M - m);
-      else pmg_store4(s, x, als, a.M - m);
+      if (a.add) x += pmg_load4(s, a.M - m);
+      if (a.out && S == SD64) pmg_store4_nt((T*)a.out + o * a.ldo + m, x, a.M - m);
+      else if (a.out) pmg_store4((T*)a.out + o * a.ldo + m, x, a.M - m);
+      else pmg_store4(s, x, a.M - m);
     }
   }
 }
@@ -421,19 +424,29 @@ struct SlopeArgs {
   Row* row;
   int* list;
   int* total;
+  float scale;           // of the logits
+  float* factor;         // f
   uint8_t* used;         // [N]
 };
 
-__device__ __forceinline__ Row slope_of(const SlopeArgs& a, int64_t n) {
+// What all rows have in common, without the logits' scale; 1 where that is 0 or not finite.
+__device__ __forceinline__ float common_of(const SlopeArgs& a) {
+  if (a.per_row || !a.g_loss) return 1.0f;
+  const float g = a.mean ? a.g_loss[0] / a.count[0] : a.g_loss[0];
+  return g != 0.0f && fabsf(g) < __builtin_inff() ? g : 1.0f;
+}
+
+__device__ __forceinline__ Row slope_of(const SlopeArgs& a, int64_t n, float common) {
   Row r = {0.0f, 0.0f, 0.0f, -1};
   const int64_t t = target_of(a.targets, a.id_bits, n);
   if (t != a.ignore && a.g_loss) {
-    r.c = a.g_loss[a.per_row ? n : 0] * (a.weight ? a.weight[n] : 1.0f);
-    if (a.mean) r.c /= a.count[0];
+    r.c = a.weight ? a.weight[n] : 1.0f;
+    if (a.per_row) r.c *= a.g_loss[n];
+    else if (common == 1.0f) r.c *= a.mean ? a.g_loss[0] / a.count[0] : a.g_loss[0];
     if (t >= 0 && t < a.V) r.target = (int)t;
     else r.c = __builtin_nanf("");
   }
-  r.a = r.c + (a.g_lse ? a.g_lse[n] : 0.0f);
+  r.a = r.c + (a.g_lse ? a.g_lse[n] / common : 0.0f);
   return r;
 }
 
@@ -441,7 +454,8 @@ template <bool WRITE> __global__ __launch_bounds__(1024) void lce_slopes_kernel(
   __shared__ int wsum[16];
   const int64_t n = (int64_t)blockIdx.x * 1024 + threadIdx.x;
   Row r = {0.0f, 0.0f, 0.0f, -1};
-  if (n < a.N) r = slope_of(a, n);
+  const float common = common_of(a);
+  if (n < a.N) r = slope_of(a, n, common);
   const bool used = r.a != 0.0f || r.c != 0.0f;
   const uint64_t mask = __ballot(used);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -464,7 +478,10 @@ template <bool WRITE> __global__ __launch_bounds__(1024) void lce_slopes_kernel(
     a.row[at] = r;
     a.list[at] = (int)n;
   }
-  if (threadIdx.x == 0 && blockIdx.x == (unsigned)a.groups - 1) a.total[0] = base + all;
+  if (threadIdx.x == 0 && blockIdx.x == (unsigned)a.groups - 1) {
+    a.total[0] = base + all;
+    a.factor[0] = common * a.scale;
+  }
 }
 
 __global__ __launch_bounds__(1024) void lce_scan_kernel(int* __restrict__ first, int n) {
@@ -498,11 +515,10 @@ __global__ __launch_bounds__(256) void lce_zero_rows_kernel(const uint8_t* __res
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t n0 = (int64_t)blockIdx.x * 64;
   uint64_t left = __ballot(n0 + lane < N && !used[n0 + lane]);
-  const bool al = (H & 3) == 0 && pmg_aligned4(dx);
   for (int k = 0; left; ++k, left &= left - 1) {
     if ((k & 3) != wave) continue;
     T* row = dx + (n0 + __ffsll((unsigned long long)left) - 1) * H;
-    for (int64_t c = lane * 4; c < H; c += 256) pmg_store4(row + c, f32x4{0.f, 0.f, 0.f, 0.f}, al, H - c);
+    for (int64_t c = lane * 4; c < H; c += 256) pmg_store4(row + c, f32x4{0.f, 0.f, 0.f, 0.f}, H - c);
   }
 }
 
@@ -594,7 +610,7 @@ int64_t piece_of(const Problem& p) {
 
 struct Layout {
   size_t xp, wp, part, at, sums;                    // forward
-  size_t row, list, total, first, used, dl, dxacc, dwacc, dbias;  // backward
+  size_t row, list, total, factor, first, used, dl, dxacc, dwacc, dbias;  // backward
   size_t bytes;
 };
 
@@ -656,6 +672,7 @@ Layout bwd_layout(const Problem& p, const BwdPlan& b) {
   L.row = take((size_t)p.N * sizeof(Row));
   L.list = take(((size_t)p.N + LIST_SLACK) * 4);
   L.total = take(4);
+  L.factor = take(4);
   L.first = take((size_t)div_up(p.N, 1024) * 4);
   L.used = take((size_t)p.N);
   L.dl = take((size_t)p.N * b.ldl * p.eb);
@@ -821,6 +838,8 @@ template <typename T> int backward(const pmg_linear_ce* a, const Problem& p, cha
   sl.row = (Row*)(ws + L.row);
   sl.list = (int*)(ws + L.list);
   sl.total = (int*)(ws + L.total);
+  sl.scale = a->logit_scale;
+  sl.factor = (float*)(ws + L.factor);
   sl.used = (uint8_t*)(ws + L.used);
   if (sl.groups > 1) {
     hipLaunchKernelGGL(lce_slopes_kernel<false>, dim3(sl.groups), dim3(1024), 0, st, sl);
@@ -833,6 +852,7 @@ template <typename T> int backward(const pmg_linear_ce* a, const Problem& p, cha
   l.row = sl.row;
   l.list = sl.list;
   l.count = sl.total;
+  l.factor = sl.factor;
   l.dl = ws + L.dl;
   l.ldl = b.ldl;
   l.dbias = a->grad_bias ? (float*)(ws + L.dbias) : nullptr;
@@ -855,6 +875,7 @@ template <typename T> int backward(const pmg_linear_ce* a, const Problem& p, cha
       g.K = v;
       g.list = sl.list;
       g.count = sl.total;
+      g.factor = sl.factor;
       g.splits = b.split_dx;
       g.out = i == b.pieces - 1 ? a->grad_hidden : nullptr;
       g.ldo = p.H;
@@ -869,6 +890,7 @@ template <typename T> int backward(const pmg_linear_ce* a, const Problem& p, cha
       g.K = p.N;
       g.list = sl.list;
       g.count = sl.total;
+      g.factor = sl.factor;
       g.splits = b.split_dw;
       g.out = (T*)a->grad_weight + v0 * p.H;
       g.ldo = p.H;

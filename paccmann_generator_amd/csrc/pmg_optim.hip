@@ -42,13 +42,12 @@ static_assert(sizeof(GradTable) <= 3800, "kernel arguments");
 
 template <typename T>
 __device__ __forceinline__ double square_sum(const T* __restrict__ g, int64_t n, int64_t lo, int chunk) {
-  const bool al = pmg_aligned4(g);
   double s = 0.0;
 #pragma unroll 4
   for (int i = threadIdx.x * 4; i < chunk; i += THREADS * 4) {
     const int64_t left = n - lo - i;
     if (left <= 0) break;
-    const f32x4 x = pmg_load4(g + lo + i, al, left);
+    const f32x4 x = pmg_load4(g + lo + i, left);
 #pragma unroll
     for (int j = 0; j < 4; ++j) s = fma((double)x[j], (double)x[j], s);
   }
@@ -95,14 +94,13 @@ __global__ __launch_bounds__(1024) void norm_join_kernel(const double* __restric
 
 template <typename T>
 __device__ __forceinline__ void scale_chunk(T* __restrict__ g, int64_t n, int64_t lo, int chunk, float c) {
-  const bool al = pmg_aligned4(g);
 #pragma unroll 4
   for (int i = threadIdx.x * 4; i < chunk; i += THREADS * 4) {
     const int64_t left = n - lo - i;
     if (left <= 0) break;
-    f32x4 x = pmg_load4(g + lo + i, al, left);
+    f32x4 x = pmg_load4(g + lo + i, left);
     x *= c;
-    pmg_store4(g + lo + i, x, al, left);
+    pmg_store4(g + lo + i, x, left);
   }
 }
 
@@ -276,21 +274,22 @@ __device__ __forceinline__ int encode_v(f32x4 x, float share) {
   return c4;
 }
 
-__device__ __forceinline__ int load_codes(const uint8_t* p, bool al, int64_t left) {
-  if (al && left >= 4) return *reinterpret_cast<const int*>(p);
+typedef int __attribute__((aligned(1))) codes4;
+__device__ __forceinline__ int load_codes(const uint8_t* p, int64_t left) {
+  if (left >= 4) return *reinterpret_cast<const codes4*>(p);
   int c = 0;
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
+  for (int j = 0; j < 3; ++j)
     if (j < left) c |= (int)p[j] << (8 * j);
   return c;
 }
-__device__ __forceinline__ void store_codes(uint8_t* p, int c, bool al, int64_t left) {
-  if (al && left >= 4) {
-    *reinterpret_cast<int*>(p) = c;
+__device__ __forceinline__ void store_codes(uint8_t* p, int c, int64_t left) {
+  if (left >= 4) {
+    *reinterpret_cast<codes4*>(p) = c;
     return;
   }
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
+  for (int j = 0; j < 3; ++j)
     if (j < left) p[j] = (uint8_t)(c >> (8 * j));
 }
 
@@ -308,8 +307,6 @@ __global__ __launch_bounds__(THREADS) void adamw_kernel(const AdamwTable t, cons
   P* __restrict__ p = (P*)t.p[i];
   const G* __restrict__ g = (const G*)t.g[i];
   float* __restrict__ w = t.w[i];
-  const bool alp = pmg_aligned4(p), alg = pmg_aligned4(g), alw = pmg_aligned4(w);
-  const bool alm = ((uintptr_t)t.m[i] & (BITS == 32 ? 15 : 3)) == 0, alv = ((uintptr_t)t.v[i] & (BITS == 32 ? 15 : 3)) == 0;
   const float rate = sc->rate, root = sc->root, factor = sc->factor, keep = sc->keep;
 
   f32x4 gx[AW_ITER], px[AW_ITER], mx[AW_ITER], vx[AW_ITER];
@@ -322,14 +319,14 @@ __global__ __launch_bounds__(THREADS) void adamw_kernel(const AdamwTable t, cons
     mc[u] = vc[u] = 0;
     mt[u] = vt[u] = 0.0f;
     if (left > 0) {
-      gx[u] = pmg_load4(g + e, alg, left);
-      px[u] = w ? pmg_load4(w + e, alw, left) : pmg_load4(p + e, alp, left);
+      gx[u] = pmg_load4(g + e, left);
+      px[u] = w ? pmg_load4(w + e, left) : pmg_load4(p + e, left);
       if (BITS == 32) {
-        mx[u] = pmg_load4((const float*)t.m[i] + e, alm, left);
-        vx[u] = pmg_load4((const float*)t.v[i] + e, alv, left);
+        mx[u] = pmg_load4((const float*)t.m[i] + e, left);
+        vx[u] = pmg_load4((const float*)t.v[i] + e, left);
       } else {
-        mc[u] = load_codes((const uint8_t*)t.m[i] + e, alm, left);
-        vc[u] = load_codes((const uint8_t*)t.v[i] + e, alv, left);
+        mc[u] = load_codes((const uint8_t*)t.m[i] + e, left);
+        vc[u] = load_codes((const uint8_t*)t.v[i] + e, left);
         mt[u] = t.mt[i][e / PMG_STATE_BLOCK];
         vt[u] = t.vt[i][e / PMG_STATE_BLOCK];
       }
@@ -359,8 +356,8 @@ __global__ __launch_bounds__(THREADS) void adamw_kernel(const AdamwTable t, cons
         if (j >= left) m[j] = v[j] = 0.0f;
       const float top_m = wave_top(m), top_v = wave_top(v);
       if (left > 0) {
-        store_codes((uint8_t*)t.m[i] + e, encode_m(m, share_of(top_m)), alm, left);
-        store_codes((uint8_t*)t.v[i] + e, encode_v(v, share_of(top_v)), alv, left);
+        store_codes((uint8_t*)t.m[i] + e, encode_m(m, share_of(top_m)), left);
+        store_codes((uint8_t*)t.v[i] + e, encode_v(v, share_of(top_v)), left);
         if ((threadIdx.x & 63) == 0) {
           t.mt[i][e / PMG_STATE_BLOCK] = top_m;
           t.vt[i][e / PMG_STATE_BLOCK] = top_v;
@@ -369,11 +366,11 @@ __global__ __launch_bounds__(THREADS) void adamw_kernel(const AdamwTable t, cons
     }
     if (left > 0) {
       if (BITS == 32) {
-        pmg_store4((float*)t.m[i] + e, m, alm, left);
-        pmg_store4((float*)t.v[i] + e, v, alv, left);
+        pmg_store4((float*)t.m[i] + e, m, left);
+        pmg_store4((float*)t.v[i] + e, v, left);
       }
-      if (w) pmg_store4(w + e, x, alw, left);
-      pmg_store4(p + e, x, alp, left);
+      if (w) pmg_store4(w + e, x, left);
+      pmg_store4(p + e, x, left);
     }
   }
 }
@@ -381,15 +378,14 @@ __global__ __launch_bounds__(THREADS) void adamw_kernel(const AdamwTable t, cons
 template <bool SIGNED>
 __global__ __launch_bounds__(THREADS) void values_kernel(const uint8_t* __restrict__ code, const float* __restrict__ top,
                                                          int64_t n, float* __restrict__ out) {
-  const bool alc = ((uintptr_t)code & 3) == 0, alo = pmg_aligned4(out);
   const int64_t lo = (int64_t)blockIdx.x * AW_CHUNK + threadIdx.x * 4;
 #pragma unroll
   for (int u = 0; u < AW_ITER; ++u) {
     const int64_t e = lo + u * (THREADS * 4), left = n - e;
     if (left <= 0) break;
-    const int c = load_codes(code + e, alc, left);
+    const int c = load_codes(code + e, left);
     const float s = top[e / PMG_STATE_BLOCK];
-    pmg_store4(out + e, SIGNED ? decode_m(c, s) : decode_v(c, s), alo, left);
+    pmg_store4(out + e, SIGNED ? decode_m(c, s) : decode_v(c, s), left);
   }
 }
 
