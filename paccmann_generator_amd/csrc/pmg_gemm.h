@@ -73,19 +73,28 @@ template <typename T, int R, bool KC, int WAVES, bool LIST, int KB> struct pmg_o
   const char* src[CNT];
   int64_t step;   // bytes from stage to stage
   int kofs[CNT];  // k of this lane's 16 bytes within a stage
-  // m contiguous with a list: the entries of the rows that this wave fetches in the next stage
+  // m contiguous with a list: the entries of the rows that this wave fetches in the next stage.  An instruction that
+  // covers one or two rows takes them through scalar loads, which do not count among the stages' vector loads; one that
+  // covers more (narrow tiles, of two stages, which wait for all loads anyway) by a load per lane.
   typedef const __attribute__((address_space(4))) int* scalar_list;
   static constexpr int ROWS = KC ? 1 : CNT * 1024 / ROWB;  // of a wave
   static constexpr int RPI = ROWS / CNT > 0 ? ROWS / CNT : 1;
+  static constexpr bool SCALAR = RPI <= 2;
+  static constexpr bool BY_LIST = LIST && !KC;
   scalar_list list;
+  const int* lane_list;
   int64_t row_bytes;
-  int next[LIST && !KC ? ROWS : 1];
+  int next[!BY_LIST ? 1 : SCALAR ? ROWS : CNT];
 
   __device__ __forceinline__ void look_up() {
-    if constexpr (LIST && !KC) {
+    if constexpr (BY_LIST && SCALAR) {
 #pragma unroll
       for (int j = 0; j < ROWS; ++j) next[j] = list[j];
       list += KSTEP;
+    } else if constexpr (BY_LIST) {
+#pragma unroll
+      for (int j = 0; j < CNT; ++j) next[j] = lane_list[kofs[j]];
+      lane_list += KSTEP;
     }
   }
 
@@ -111,9 +120,10 @@ template <typename T, int R, bool KC, int WAVES, bool LIST, int KB> struct pmg_o
         src[j] = (const char*)base + ((LIST ? 0 : (k0 + k) * ld) + m) * (int64_t)sizeof(T);
       }
     }
-    if (LIST && !KC) {
+    if (BY_LIST) {
       row_bytes = ld * (int64_t)sizeof(T);
       list = (scalar_list)(rows + k0) + __builtin_amdgcn_readfirstlane(wave) * ROWS;
+      lane_list = rows + k0;
       look_up();
     }
   }
@@ -126,24 +136,26 @@ template <typename T, int R, bool KC, int WAVES, bool LIST, int KB> struct pmg_o
 #pragma unroll
     for (int j = 0; j < CNT; ++j) {
       const char* from = src[j];
-      if constexpr (LIST && !KC) {
+      if constexpr (BY_LIST && SCALAR) {
         int64_t at = next[j * RPI] * row_bytes;
-#pragma unroll
-        for (int r = 1; r < RPI; ++r) at = lane / (64 / RPI) == r ? next[j * RPI + r] * row_bytes : at;
+        if (RPI == 2) at = lane < 32 ? at : next[j * RPI + RPI - 1] * row_bytes;
         from += at;
+      } else if constexpr (BY_LIST) {
+        from += next[j] * row_bytes;
       } else if (!PART) {
         src[j] += step;
       }
       if (PART) from = kofs[j] < left ? from : (const char*)&pmg_zero16;
       pmg_load_lds16(from, d + j * 1024);
     }
-    if (LIST && !KC && !PART) look_up();
+    if (BY_LIST && !PART) look_up();
   }
 
   // behind a PART stage at the end of k: back by n stages
   __device__ __forceinline__ void back(int64_t n) {
-    if constexpr (LIST && !KC) {
+    if constexpr (BY_LIST) {
       list -= (n + 1) * KSTEP;
+      lane_list -= (n + 1) * KSTEP;
       look_up();
     } else {
 #pragma unroll
@@ -209,6 +221,7 @@ struct pmg_tile {
   static constexpr int LOADS = OpA::CNT + OpB::CNT;  // of a wave and stage
   static constexpr int KK = KB / 64, HI = MI / 2;
   static_assert(MI % 2 == 0, "two halves");
+  static_assert((!OpA::BY_LIST || OpA::SCALAR || STAGES == 2) && !OpB::BY_LIST, "loads that stage() does not count");
 
   OpA a;
   OpB b;

@@ -228,13 +228,32 @@ struct GradArgs {
   int64_t ldo;
   float* acc;            // fp32 [splits][N][M], where the sums go (splits > 1) or are added up over pieces
   int add;               // add what acc holds
+  const uint8_t* used;   // dx: which rows of the batch have a slope;
+  void* zeroed;          // the others become zero here (null: not in this launch)
 };
+
+// Zero rows of dx for 64 rows of the batch that have no slope; a wave takes one row after the other in turn.
+template <typename T>
+__device__ __forceinline__ void zero_rows(const uint8_t* __restrict__ used, int64_t n0, int64_t N, int64_t H, int64_t ldo,
+                                          T* __restrict__ dx) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  uint64_t left = __ballot(n0 + lane < N && !used[n0 + lane]);
+  for (int k = 0; left; ++k, left &= left - 1) {
+    if (k % waves != wave) continue;
+    T* row = dx + (n0 + __ffsll((unsigned long long)left) - 1) * ldo;
+    for (int64_t c = lane * 4; c < H; c += 256) pmg_store4(row + c, f32x4{0.f, 0.f, 0.f, 0.f}, H - c);
+  }
+}
 
 template <typename T, int S, bool BKC>
 __global__ __launch_bounds__(THREADS_OF<S>) void lce_grad_kernel(const GradArgs a) {
   typedef TileOf<T, S, false, BKC, !BKC, false> Tile;
   constexpr int BM = SHAPES[S].BM, BN = SHAPES[S].BN, WM = SHAPES[S].WM, WN = SHAPES[S].WN;
   extern __shared__ __attribute__((aligned(16))) char smem[];
+  if (BKC && (int64_t)blockIdx.x >= (int64_t)a.tiles_m * a.tiles_n) {  // behind the tiles
+    if (blockIdx.y == 0) zero_rows(a.used, ((int64_t)blockIdx.x - (int64_t)a.tiles_m * a.tiles_n) * 64, a.N, a.M, a.ldo, (T*)a.zeroed);
+    return;
+  }
   int tm, tn;
   pmg_tile_of(blockIdx.x, a.tiles_m, a.tiles_n, &tm, &tn);
   const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
@@ -265,7 +284,7 @@ __global__ __launch_bounds__(THREADS_OF<S>) void lce_grad_kernel(const GradArgs 
       f32x4 x = acc[i][j] * f;
       float* s = sums + n * a.M + m;
       if (a.add) x += pmg_load4(s, a.M - m);
-      if (a.out && S == SD64) pmg_store4_nt((T*)a.out + o * a.ldo + m, x, a.M - m);
+      if (a.out && S == SD64 && sizeof(T) == 4) pmg_store4_nt((T*)a.out + o * a.ldo + m, x, a.M - m);
       else if (a.out) pmg_store4((T*)a.out + o * a.ldo + m, x, a.M - m);
       else pmg_store4(s, x, a.M - m);
     }
@@ -322,6 +341,8 @@ struct RowArgs {
   float* nll;            // [N], weighted; null: not wanted
   struct LossPart* sums; // [workgroups] or null
   int rows;
+  int mean;
+  float *loss, *count;   // one workgroup: the reduced loss at once
 };
 
 struct LossPart {
@@ -350,6 +371,11 @@ __device__ __forceinline__ LossPart block_sum(double s, int64_t c) {
       p.count += wc[w];
     }
   return p;
+}
+
+__device__ __forceinline__ void reduced_loss(const LossPart& p, int mean, float* loss, float* count) {
+  loss[0] = (float)(mean ? (p.count > 0 ? p.sum / (double)p.count : 0.0) : p.sum);
+  count[0] = (float)p.count;
 }
 
 __global__ __launch_bounds__(1024) void lce_rows_kernel(const RowArgs a) {
@@ -390,7 +416,10 @@ __global__ __launch_bounds__(1024) void lce_rows_kernel(const RowArgs a) {
   }
   if (a.sums) {
     const LossPart p = block_sum((double)nll, in);
-    if (threadIdx.x == 0) a.sums[blockIdx.x] = p;
+    if (threadIdx.x == 0) {
+      if (a.loss) reduced_loss(p, a.mean, a.loss, a.count);
+      else a.sums[blockIdx.x] = p;
+    }
   }
 }
 
@@ -406,13 +435,12 @@ __global__ __launch_bounds__(1024) void lce_loss_kernel(const LossPart* __restri
     c += sums[i].count;
   }
   const LossPart p = block_sum(s, c);
-  if (threadIdx.x == 0) {
-    loss[0] = (float)(mean ? (p.count > 0 ? p.sum / (double)p.count : 0.0) : p.sum);
-    count[0] = (float)p.count;
-  }
+  if (threadIdx.x == 0) reduced_loss(p, mean, loss, count);
 }
 
-// The rows with a slope, in their order: counts per 1024 rows (WRITE false), their scan, the list (WRITE true).
+// The rows with a slope, in their order.  Up to 16 groups of 1024 rows count the rows before theirs by themselves; of
+// more groups the counts (WRITE false) are scanned between two launches.
+constexpr int OWN_GROUPS = 16;
 struct SlopeArgs {
   const float *g_loss, *g_lse, *lse, *count, *weight;
   int per_row, mean;
@@ -470,7 +498,20 @@ template <bool WRITE> __global__ __launch_bounds__(1024) void lce_slopes_kernel(
     if (threadIdx.x == 0) a.first[blockIdx.x] = all;
     return;
   }
-  const int base = a.groups > 1 ? a.first[blockIdx.x] : 0;
+  int base = a.groups > OWN_GROUPS ? a.first[blockIdx.x] : 0;
+  if (a.groups <= OWN_GROUPS && blockIdx.x > 0) {
+    int mine = 0;
+#pragma unroll 4
+    for (int g = 0; g < (int)blockIdx.x; ++g) {
+      const Row q = slope_of(a, (int64_t)g * 1024 + threadIdx.x, common);
+      mine += q.a != 0.0f || q.c != 0.0f;
+    }
+    for (int o = 32; o > 0; o >>= 1) mine += __shfl_xor(mine, o, 64);
+    __shared__ int earlier[16];
+    if (lane == 0) earlier[wave] = mine;
+    __syncthreads();
+    for (int w = 0; w < 16; ++w) base += earlier[w];
+  }
   if (n < a.N) a.used[n] = used;
   if (used) {
     const int at = base + before + __popcll(mask & ((1ull << lane) - 1));
@@ -507,21 +548,6 @@ __global__ __launch_bounds__(1024) void lce_scan_kernel(int* __restrict__ first,
   }
 }
 
-// zero rows of the gradient of hidden for the rows without a slope; a workgroup looks at 64 rows, a wave takes every
-// fourth of those it finds
-template <typename T>
-__global__ __launch_bounds__(256) void lce_zero_rows_kernel(const uint8_t* __restrict__ used, int64_t N, int64_t H,
-                                                            T* __restrict__ dx) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t n0 = (int64_t)blockIdx.x * 64;
-  uint64_t left = __ballot(n0 + lane < N && !used[n0 + lane]);
-  for (int k = 0; left; ++k, left &= left - 1) {
-    if ((k & 3) != wave) continue;
-    T* row = dx + (n0 + __ffsll((unsigned long long)left) - 1) * H;
-    for (int64_t c = lane * 4; c < H; c += 256) pmg_store4(row + c, f32x4{0.f, 0.f, 0.f, 0.f}, H - c);
-  }
-}
-
 // rows of `width` elements, `ld` apart, into rows of `wide` (a multiple of 16 bytes), zero behind the end
 template <typename T>
 __global__ __launch_bounds__(256) void lce_pack_kernel(const T* __restrict__ src, int64_t ld, int64_t rows, int64_t width,
@@ -540,50 +566,55 @@ constexpr int CUS = 256;
 
 int64_t tiles_of(int s, int64_t M, int64_t N) { return div_up(M, SHAPES[s].BM) * div_up(N, SHAPES[s].BN); }
 
-// The square whose rounds over the chip cost least: a round runs per_cu tiles on every CU; against the large one's
-// rate the middle one has 0.85 of it, the small one 0.6.
-int best_square(int64_t M, int64_t N) {
+// Parts of a long sum where there are too few tiles for the chip; at least eight stages a part.
+int splits_of(int s, int64_t M, int64_t N, int64_t K, int64_t eb) {
+  const int64_t tiles = tiles_of(s, M, N), slots = (int64_t)CUS * SHAPES[s].per_cu;
+  if (tiles * 2 > slots) return 1;
+  const int64_t want = slots / tiles, most = div_up(K * eb, (int64_t)SHAPES[s].KB * 8);
+  return (int)(want < 1 || most < 1 ? 1 : want < most ? (want < 1024 ? want : 1024) : (most < 1024 ? most : 1024));
+}
+
+// Microseconds that a product of this shape takes, roughly: rounds of per_cu tiles on every CU, each as long as its
+// products at the rate the shape reaches on a full chip (a CU: 4.6 Tflop/s in bf16, 0.55 in fp32; the middle square 0.85
+// of it, the small one 0.6) and a start of 3 us; one tile a CU does not write its result under another's products;
+// split sums are written and read once more.
+double cost_of(int s, int64_t M, int64_t N, int64_t K, int64_t eb, bool split) {
+  const Shape& h = SHAPES[s];
+  const int splits = split ? splits_of(s, M, N, K, eb) : 1;
+  const double rate = (eb == 2 ? 4.6e6 : 0.55e6) * (s == S256 ? 1.0 : s == S64 ? 0.6 : 0.85);
+  const double rounds = (double)div_up(tiles_of(s, M, N) * splits, (int64_t)CUS * h.per_cu);
+  const double area = (double)h.BM * h.BN, k = (double)div_up(K, splits);
+  double us = rounds * (h.per_cu * area * k * 2 / rate + 3 + (h.per_cu == 1 ? area * (splits > 1 ? 4 : eb) * CUS / 4e6 : 0));
+  if (splits > 1) us += 4 + (double)M * N * (8 * splits + eb) / 4e6;
+  return us;
+}
+
+int best_square(int64_t M, int64_t N, int64_t K, int64_t eb, bool split) {
   int best = S256;
-  double least = 0;
-  for (int s = S256; s <= S64; ++s) {
-    const int64_t t = tiles_of(s, M, N);
-    const double rounds = (double)div_up(t, (int64_t)CUS * SHAPES[s].per_cu);
-    const double cost = rounds * SHAPES[s].per_cu * SHAPES[s].BM * SHAPES[s].BN * (s == S256 ? 1.0 : s == S128 ? 1 / 0.85 : 1 / 0.6);
-    if (s == S256 || cost < least) {
-      best = s;
-      least = cost;
-    }
-  }
+  for (int s = S128; s <= S64; ++s)
+    if (cost_of(s, M, N, K, eb, split) < cost_of(best, M, N, K, eb, split)) best = s;
   return best;
 }
 
-int logits_shape(int64_t V, int64_t N, bool backward) {
+int logits_shape(int64_t V, int64_t N, int64_t H, int64_t eb, bool backward) {
   if (!backward && N <= 64) {
     if (N <= 16) return div_up(V, 128) >= 3 * CUS ? SK16W : SK16;
     return N <= 32 ? SK32 : SK64;
   }
   if (V <= 64) return div_up(N, 128) >= CUS ? SM64 : S64;
-  return best_square(V, N);
+  return best_square(V, N, H, eb, false);
 }
 
 // A short sum (few vocabulary entries) is bound by writing dx: small tiles, several a CU, so that some write while
-// others multiply, and stores that pass the caches by (fp32, 524288 x 512 over 60: 380 us; 410 us with plain stores, 478
-// us with 64 x 256, 506 us with the large square).
-int dx_shape(int64_t H, int64_t N, int64_t K) { return K <= 256 && H > 64 ? SD64 : best_square(H, N); }
-
-int dw_shape(int64_t H, int64_t V) {
-  if (V <= 64 && H > 64) return SN64;
-  return best_square(H, V);
+// others multiply, and in fp32 stores that pass the caches by (524288 x 512 over 60: 380 us; 410 us with plain stores, 478
+// us with 64 x 256, 506 us with the large square; bf16 stores of 8 bytes a lane need the cache to become whole lines).
+int dx_shape(int64_t H, int64_t N, int64_t K, int64_t eb, bool split) {
+  return K <= 256 && H > 64 ? SD64 : best_square(H, N, K, eb, split);
 }
 
-// Parts of a long sum when there are too few tiles for the chip; at least eight stages a part.
-int splits_of(int s, int64_t M, int64_t N, int64_t K, int kstep) {
-  const int64_t tiles = tiles_of(s, M, N), slots = (int64_t)CUS * SHAPES[s].per_cu;
-  if (tiles * 2 > slots) return 1;
-  int64_t want = slots / tiles;
-  const int64_t most = div_up(K, (int64_t)kstep * 8);
-  if (want > most) want = most;
-  return want < 1 ? 1 : want > 1024 ? 1024 : (int)want;
+int dw_shape(int64_t H, int64_t V, int64_t N, int64_t eb) {
+  if (V <= 64 && H > 64) return SN64;
+  return best_square(H, V, N, eb, true);
 }
 
 struct Problem {
@@ -592,7 +623,6 @@ struct Problem {
   bool pack_x, pack_w;
   int64_t Hp;       // hidden size of packed rows
   size_t eb;
-  int kstep;
 };
 
 // Vocabulary entries of a backward piece: dl of a piece takes about 256 MB.  8192 tokens over 128000 (2 GB in one piece):
@@ -637,7 +667,7 @@ Layout fwd_layout(const Problem& p) {
   Taker take;
   L.xp = take(p.pack_x ? (size_t)p.N * p.Hp * p.eb : 0);
   L.wp = take(p.pack_w ? (size_t)p.V * p.Hp * p.eb : 0);
-  const int s = logits_shape(p.V, p.N, false);
+  const int s = logits_shape(p.V, p.N, p.Hp, (int64_t)p.eb, false);
   L.part = take((size_t)div_up(p.V, SHAPES[s].BM) * p.N * sizeof(float2));
   L.at = take((size_t)p.N * 4);
   L.sums = take((size_t)div_up(p.N, rows_of(p.N, div_up(p.V, SHAPES[s].BM))) * sizeof(LossPart));
@@ -656,11 +686,12 @@ BwdPlan bwd_plan(const Problem& p) {
   b.piece = piece_of(p);
   b.pieces = div_up(p.V, b.piece);
   b.ldl = up(b.piece, 64);
-  b.s_dl = logits_shape(b.piece, p.N, true);
-  b.s_dx = dx_shape(p.H, p.N, b.piece);
-  b.s_dw = dw_shape(p.H, b.piece);
-  b.split_dx = b.pieces == 1 ? splits_of(b.s_dx, p.H, p.N, b.piece, p.kstep) : 1;
-  b.split_dw = splits_of(b.s_dw, p.H, b.piece, p.N, p.kstep);
+  const int64_t eb = (int64_t)p.eb;
+  b.s_dl = logits_shape(b.piece, p.N, p.Hp, eb, true);
+  b.s_dx = dx_shape(p.H, p.N, b.piece, eb, b.pieces == 1);
+  b.s_dw = dw_shape(p.H, b.piece, p.N, eb);
+  b.split_dx = b.pieces == 1 ? splits_of(b.s_dx, p.H, p.N, b.piece, eb) : 1;
+  b.split_dw = splits_of(b.s_dw, p.H, b.piece, p.N, eb);
   return b;
 }
 
@@ -691,7 +722,6 @@ int problem_of(const pmg_linear_ce* a, Problem* p) {
   if (a->reduction != PMG_REDUCE_NONE && a->reduction != PMG_REDUCE_SUM && a->reduction != PMG_REDUCE_MEAN) return PMG_E_ARG;
   p->N = a->N; p->V = a->V; p->H = a->H; p->dtype = a->dtype;
   p->eb = pmg_elem_bytes(a->dtype);
-  p->kstep = (int)(128 / p->eb);
   const int64_t e16 = 16 / (int64_t)p->eb;
   p->Hp = up(a->H, e16);
   // 16-byte loads: rows that do not begin at multiples of 16 bytes, or whose end does not, are copied to rows that do
@@ -734,7 +764,9 @@ template <typename T, bool BACKWARD> int logits(int s, LogitArgs a, hipStream_t 
 template <typename T, int S, bool BKC> int launch_grad(const GradArgs& a, hipStream_t st) {
   static std::atomic<unsigned long long> done{0};
   if (const hipError_t e = pmg_full_lds_once((const void*)&lce_grad_kernel<T, S, BKC>, &done)) return (int)e;
-  hipLaunchKernelGGL((lce_grad_kernel<T, S, BKC>), dim3((unsigned)((int64_t)a.tiles_m * a.tiles_n), a.splits), dim3(THREADS_OF<S>),
+  const int64_t blocks = (int64_t)a.tiles_m * a.tiles_n + (BKC && a.zeroed ? div_up(a.N, 64) : 0);
+  if (blocks > 0x7fffffff) return PMG_E_ARG;
+  hipLaunchKernelGGL((lce_grad_kernel<T, S, BKC>), dim3((unsigned)blocks, a.splits), dim3(THREADS_OF<S>),
                      (TileOf<T, S, false, BKC, !BKC, false>::LDS), st, a);
   return (int)hipGetLastError();
 }
@@ -800,7 +832,7 @@ template <typename T> int forward(const pmg_linear_ce* a, const Problem& p, char
   l.v0 = 0;
   l.part = (float2*)(ws + L.part);
   l.at_target = (float*)(ws + L.at);
-  const int s = logits_shape(p.V, p.N, false);
+  const int s = logits_shape(p.V, p.N, p.Hp, (int64_t)p.eb, false);
   if (const int rc = logits<T, false>(s, l, st)) return rc;
   RowArgs r = {};
   r.part = l.part;
@@ -815,10 +847,14 @@ template <typename T> int forward(const pmg_linear_ce* a, const Problem& p, char
   r.sums = none ? nullptr : (LossPart*)(ws + L.sums);
   r.rows = rows_of(p.N, r.tiles);
   const int groups = (int)div_up(p.N, r.rows);
+  r.mean = a->reduction == PMG_REDUCE_MEAN;
+  if (groups == 1 && !none) {
+    r.loss = a->loss;
+    r.count = a->count;
+  }
   hipLaunchKernelGGL(lce_rows_kernel, dim3((unsigned)groups), dim3(1024), 0, st, r);
-  if (!none)
-    hipLaunchKernelGGL(lce_loss_kernel, dim3(1), dim3(1024), 0, st, r.sums, groups, a->reduction == PMG_REDUCE_MEAN, a->loss,
-                       a->count);
+  if (!none && groups > 1)
+    hipLaunchKernelGGL(lce_loss_kernel, dim3(1), dim3(1024), 0, st, r.sums, groups, r.mean, a->loss, a->count);
   return (int)hipGetLastError();
 }
 
@@ -841,14 +877,11 @@ template <typename T> int backward(const pmg_linear_ce* a, const Problem& p, cha
   sl.scale = a->logit_scale;
   sl.factor = (float*)(ws + L.factor);
   sl.used = (uint8_t*)(ws + L.used);
-  if (sl.groups > 1) {
+  if (sl.groups > OWN_GROUPS) {
     hipLaunchKernelGGL(lce_slopes_kernel<false>, dim3(sl.groups), dim3(1024), 0, st, sl);
     hipLaunchKernelGGL(lce_scan_kernel, dim3(1), dim3(1024), 0, st, sl.first, sl.groups);
   }
   hipLaunchKernelGGL(lce_slopes_kernel<true>, dim3(sl.groups), dim3(1024), 0, st, sl);
-  if (a->grad_hidden)
-    hipLaunchKernelGGL(lce_zero_rows_kernel<T>, dim3((unsigned)div_up(p.N, 64)), dim3(256), 0, st, sl.used, p.N, p.H,
-                       (T*)a->grad_hidden);
   l.row = sl.row;
   l.list = sl.list;
   l.count = sl.total;
@@ -881,6 +914,8 @@ template <typename T> int backward(const pmg_linear_ce* a, const Problem& p, cha
       g.ldo = p.H;
       g.acc = b.pieces > 1 || b.split_dx > 1 ? (float*)(ws + L.dxacc) : nullptr;
       g.add = i > 0;
+      g.used = sl.used;
+      g.zeroed = i == 0 ? a->grad_hidden : nullptr;
       if (const int rc = grad<T, true>(b.s_dx, g, st)) return rc;
     }
     if (a->grad_weight) {
