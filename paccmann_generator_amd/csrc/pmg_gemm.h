@@ -14,7 +14,11 @@
 //                 reads (ds_read_b64_tr_b16), an fp32 fragment four single ones
 // An operand may be read through a list of its rows (of m or n where k is contiguous, of k otherwise): the
 // training rows of a batch stay where they are.
-// Lane l of a wave holds of a 16x16 tile of D column n = l & 15 and rows m = 4 (l >> 4) .. + 3.
+// Lane l of a wave holds of a 16x16 tile of D column n = l & 15 and four rows m.  Which rows of m a fragment of A has is
+// free: in bf16 two fragments share 32 rows so that a lane's eight are neighbours (8 (l >> 4) .. + 7, the first four in
+// fragment i for even l >> 4 and in i + 1 for odd: half of the lanes read the other half of 16 bytes, which keeps all
+// banks busy) and are stored as 16 bytes, 64 in a row with the lanes beside it; in fp32 four are 16 bytes already (m =
+// 4 (l >> 4) .. + 3).
 #pragma once
 #include "pmg_kernels.h"
 #include "pmg_types.h"
@@ -49,8 +53,8 @@ __device__ __forceinline__ void pmg_load_lds16(const char* src, lds_char* dst) {
 }
 
 // One operand's share of a stage: R rows of m (or n), 128 bytes of k.
-//   KC: k contiguous.  WAVES waves fill it, 1 KB an instruction.  LIST: rows by a list.
-template <typename T, int R, bool KC, int WAVES, bool LIST, int KB> struct pmg_operand {
+//   KC: k contiguous.  WAVES waves fill it, 1 KB an instruction.  LIST: rows by a list.  PAIR: fragments share 32 rows.
+template <typename T, int R, bool KC, int WAVES, bool LIST, int KB, bool PAIR> struct pmg_operand {
   static constexpr int E16 = 16 / sizeof(T);
   static constexpr int KSTEP = KB / sizeof(T);
   static constexpr int BYTES = R * KB;
@@ -62,11 +66,13 @@ template <typename T, int R, bool KC, int WAVES, bool LIST, int KB> struct pmg_o
   static_assert(KC || PIECES >= 8, "the permutation stays inside a row");
 
   static __device__ __forceinline__ int perm(int k) {  // of the 16-byte pieces of row k (m contiguous)
+    if (PAIR) return ((k & 1) | (((k >> 1) & 1) << 2) | (((k >> 3) & 1) << 3)) & (PIECES - 1);
     if (sizeof(T) == 2) return (((k & 3) | (((k >> 3) & 3) << 2)) & (PIECES / 2 - 1)) << 1;
     return (((k >> 2) & 3) << 2) & (PIECES - 1);
   }
 
   static __device__ __forceinline__ int perm_k(int row) {  // of the pieces of a row (k contiguous)
+    if (PAIR) return KB == 128 ? ((row >> 1) & 1) | (((row >> 3) & 3) << 1) : (row >> 3) & 3;
     return KB == 128 ? row & 7 : (row >> 2) & 3;
   }
 
@@ -137,9 +143,10 @@ template <typename T, int R, bool KC, int WAVES, bool LIST, int KB> struct pmg_o
     for (int j = 0; j < CNT; ++j) {
       const char* from = src[j];
       if constexpr (BY_LIST && SCALAR) {
-        int64_t at = next[j * RPI] * row_bytes;
-        if (RPI == 2) at = lane < 32 ? at : next[j * RPI + RPI - 1] * row_bytes;
-        from += at;
+        // (named scalar values: a choice between two elements would make the array's index depend on the lane)
+        const int64_t at = __builtin_amdgcn_readfirstlane(next[j * RPI]) * row_bytes;
+        const int64_t behind = __builtin_amdgcn_readfirstlane(next[j * RPI + RPI - 1]) * row_bytes;
+        from += RPI == 2 && lane >= 32 ? behind : at;
       } else if constexpr (BY_LIST) {
         from += next[j] * row_bytes;
       } else if (!PART) {
@@ -164,34 +171,37 @@ template <typename T, int R, bool KC, int WAVES, bool LIST, int KB> struct pmg_o
   }
 
   typedef typename pmg_frag<T>::type frag;
-  // the fragment of rows row .. row + 15 (of this operand's R) for half kk of the stage
-  static __device__ __forceinline__ frag read(const lds_char* s, int row, int kk) {
+  // fragment f of the rows from `row` (of this operand's R) for half kk of the stage
+  static __device__ __forceinline__ frag read(const lds_char* s, int row, int f, int kk) {
     const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
+    // where the q-th four of its rows begins
+    const auto quad = [&](int q) { return row + (PAIR ? (f >> 1) * 32 + 8 * q + 4 * ((f ^ q) & 1) : f * 16 + 4 * q); };
     if (KC) {
-      const int r = row + i;
+      const int r = quad(i >> 2) + (i & 3);
       return *(const __attribute__((address_space(3))) frag*)(s + r * KB + (((kk * 4 + g) ^ perm_k(r)) << 4));
     } else if constexpr (sizeof(T) == 2) {
-      frag f;
+      frag out;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int k = kk * 32 + 8 * g + 4 * h + (i >> 2);
-        const int c = (row >> 3) + ((i & 3) >> 1);
+        const int m = quad(i & 3), c = m >> 3;
         typedef short s16x4 __attribute__((ext_vector_type(4)));
         const s16x4 t = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (__attribute__((address_space(3))) s16x4*)(s + k * ROWB + ((c ^ perm(k)) << 4) + ((i & 1) << 3)));
+            (__attribute__((address_space(3))) s16x4*)(s + k * ROWB + ((c ^ perm(k)) << 4) + ((m & 4) << 1)));
         const bf16x4 v = __builtin_bit_cast(bf16x4, t);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) f[4 * h + j] = v[j];
+        for (int j = 0; j < 4; ++j) out[4 * h + j] = v[j];
       }
-      return f;
+      return out;
     } else {
-      frag f;
+      static_assert(!PAIR, "fp32");
+      frag out;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int k = kk * 16 + 4 * g + j, m = row + i;
-        f[j] = *(const __attribute__((address_space(3))) float*)(s + k * ROWB + (((m >> 2) ^ perm(k)) << 4) + ((m & 3) << 2));
+        const int k = kk * 16 + 4 * g + j, m = quad(0) + i;
+        out[j] = *(const __attribute__((address_space(3))) float*)(s + k * ROWB + (((m >> 2) ^ perm(k)) << 4) + ((m & 3) << 2));
       }
-      return f;
+      return out;
     }
   }
 };
@@ -213,8 +223,9 @@ template <typename T, int BM, int BN, int WM, int WN, bool AKC, bool BKC, bool A
 struct pmg_tile {
   static constexpr int WAVES = WM * WN, THREADS = WAVES * 64;
   static constexpr int MI = BM / WM / 16, NI = BN / WN / 16;
-  typedef pmg_operand<T, BM, AKC, WAVES, ALIST, KB> OpA;
-  typedef pmg_operand<T, BN, BKC, WAVES, BLIST, KB> OpB;
+  static constexpr bool PAIR = sizeof(T) == 2;
+  typedef pmg_operand<T, BM, AKC, WAVES, ALIST, KB, PAIR> OpA;
+  typedef pmg_operand<T, BN, BKC, WAVES, BLIST, KB, false> OpB;
   static constexpr int STAGE = OpA::BYTES + OpB::BYTES;
   static constexpr int LDS = STAGES * STAGE;
   static constexpr int KSTEP = OpA::KSTEP;
@@ -222,6 +233,16 @@ struct pmg_tile {
   static constexpr int KK = KB / 64, HI = MI / 2;
   static_assert(MI % 2 == 0, "two halves");
   static_assert((!OpA::BY_LIST || OpA::SCALAR || STAGES == 2) && !OpB::BY_LIST, "loads that stage() does not count");
+
+  // row of acc[i][.][0] of lane 0 .. 63 in the wave's part of m
+  static __device__ __forceinline__ int row_of(int i) {
+    const int g = (threadIdx.x & 63) >> 4;
+    return PAIR ? (i >> 1) * 32 + 8 * g + 4 * ((i ^ g) & 1) : i * 16 + 4 * g;
+  }
+
+  // PAIR: the first row of a lane's eight in fragments i and i + 1 (i even), and whether fragment i has the upper four
+  static __device__ __forceinline__ int pair_of(int i) { return (i >> 1) * 32 + 8 * ((threadIdx.x & 63) >> 4); }
+  static __device__ __forceinline__ bool swapped() { return (threadIdx.x >> 4) & 1; }
 
   OpA a;
   OpB b;
@@ -231,11 +252,11 @@ struct pmg_tile {
 
   __device__ __forceinline__ void read_a(const lds_char* s, int half, int kk) {
 #pragma unroll
-    for (int i = 0; i < HI; ++i) fa[half][i] = OpA::read(s, rowA + (half * HI + i) * 16, kk);
+    for (int i = 0; i < HI; ++i) fa[half][i] = OpA::read(s, rowA, half * HI + i, kk);
   }
   __device__ __forceinline__ void read_b(const lds_char* s, int set, int kk) {
 #pragma unroll
-    for (int j = 0; j < NI; ++j) fb[set][j] = OpB::read(s + OpA::BYTES, rowB + j * 16, kk);
+    for (int j = 0; j < NI; ++j) fb[set][j] = OpB::read(s + OpA::BYTES, rowB, j, kk);
   }
   __device__ __forceinline__ void multiply(f32x4 (&acc)[MI][NI], int half, int set) {
 #pragma unroll

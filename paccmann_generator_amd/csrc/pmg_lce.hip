@@ -101,7 +101,8 @@ __global__ __launch_bounds__(THREADS_OF<S>) void lce_logits_kernel(const LogitAr
 
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / WN, wn = wave % WN;
   const int g = lane >> 4, col = lane & 15;
-  const int64_t mw = m0 + wm * (BM / WM) + 4 * g;  // this lane's rows: mw + 16 i + e
+  const int64_t mw = m0 + wm * (BM / WM);               // this lane's rows: mw + row_of(i) + e
+  const int rows = a.V - mw < BM ? (int)(a.V - mw) : BM;  // of them in the vocabulary (may be none)
   const T* bias = (const T*)a.bias;
   // logits; entries behind the vocabulary's end do not take part
 #pragma unroll
@@ -110,13 +111,13 @@ __global__ __launch_bounds__(THREADS_OF<S>) void lce_logits_kernel(const LogitAr
     if (bias) {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (mw + i * 16 + e < a.V) b[e] = (float)bias[mw + i * 16 + e];
+        if (Tile::row_of(i) + e < rows) b[e] = (float)bias[mw + Tile::row_of(i) + e];
     }
 #pragma unroll
     for (int j = 0; j < NI; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        acc[i][j][e] = mw + i * 16 + e < a.V ? (acc[i][j][e] + b[e]) * a.scale : -__builtin_inff();
+        acc[i][j][e] = Tile::row_of(i) + e < rows ? (acc[i][j][e] + b[e]) * a.scale : -__builtin_inff();
   }
 
   if constexpr (!BACKWARD) {
@@ -141,12 +142,14 @@ __global__ __launch_bounds__(THREADS_OF<S>) void lce_logits_kernel(const LogitAr
       sum += __shfl_xor(sum, 32, 64);
       if (g == 0) red[wm * BN + wn * (BN / WN) + j * 16 + col] = make_float2(top, sum);
       if (n < a.N) {
-        const int64_t t = target_of(a.targets, a.id_bits, n) - a.v0;
+        const int64_t t = target_of(a.targets, a.id_bits, n) - a.v0 - mw;
+        if (t >= 0 && t < rows) {
 #pragma unroll
-        for (int i = 0; i < MI; ++i)
+          for (int i = 0; i < MI; ++i)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (mw + i * 16 + e == t && t < a.V) a.at_target[n] = acc[i][j][e];
+            for (int e = 0; e < 4; ++e)
+              if (Tile::row_of(i) + e == (int)t) a.at_target[n] = acc[i][j][e];
+        }
       }
     }
     __syncthreads();
@@ -163,30 +166,35 @@ __global__ __launch_bounds__(THREADS_OF<S>) void lce_logits_kernel(const LogitAr
     }
   } else {
     T* dl = (T*)a.dl;
-    float db[MI][4];
-#pragma unroll
-    for (int i = 0; i < MI; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) db[i][e] = 0.0f;
+    const int wide = a.ldl - mw < BM ? (int)(a.ldl - mw) : BM;  // ldl is a multiple of 64
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
       const int64_t n = n0 + wn * (BN / WN) + j * 16 + col;
+      Row r = {0.0f, 0.0f, 0.0f, -1};
+      if (n < N) r = a.row[n];
+      const int64_t behind = (int64_t)r.target - a.v0 - mw;
+      const int t = behind >= 0 && behind < rows ? (int)behind : -1;
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          // entries behind the vocabulary's end and rows behind the last are zero
+          float x = n < N && Tile::row_of(i) + e < rows ? r.a * exp_of<T>(acc[i][j][e] - r.lse) : 0.0f;
+          if (Tile::row_of(i) + e == t) x -= r.c;
+          acc[i][j][e] = x;
+        }
       if (n < N) {
-        const Row r = a.row[n];
-        const int64_t t = (int64_t)r.target - a.v0;
+        T* to = dl + n * a.ldl + mw;
 #pragma unroll
-        for (int i = 0; i < MI; ++i) {
-          f32x4 d;
+        for (int i = 0; i < MI; i += 2) {
+          if constexpr (Tile::PAIR) {
+            const bool up = Tile::swapped();
+            if (Tile::pair_of(i) < wide) pmg_store8(to + Tile::pair_of(i), up ? acc[i + 1][j] : acc[i][j], up ? acc[i][j] : acc[i + 1][j], 8);
+          } else {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int64_t v = mw + i * 16 + e;
-            float x = v < a.V ? r.a * exp_of<T>(acc[i][j][e] - r.lse) : 0.0f;  // entries behind the end are zero
-            if (v == t && v < a.V) x -= r.c;
-            d[e] = x;
-            db[i][e] += x;
+            for (int h = 0; h < 2; ++h)
+              if (Tile::row_of(i + h) < wide) pmg_store4(to + Tile::row_of(i + h), acc[i + h][j]);
           }
-          const int64_t v = mw + i * 16;
-          if (v < a.ldl) pmg_store4(dl + n * a.ldl + v, d);  // ldl is a multiple of 64
         }
       }
     }
@@ -196,12 +204,14 @@ __global__ __launch_bounds__(THREADS_OF<S>) void lce_logits_kernel(const LogitAr
       for (int i = 0; i < MI; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          float s = db[i][e];
+          float s = 0.0f;
+#pragma unroll
+          for (int j = 0; j < NI; ++j) s += acc[i][j][e];
           s += __shfl_xor(s, 1, 64);
           s += __shfl_xor(s, 2, 64);
           s += __shfl_xor(s, 4, 64);
           s += __shfl_xor(s, 8, 64);
-          if (col == 0) red[wn * BM + wm * (BM / WM) + i * 16 + 4 * g + e] = s;
+          if (col == 0) red[wn * BM + wm * (BM / WM) + Tile::row_of(i) + e] = s;
         }
       __syncthreads();
       for (int r = threadIdx.x; r < BM; r += Tile::THREADS) {
@@ -262,7 +272,7 @@ __global__ __launch_bounds__(THREADS_OF<S>) void lce_grad_kernel(const GradArgs 
   const int64_t steps = (K + Tile::KSTEP - 1) / Tile::KSTEP, per = (steps + a.splits - 1) / a.splits * Tile::KSTEP;
   const int64_t k0 = per * blockIdx.y, k1 = k0 + per < K ? k0 + per : K;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t mw = m0 + (wave / WN) * (BM / WM) + 4 * (lane >> 4), nw = n0 + (wave % WN) * (BN / WN) + (lane & 15);
+  const int64_t mw = m0 + (wave / WN) * (BM / WM), nw = n0 + (wave % WN) * (BN / WN) + (lane & 15);
   int place[Tile::NI];  // of this lane's rows of the result
   if (BKC) {
 #pragma unroll
@@ -278,15 +288,21 @@ __global__ __launch_bounds__(THREADS_OF<S>) void lce_grad_kernel(const GradArgs 
     if (n >= N) continue;
     const int64_t o = BKC ? place[j] : n;
 #pragma unroll
-    for (int i = 0; i < Tile::MI; ++i) {
-      const int64_t m = mw + i * 16;
-      if (m >= a.M) continue;
-      f32x4 x = acc[i][j] * f;
-      float* s = sums + n * a.M + m;
-      if (a.add) x += pmg_load4(s, a.M - m);
-      if (a.out && S == SD64 && sizeof(T) == 4) pmg_store4_nt((T*)a.out + o * a.ldo + m, x, a.M - m);
-      else if (a.out) pmg_store4((T*)a.out + o * a.ldo + m, x, a.M - m);
-      else pmg_store4(s, x, a.M - m);
+    for (int i = 0; i < Tile::MI; i += 2) {
+      f32x4 x[2] = {acc[i][j] * f, acc[i + 1][j] * f};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int64_t m = mw + Tile::row_of(i + h), left = a.M - m;
+        if (left <= 0) continue;
+        float* s = sums + n * a.M + m;
+        if (a.add) x[h] += pmg_load4(s, left);
+        if (!a.out) pmg_store4(s, x[h], left);
+        else if (!Tile::PAIR && S == SD64) pmg_store4_nt((T*)a.out + o * a.ldo + m, x[h], left);
+        else if (!Tile::PAIR) pmg_store4((T*)a.out + o * a.ldo + m, x[h], left);
+      }
+      const int64_t m = mw + Tile::pair_of(i);
+      const bool up = Tile::swapped();
+      if (Tile::PAIR && a.out && m < a.M) pmg_store8((T*)a.out + o * a.ldo + m, up ? x[1] : x[0], up ? x[0] : x[1], a.M - m);
     }
   }
 }

@@ -46,6 +46,22 @@ template <typename T> __device__ __forceinline__ void pmg_store4_nt(T* p, f32x4 
   __builtin_nontemporal_store(v, reinterpret_cast<mem*>(p));
 }
 
+// eight elements of which `left` (>= 1) remain
+template <typename T> __device__ __forceinline__ void pmg_store8(T* p, f32x4 x, f32x4 y, int64_t left) {
+  if (left >= 8) {
+    typename pmg_vec<T, 8>::type v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[j] = (T)x[j];
+      v[4 + j] = (T)y[j];
+    }
+    *reinterpret_cast<typename pmg_vec<T, 8>::in_memory*>(p) = v;
+    return;
+  }
+  pmg_store4(p, x, left);
+  if (left > 4) pmg_store4(p + 4, y, left - 4);
+}
+
 static inline size_t pmg_elem_bytes(int dtype) { return dtype == PMG_F32 ? 4 : 2; }
 static inline bool pmg_dtype_ok(int dtype) { return dtype == PMG_F32 || dtype == PMG_BF16 || dtype == PMG_F16; }
 
