@@ -82,6 +82,8 @@ typedef struct pmg_linear_ce {
   void* grad_hidden;       /* [N,H] contiguous */
   void* grad_weight;       /* [V,H] contiguous */
   void* grad_bias;         /* [V] */
+  float* logits;           /* [N, V rounded up to a multiple of 4], 16-byte aligned, or NULL; forward: written (behind a
+                              row's V entries: anything), backward: read in place of forming them again */
 } pmg_linear_ce;
 
 /* Bytes of scratch of one direction.  It does not grow with N x V: the backward keeps the slopes of a

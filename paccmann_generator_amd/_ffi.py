@@ -79,7 +79,7 @@ class PmgLinearCe(C.Structure):
         ('reduction', C.c_int), ('logit_scale', C.c_float), ('ignore_index', C.c_int64), ('ld_hidden', C.c_int64),
         ('ld_weight', C.c_int64), ('hidden', _F), ('weight', _F), ('bias', _F), ('targets', _F), ('row_weight', _F),
         ('loss', _F), ('lse', _F), ('count', _F), ('grad_loss', _F), ('grad_lse', _F), ('grad_hidden', _F),
-        ('grad_weight', _F), ('grad_bias', _F),
+        ('grad_weight', _F), ('grad_bias', _F), ('logits', _F),
     ]
 
 

@@ -1,5 +1,5 @@
 // Cross entropy of a linear vocabulary projection, with its gradients (include/pmg_lm.h); the logits are
-// never kept.
+// not kept, unless the caller gives a place for them.
 //
 //   l = s (x W^T + b)     lse_n = log sum_v exp l_nv     nll_n = lse_n - l_{n,t_n}
 //   dl_nv = a_n exp(l_nv - lse_n) - c_n [v = t_n]    dx = f dl W    dW = f dl^T x    db = f sum_n dl_n
@@ -17,7 +17,9 @@
 // Rows without a slope (ignored targets, zero weights) take no part in the backward: the others are listed, the
 // products run over the list, and the rows left out get a zero gradient whatever they hold.
 // Bound by the matrix units for many tokens (8 N V H operations, two of them for the second forming of the
-// logits), by reading W for few.
+// logits), by reading W for few.  With few vocabulary entries kept logits are much shorter than the hidden rows they are
+// made of: the backward reads them and forms nothing again (524288 rows of 512 fp32 over 60: 126 MB in place of 1 GB and a
+// quarter of the operations).
 #include "pmg_gemm.h"
 
 namespace {
@@ -61,6 +63,8 @@ struct LogitArgs {
   float scale;
   const void* targets;
   int id_bits;
+  float* kept;           // logits of all tokens, rows of ldk (a multiple of 4); forward: written, backward: read; or null
+  int64_t ldk;
   // forward
   float2* part;          // [tiles_m][N]
   float* at_target;      // [N]
@@ -85,8 +89,11 @@ struct Row {
 };
 
 // ------------------------------------------------------------------------------------------ logits
-template <typename T, int S, bool BACKWARD>
+enum { FORWARD, REFORM, KEPT };  // the backward forms the logits again, or reads those that were kept
+
+template <typename T, int S, int WAY>
 __global__ __launch_bounds__(THREADS_OF<S>) void lce_logits_kernel(const LogitArgs a) {
+  constexpr bool BACKWARD = WAY != FORWARD;
   typedef TileOf<T, S, true, true, false, BACKWARD> Tile;
   constexpr int BM = SHAPES[S].BM, BN = SHAPES[S].BN, WM = SHAPES[S].WM, WN = SHAPES[S].WN;
   constexpr int MI = Tile::MI, NI = Tile::NI;
@@ -97,30 +104,54 @@ __global__ __launch_bounds__(THREADS_OF<S>) void lce_logits_kernel(const LogitAr
   const int64_t N = BACKWARD ? uniform_of(a.count) : a.N;
   if (BACKWARD && n0 >= N) return;
   f32x4 acc[MI][NI];
-  Tile::run(acc, (lds_char*)smem, a.W, a.ldw, nullptr, m0, a.V, a.X, a.ldx, a.list, n0, N, 0, a.K);
+  if constexpr (WAY != KEPT)
+    Tile::run(acc, (lds_char*)smem, a.W, a.ldw, nullptr, m0, a.V, a.X, a.ldx, a.list, n0, N, 0, a.K);
 
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / WN, wn = wave % WN;
   const int g = lane >> 4, col = lane & 15;
   const int64_t mw = m0 + wm * (BM / WM);               // this lane's rows: mw + row_of(i) + e
   const int rows = a.V - mw < BM ? (int)(a.V - mw) : BM;  // of them in the vocabulary (may be none)
   const T* bias = (const T*)a.bias;
-  // logits; entries behind the vocabulary's end do not take part
+  if constexpr (WAY == KEPT) {
 #pragma unroll
-  for (int i = 0; i < MI; ++i) {
-    f32x4 b = {0.f, 0.f, 0.f, 0.f};
-    if (bias) {
+    for (int j = 0; j < NI; ++j) {
+      const int64_t n = n0 + wn * (BN / WN) + j * 16 + col;
+      const float* from = a.kept + (n < N ? (int64_t)a.list[n] : 0) * a.ldk + a.v0 + mw;
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (Tile::row_of(i) + e < rows) b[e] = (float)bias[mw + Tile::row_of(i) + e];
+      for (int i = 0; i < MI; ++i) {
+        acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (n < N && Tile::row_of(i) < rows) acc[i][j] = *(const f32x4*)(from + Tile::row_of(i));
+      }
     }
+  } else {
+    // logits; entries behind the vocabulary's end do not take part
 #pragma unroll
-    for (int j = 0; j < NI; ++j)
+    for (int i = 0; i < MI; ++i) {
+      f32x4 b = {0.f, 0.f, 0.f, 0.f};
+      if (bias) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        acc[i][j][e] = Tile::row_of(i) + e < rows ? (acc[i][j][e] + b[e]) * a.scale : -__builtin_inff();
+        for (int e = 0; e < 4; ++e)
+          if (Tile::row_of(i) + e < rows) b[e] = (float)bias[mw + Tile::row_of(i) + e];
+      }
+#pragma unroll
+      for (int j = 0; j < NI; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          acc[i][j][e] = Tile::row_of(i) + e < rows ? (acc[i][j][e] + b[e]) * a.scale : -__builtin_inff();
+    }
   }
 
   if constexpr (!BACKWARD) {
+    if (a.kept) {
+#pragma unroll
+      for (int j = 0; j < NI; ++j) {
+        const int64_t n = n0 + wn * (BN / WN) + j * 16 + col;
+        float* to = a.kept + n * a.ldk + mw;
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+          if (n < a.N && Tile::row_of(i) < rows) *(f32x4*)(to + Tile::row_of(i)) = acc[i][j];
+      }
+    }
     float2* red = (float2*)smem;  // [WM][BN]
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
@@ -638,6 +669,7 @@ struct Problem {
   int dtype;
   bool pack_x, pack_w;
   int64_t Hp;       // hidden size of packed rows
+  bool kept;        // logits
   size_t eb;
 };
 
@@ -703,7 +735,7 @@ BwdPlan bwd_plan(const Problem& p) {
   b.pieces = div_up(p.V, b.piece);
   b.ldl = up(b.piece, 64);
   const int64_t eb = (int64_t)p.eb;
-  b.s_dl = logits_shape(b.piece, p.N, p.Hp, eb, true);
+  b.s_dl = p.kept ? S64 : logits_shape(b.piece, p.N, p.Hp, eb, true);  // (kept: no product, any shape)
   b.s_dx = dx_shape(p.H, p.N, b.piece, eb, b.pieces == 1);
   b.s_dw = dw_shape(p.H, b.piece, p.N, eb);
   b.split_dx = b.pieces == 1 ? splits_of(b.s_dx, p.H, p.N, b.piece, eb) : 1;
@@ -740,39 +772,42 @@ int problem_of(const pmg_linear_ce* a, Problem* p) {
   p->eb = pmg_elem_bytes(a->dtype);
   const int64_t e16 = 16 / (int64_t)p->eb;
   p->Hp = up(a->H, e16);
+  p->kept = a->logits != nullptr;
   // 16-byte loads: rows that do not begin at multiples of 16 bytes, or whose end does not, are copied to rows that do
   const bool tail = a->H % e16 != 0;
   p->pack_x = tail || a->ld_hidden % e16 != 0 || ((uintptr_t)a->hidden & 15) != 0;
   p->pack_w = tail || a->ld_weight % e16 != 0 || ((uintptr_t)a->weight & 15) != 0;
   const size_t eb = p->eb;
   if (((uintptr_t)a->hidden | (uintptr_t)a->weight | (uintptr_t)a->bias) & (eb - 1)) return PMG_E_ALIGN;
+  if ((uintptr_t)a->logits & 15) return PMG_E_ALIGN;
   if (((uintptr_t)a->targets & (a->id_bits / 8 - 1)) || ((uintptr_t)a->row_weight & 3)) return PMG_E_ALIGN;
   return PMG_OK;
 }
 
-template <typename T, int S, bool BACKWARD> int launch_logits(const LogitArgs& a, hipStream_t st) {
+template <typename T, int S, int WAY> int launch_logits(const LogitArgs& a, hipStream_t st) {
   static std::atomic<unsigned long long> done{0};
-  if (const hipError_t e = pmg_full_lds_once((const void*)&lce_logits_kernel<T, S, BACKWARD>, &done)) return (int)e;
-  hipLaunchKernelGGL((lce_logits_kernel<T, S, BACKWARD>), dim3((unsigned)((int64_t)a.tiles_m * a.tiles_n)), dim3(THREADS_OF<S>),
-                     (TileOf<T, S, true, true, false, BACKWARD>::LDS), st, a);
+  if (const hipError_t e = pmg_full_lds_once((const void*)&lce_logits_kernel<T, S, WAY>, &done)) return (int)e;
+  // without the product only the sums over the tokens are in LDS
+  constexpr int LDS = WAY == KEPT ? SHAPES[S].WN * SHAPES[S].BM * (int)sizeof(float) : TileOf<T, S, true, true, false, WAY != FORWARD>::LDS;
+  hipLaunchKernelGGL((lce_logits_kernel<T, S, WAY>), dim3((unsigned)((int64_t)a.tiles_m * a.tiles_n)), dim3(THREADS_OF<S>), LDS, st, a);
   return (int)hipGetLastError();
 }
 
-template <typename T, bool BACKWARD> int logits(int s, LogitArgs a, hipStream_t st) {
+template <typename T, int WAY> int logits(int s, LogitArgs a, hipStream_t st) {
   a.tiles_m = (int)div_up(a.V, SHAPES[s].BM);
   a.tiles_n = (int)div_up(a.N, SHAPES[s].BN);
   if ((int64_t)a.tiles_m * a.tiles_n > 0x7fffffff) return PMG_E_ARG;
-  switch (s) {
-    case S256: return launch_logits<T, S256, BACKWARD>(a, st);
-    case S128: return launch_logits<T, S128, BACKWARD>(a, st);
-    case S64: return launch_logits<T, S64, BACKWARD>(a, st);
-    case SM64: return launch_logits<T, SM64, BACKWARD>(a, st);
-  }
-  if constexpr (!BACKWARD) switch (s) {
-      case SK16W: return launch_logits<T, SK16W, false>(a, st);
-      case SK16: return launch_logits<T, SK16, false>(a, st);
-      case SK32: return launch_logits<T, SK32, false>(a, st);
-      case SK64: return launch_logits<T, SK64, false>(a, st);
+  if (s == S64) return launch_logits<T, S64, WAY>(a, st);
+  if constexpr (WAY != KEPT) switch (s) {
+      case S256: return launch_logits<T, S256, WAY>(a, st);
+      case S128: return launch_logits<T, S128, WAY>(a, st);
+      case SM64: return launch_logits<T, SM64, WAY>(a, st);
+    }
+  if constexpr (WAY == FORWARD) switch (s) {
+      case SK16W: return launch_logits<T, SK16W, WAY>(a, st);
+      case SK16: return launch_logits<T, SK16, WAY>(a, st);
+      case SK32: return launch_logits<T, SK32, WAY>(a, st);
+      case SK64: return launch_logits<T, SK64, WAY>(a, st);
     }
   return PMG_E_ARG;
 }
@@ -837,6 +872,7 @@ int operands(const pmg_linear_ce* a, const Problem& p, const Layout& L, char* ws
   l->K = p.Hp;
   l->scale = a->logit_scale;
   l->targets = a->targets; l->id_bits = a->id_bits;
+  l->kept = a->logits; l->ldk = up(p.V, 4);
   return PMG_OK;
 }
 
@@ -849,7 +885,7 @@ template <typename T> int forward(const pmg_linear_ce* a, const Problem& p, char
   l.part = (float2*)(ws + L.part);
   l.at_target = (float*)(ws + L.at);
   const int s = logits_shape(p.V, p.N, p.Hp, (int64_t)p.eb, false);
-  if (const int rc = logits<T, false>(s, l, st)) return rc;
+  if (const int rc = logits<T, FORWARD>(s, l, st)) return rc;
   RowArgs r = {};
   r.part = l.part;
   r.at_target = l.at_target;
@@ -913,7 +949,7 @@ template <typename T> int backward(const pmg_linear_ce* a, const Problem& p, cha
     l.V = v;
     l.W = W + v0 * l.ldw * (int64_t)p.eb;
     l.bias = bias ? bias + v0 * (int64_t)p.eb : nullptr;
-    if (const int rc = logits<T, true>(b.s_dl, l, st)) return rc;
+    if (const int rc = l.kept ? logits<T, KEPT>(b.s_dl, l, st) : logits<T, REFORM>(b.s_dl, l, st)) return rc;
     if (a->grad_bias)
       hipLaunchKernelGGL(lce_dbias_kernel<T>, dim3((unsigned)div_up(v, 64)), dim3(1024), 0, st, l.dbias,
                          SHAPES[b.s_dl].BN, sl.total, b.ldl, v, (T*)a->grad_bias + v0);

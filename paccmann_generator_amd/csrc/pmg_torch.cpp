@@ -201,20 +201,32 @@ struct CeCall {
   }
 };
 
-std::tuple<Tensor, Tensor, Tensor> linear_ce(const Tensor& hidden, const Tensor& weight, const OptTensor& bias,
-                                             const Tensor& targets, const OptTensor& row_weight, int64_t ignore_index,
-                                             double logit_scale, int64_t reduction) {
+// The logits too where `keep` says so (else an empty tensor).
+std::tuple<Tensor, Tensor, Tensor, Tensor> linear_ce_keep(const Tensor& hidden, const Tensor& weight, const OptTensor& bias,
+                                                          const Tensor& targets, const OptTensor& row_weight,
+                                                          int64_t ignore_index, double logit_scale, int64_t reduction,
+                                                          bool keep) {
   CeCall c(hidden, weight, bias, targets, row_weight, ignore_index, logit_scale, reduction);
   const bool none = reduction == PMG_REDUCE_NONE;
   Tensor loss = fp32(none ? targets.sizes() : at::IntArrayRef(), hidden), lse = fp32(targets.sizes(), hidden);
   Tensor count = none ? fp32({0}, hidden) : fp32({}, hidden);
-  if (c.a.N == 0) return {loss.zero_(), lse, count.zero_()};
+  Tensor logits = fp32({keep ? c.a.N : 0, (c.a.V + 3) / 4 * 4}, hidden);
+  if (c.a.N == 0) return {loss.zero_(), lse, count.zero_(), logits};
+  c.a.logits = keep ? (float*)logits.data_ptr() : nullptr;
   const Tensor ws = c.workspace(0);
   c.a.loss = (float*)loss.data_ptr();
   c.a.lse = (float*)lse.data_ptr();
   c.a.count = none ? nullptr : (float*)count.data_ptr();
   On on(hidden.device());
   check(pmg_linear_ce_fwd(&c.a, ws.data_ptr(), on.stream), "pmg_linear_ce_fwd");
+  return {loss, lse, count, logits};
+}
+
+std::tuple<Tensor, Tensor, Tensor> linear_ce(const Tensor& hidden, const Tensor& weight, const OptTensor& bias,
+                                             const Tensor& targets, const OptTensor& row_weight, int64_t ignore_index,
+                                             double logit_scale, int64_t reduction) {
+  auto [loss, lse, count, logits] =
+      linear_ce_keep(hidden, weight, bias, targets, row_weight, ignore_index, logit_scale, reduction, false);
   return {loss, lse, count};
 }
 
@@ -222,7 +234,7 @@ std::tuple<Tensor, Tensor, Tensor> linear_ce_bwd(const OptTensor& grad_loss, con
                                                  const Tensor& weight, const OptTensor& bias, const Tensor& targets,
                                                  const OptTensor& row_weight, const Tensor& lse, const Tensor& count,
                                                  int64_t ignore_index, double logit_scale, int64_t reduction,
-                                                 std::array<bool, 3> wanted) {
+                                                 std::array<bool, 3> wanted, const OptTensor& logits) {
   CeCall c(hidden, weight, bias, targets, row_weight, ignore_index, logit_scale, reduction);
   TORCH_CHECK(!wanted[2] || bias, "pmg::linear_cross_entropy_bwd: there is no bias");
   const auto out = [&](bool want, at::IntArrayRef size) {
@@ -236,6 +248,13 @@ std::tuple<Tensor, Tensor, Tensor> linear_ce_bwd(const OptTensor& grad_loss, con
   TORCH_CHECK(lse.scalar_type() == at::kFloat && lse.sizes() == targets.sizes() && lse.is_contiguous() &&
                   count.scalar_type() == at::kFloat && (none || count.numel() == 1),
               "pmg::linear_cross_entropy_bwd: lse and count must be those of the forward call");
+  if (logits && logits->numel()) {
+    need_device(*logits, hidden.device());
+    TORCH_CHECK(logits->scalar_type() == at::kFloat && logits->is_contiguous() && logits->dim() == 2 &&
+                    logits->size(0) == c.a.N && logits->size(1) == (c.a.V + 3) / 4 * 4,
+                "pmg::linear_cross_entropy_bwd: logits must be those of the forward call");
+    c.a.logits = (float*)logits->data_ptr();
+  }
   Tensor slope[2];
   for (int k = 0; k < 2; ++k) {
     const OptTensor& g = k == 0 ? grad_loss : grad_lse;
@@ -261,13 +280,14 @@ std::tuple<Tensor, Tensor, Tensor> linear_ce_bwd(const OptTensor& grad_loss, con
 struct LinearCeGrad : torch::autograd::Function<LinearCeGrad> {
   static variable_list forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight, const OptTensor& bias,
                                const Tensor& targets, const OptTensor& row_weight, int64_t ignore_index, double logit_scale,
-                               int64_t reduction) {
-    static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("pmg::linear_cross_entropy", "").typed<decltype(linear_ce)>();
+                               int64_t reduction, bool keep) {
+    static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("pmg::linear_cross_entropy_keep", "").typed<decltype(linear_ce_keep)>();
     at::AutoDispatchBelowADInplaceOrView below;
-    auto [loss, lse, count] = op.call(hidden, weight, bias, targets, row_weight, ignore_index, logit_scale, reduction);
+    auto [loss, lse, count, logits] = op.call(hidden, weight, bias, targets, row_weight, ignore_index, logit_scale, reduction, keep);
     ctx->set_materialize_grads(false);
     ctx->mark_non_differentiable({count});
-    ctx->save_for_backward({hidden, weight, bias.value_or(Tensor()), targets, row_weight.value_or(Tensor()), lse, count});
+    ctx->save_for_backward({hidden, weight, bias.value_or(Tensor()), targets, row_weight.value_or(Tensor()), lse, count,
+                            logits});
     ctx->saved_data["wanted"] =
         c10::List<bool>({hidden.requires_grad(), weight.requires_grad(), bias && bias->defined() && bias->requires_grad()});
     ctx->saved_data["ignore"] = ignore_index;
@@ -278,14 +298,14 @@ struct LinearCeGrad : torch::autograd::Function<LinearCeGrad> {
   static variable_list backward(AutogradContext* ctx, variable_list grad) {
     static auto op =
         c10::Dispatcher::singleton().findSchemaOrThrow("pmg::linear_cross_entropy_bwd", "").typed<decltype(linear_ce_bwd)>();
-    variable_list out(8);
+    variable_list out(9);
     const auto wanted = ctx->saved_data["wanted"].toBoolList();
     if (!grad[0].defined() && !grad[1].defined()) return out;
     const auto s = ctx->get_saved_variables();
     const auto opt = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
     auto [dx, dw, db] = op.call(opt(grad[0]), opt(grad[1]), s[0], s[1], opt(s[2]), s[3], opt(s[4]), s[5], s[6],
                                 ctx->saved_data["ignore"].toInt(), ctx->saved_data["scale"].toDouble(),
-                                ctx->saved_data["reduction"].toInt(), {wanted.get(0), wanted.get(1), wanted.get(2)});
+                                ctx->saved_data["reduction"].toInt(), {wanted.get(0), wanted.get(1), wanted.get(2)}, s[7]);
     if (wanted.get(0)) out[0] = dx;
     if (wanted.get(1)) out[1] = dw;
     if (wanted.get(2)) out[2] = db;
@@ -296,7 +316,12 @@ struct LinearCeGrad : torch::autograd::Function<LinearCeGrad> {
 std::tuple<Tensor, Tensor, Tensor> linear_ce_autograd(const Tensor& hidden, const Tensor& weight, const OptTensor& bias,
                                                       const Tensor& targets, const OptTensor& row_weight, int64_t ignore_index,
                                                       double logit_scale, int64_t reduction) {
-  auto out = LinearCeGrad::apply(hidden, weight, bias, targets, row_weight, ignore_index, logit_scale, reduction);
+  // Training keeps logits that take at most a quarter of the bytes of the hidden rows they are made of: reading them (and
+  // their slopes) is then cheaper than reading the hidden rows once more, before any product.  524288 rows of 512 fp32 over
+  // 60: KEPT us a step, REFORMED without.
+  const bool grads = at::GradMode::is_enabled() && (hidden.requires_grad() || weight.requires_grad() || (bias && bias->requires_grad()));
+  const bool keep = grads && weight.dim() == 2 && 16 * weight.sym_size(0) <= weight.sym_size(1) * weight.element_size();
+  auto out = LinearCeGrad::apply(hidden, weight, bias, targets, row_weight, ignore_index, logit_scale, reduction, keep);
   return {out[0], out[1], out[2]};
 }
 
@@ -460,8 +485,11 @@ TORCH_LIBRARY_FRAGMENT(pmg, m) {
       "linear_cross_entropy(Tensor hidden, Tensor weight, Tensor? bias, Tensor targets, Tensor? row_weight, int ignore_index, "
       "float logit_scale, int reduction) -> (Tensor, Tensor, Tensor)");
   m.def(
+      "linear_cross_entropy_keep(Tensor hidden, Tensor weight, Tensor? bias, Tensor targets, Tensor? row_weight, int ignore_index, "
+      "float logit_scale, int reduction, bool keep) -> (Tensor, Tensor, Tensor, Tensor)");
+  m.def(
       "linear_cross_entropy_bwd(Tensor? grad_loss, Tensor? grad_lse, Tensor hidden, Tensor weight, Tensor? bias, Tensor targets, "
-      "Tensor? row_weight, Tensor lse, Tensor count, int ignore_index, float logit_scale, int reduction, bool[3] wanted) -> "
+      "Tensor? row_weight, Tensor lse, Tensor count, int ignore_index, float logit_scale, int reduction, bool[3] wanted, Tensor? logits=None) -> "
       "(Tensor, Tensor, Tensor)");
   m.def("grad_norm(Tensor[] grads) -> Tensor");
   m.def("clip_grad_norm_(Tensor(a!)[] grads, float max_norm) -> Tensor");
@@ -476,6 +504,7 @@ TORCH_LIBRARY_IMPL(pmg, CUDA, m) {
   m.impl("embedding", embedding);
   m.impl("embedding_bwd", embedding_bwd);
   m.impl("linear_cross_entropy", linear_ce);
+  m.impl("linear_cross_entropy_keep", linear_ce_keep);
   m.impl("linear_cross_entropy_bwd", linear_ce_bwd);
   m.impl("grad_norm", grad_norm);
   m.impl("clip_grad_norm_", clip_grad_norm);

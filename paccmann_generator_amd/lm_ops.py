@@ -91,9 +91,17 @@ def _(hidden, weight, bias, targets, row_weight, ignore_index, logit_scale, redu
             hidden.new_empty(() if reduction else (0,), **f32))
 
 
+@torch.library.register_fake('pmg::linear_cross_entropy_keep')
+def _(hidden, weight, bias, targets, row_weight, ignore_index, logit_scale, reduction, keep):
+    f32 = dict(dtype=torch.float32)
+    return (hidden.new_empty(() if reduction else targets.shape, **f32), hidden.new_empty(targets.shape, **f32),
+            hidden.new_empty(() if reduction else (0,), **f32),
+            hidden.new_empty((targets.numel() if keep else 0, (weight.shape[0] + 3) // 4 * 4), **f32))
+
+
 @torch.library.register_fake('pmg::linear_cross_entropy_bwd')
 def _(grad_loss, grad_lse, hidden, weight, bias, targets, row_weight, lse, count, ignore_index, logit_scale, reduction,
-      wanted):
+      wanted, logits=None):
     return (hidden.new_empty(hidden.shape if wanted[0] else (0,)), weight.new_empty(weight.shape if wanted[1] else (0,)),
             weight.new_empty((weight.shape[0],) if wanted[2] else (0,)))
 
@@ -102,14 +110,15 @@ def _(grad_loss, grad_lse, hidden, weight, bias, targets, row_weight, lse, count
 def linear_cross_entropy(hidden: Tensor, weight: Tensor, targets: Tensor, bias: Optional[Tensor] = None,
                          row_weight: Optional[Tensor] = None, ignore_index: int = -100, logit_scale: float = 1.0,
                          reduction: str = 'mean', trusted_tokens: bool = False) -> Tuple[Tensor, Tensor]:
-    """(loss, lse) of ``logit_scale * (hidden @ weight.T + bias)`` against ``targets``, without keeping the logits.
+    """(loss, lse) of ``logit_scale * (hidden @ weight.T + bias)`` against ``targets``.  The logits are not kept
+    (for training they are where a row of them, in fp32, takes at most a quarter of the bytes of a hidden row).
 
     ``hidden`` [..., H], ``weight`` [V, H] and ``bias`` [V] are all fp32 or all bf16; ``targets`` [...] int64 or int32.
     The loss of a row is its negative log-probability times ``row_weight`` (fp32 [...], a reward say; it gets no
     gradient) and 0 where the target is ``ignore_index``.  ``reduction``: 'none' ([...]), 'sum', or 'mean' over the rows
     with a target (0 without any).  ``lse`` [...] is the log-sum-exp of every row's logits.  Differentiable through both
-    w.r.t. hidden, weight and bias: the logits are formed again, a piece of the vocabulary at a time, for the rows whose
-    loss or lse has a slope; the others have zero gradients and add nothing, whatever they hold.
+    w.r.t. hidden, weight and bias: logits that were not kept are formed again, a piece of the vocabulary at a time, for
+    the rows whose loss or lse has a slope; the others have zero gradients and add nothing, whatever they hold.
     ``trusted_tokens`` skips the range check of the targets, which synchronises (captured graphs need it skipped): a
     target out of range then gives NaN."""
     if reduction not in _ffi.PMG_REDUCE:

@@ -283,3 +283,46 @@ def test_refusals(gpu):
     for a, c, d, kw in bad:
         with pytest.raises(_ffi.PmgError):
             ops.linear_cross_entropy(a, c, d, **kw)
+
+
+# Few vocabulary entries against the hidden size: training keeps the logits (16 V <= bytes of a hidden row)
+KEPT = [(1, 1, 64), (70, 3, 48), (300, 60, 480), (2000, 17, 296), (33, 129, 1056), (20000, 61, 504), (65, 128, 1024)]
+
+
+@pytest.mark.parametrize('dtype', TYPES, ids=str)
+@pytest.mark.parametrize('N,V,H', KEPT)
+def test_logits_kept_for_the_backward(gpu, dtype, N, V, H):
+    if 16 * V > H * dtype.itemsize:
+        V = H * dtype.itemsize // 16
+    _check(*_data(N, V, H, dtype, seed=N + V + H))
+    z = torch.randn(N, generator=torch.Generator().manual_seed(1))
+    z[N // 2] = 0.0
+    _check(*_data(N, V, H, dtype, seed=N, bias=True, weighted=True, ignored=0.3), scale=0.7, reduction='none', lse_slope=z)
+
+
+@pytest.mark.parametrize('dtype', TYPES, ids=str)
+@pytest.mark.parametrize('N,V,H', [(524288, 603, 16), (50, 700, 32), (20, 5, 16)])
+def test_kept_logits_give_the_gradients_of_formed_ones(gpu, dtype, N, V, H):
+    """In pieces of the vocabulary, over listed rows: the slopes are those of logits formed again (equal products; the
+    tiles' shapes may sum them in another order)."""
+    x, w, b, t, r = _cuda(*_data(N, V, H, dtype, seed=4, bias=True, weighted=True, ignored=0.4))
+    call = (x, w, b, t, r, -100, 0.8, 1)
+    loss, lse, count = torch.ops.pmg.linear_cross_entropy(*call)
+    l2, e2, c2, logits = torch.ops.pmg.linear_cross_entropy_keep(*call, True)
+    assert torch.equal(loss, l2) and torch.equal(lse, e2) and torch.equal(count, c2) and logits.shape == (N, (V + 3) // 4 * 4)
+    empty = torch.ops.pmg.linear_cross_entropy_keep(*call, False)[3]
+    back = lambda k: torch.ops.pmg.linear_cross_entropy_bwd(torch.ones_like(loss), None, *call[:5], lse, count, *call[5:],   # noqa: E731
+                                                            [True] * 3, k)
+    want, same = back(None), back(empty)
+    got = back(logits)
+    size = (H + 16) * U * float((x.float().abs().amax(0) * w.float().abs().amax(0)).sum() + 2)
+    for a, c, d, other in zip(got, want, same, (w, x, None)):
+        assert torch.equal(c, d)
+        # dl differs by its relative error at most (a logit's rounding, dl's own), in a sum of at most this many terms
+        terms = {0: V, 1: N, None: N}[0 if other is w else 1 if other is x else None]
+        most = (1.3 if terms == N else 1.0) * 0.8 * (float(other.float().abs().max()) if other is not None else 1.0)
+        step = torch.finfo(dtype).eps / 2
+        scale = most * (2.0 if terms == V else float(r.abs().sum()) * 2)
+        assert bool(((a.float() - c.float()).abs() <= scale * (4 * size + 2 * step) + 2 * step * c.float().abs()).all())
+    with pytest.raises(RuntimeError, match='logits must be'):
+        back(logits[:, :-1] if V > 4 else logits[:-1])
