@@ -22,6 +22,8 @@
 // quarter of the operations).
 #include "pmg_gemm.h"
 
+#include <type_traits>
+
 namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
@@ -273,16 +275,16 @@ struct GradArgs {
   void* zeroed;          // the others become zero here (null: not in this launch)
 };
 
-// Zero rows of dx for 64 rows of the batch that have no slope; a wave takes one row after the other in turn.
+// Zero columns c0 .. H of rows of dx for 64 rows of the batch that have no slope; a wave takes one row after the other in turn.
 template <typename T>
-__device__ __forceinline__ void zero_rows(const uint8_t* __restrict__ used, int64_t n0, int64_t N, int64_t H, int64_t ldo,
-                                          T* __restrict__ dx) {
+__device__ __forceinline__ void zero_rows(const uint8_t* __restrict__ used, int64_t n0, int64_t N, int64_t c0, int64_t H,
+                                          int64_t ldo, T* __restrict__ dx) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
   uint64_t left = __ballot(n0 + lane < N && !used[n0 + lane]);
   for (int k = 0; left; ++k, left &= left - 1) {
     if (k % waves != wave) continue;
     T* row = dx + (n0 + __ffsll((unsigned long long)left) - 1) * ldo;
-    for (int64_t c = lane * 4; c < H; c += 256) pmg_store4(row + c, f32x4{0.f, 0.f, 0.f, 0.f}, H - c);
+    for (int64_t c = c0 + lane * 4; c < H; c += 256) pmg_store4(row + c, f32x4{0.f, 0.f, 0.f, 0.f}, H - c);
   }
 }
 
@@ -292,7 +294,7 @@ __global__ __launch_bounds__(THREADS_OF<S>) void lce_grad_kernel(const GradArgs 
   constexpr int BM = SHAPES[S].BM, BN = SHAPES[S].BN, WM = SHAPES[S].WM, WN = SHAPES[S].WN;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   if (BKC && (int64_t)blockIdx.x >= (int64_t)a.tiles_m * a.tiles_n) {  // behind the tiles
-    if (blockIdx.y == 0) zero_rows(a.used, ((int64_t)blockIdx.x - (int64_t)a.tiles_m * a.tiles_n) * 64, a.N, a.M, a.ldo, (T*)a.zeroed);
+    if (blockIdx.y == 0) zero_rows(a.used, ((int64_t)blockIdx.x - (int64_t)a.tiles_m * a.tiles_n) * 64, a.N, 0, a.M, a.ldo, (T*)a.zeroed);
     return;
   }
   int tm, tn;
@@ -335,6 +337,122 @@ __global__ __launch_bounds__(THREADS_OF<S>) void lce_grad_kernel(const GradArgs 
       const bool up = Tile::swapped();
       if (Tile::PAIR && a.out && m < a.M) pmg_store8((T*)a.out + o * a.ldo + m, up ? x[1] : x[0], up ? x[0] : x[1], a.M - m);
     }
+  }
+}
+
+// dx over at most 64 vocabulary entries, bound by writing dx (fp32: and by the matrix units, 64 columns of k a token).  A
+// wave keeps its 256 bytes of columns of W in registers, in the fragments' layout, and streams over tokens: the workgroup
+// fetches the slopes of 64 tokens ahead, in whole rows, and passes them through LDS (16-byte pieces of a row permuted, so
+// that the rows of a fragment lie in different banks).  Tokens are the products' m and columns their n, lane l & 15 of
+// fragment i has column MI (l & 15) + i: a lane's results of a token are neighbours, and those of 16 lanes are 256 bytes in
+// a row.  524288 x 512 fp32 over 60: 316 us (3.4 TB/s written, 109 Tflop/s); 185763 x 2944 bf16 over 17, half of the rows
+// zero: 208 us (5.3 TB/s).  With the short sums' tiles 370 us and 370 us; with fragments read straight from memory, where
+// neighbouring lanes read different rows, 452 and 234, and with products whose lanes are tokens, so that neighbouring lanes
+// write different rows, 536 and 295.
+constexpr int NARROW = 64, NARROW_TOKENS = 64, NARROW_PER_CU = 3;  // vocabulary entries, tokens at a time, workgroups a CU
+template <typename T>
+__global__ __launch_bounds__(256, NARROW_PER_CU) void lce_dx_narrow_kernel(const GradArgs a) {
+  constexpr int E = 16 / sizeof(T), KK = NARROW / (4 * E), MI = E, COLS = MI * 16;
+  constexpr int PIECES = NARROW / E, FETCH = NARROW_TOKENS * PIECES / 256;
+  typedef typename pmg_frag<T>::type frag;
+  __shared__ __attribute__((aligned(16))) frag slopes[2][NARROW_TOKENS * PIECES];
+  __shared__ __attribute__((aligned(16))) unsigned places[2][NARROW_TOKENS];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, i16 = lane & 15;
+  const int64_t m0 = ((int64_t)blockIdx.y * 4 + wave) * COLS;
+  const int N = uniform_of(a.count), step = gridDim.x * NARROW_TOKENS;
+  if (N < a.N) {
+    const int64_t c0 = (int64_t)blockIdx.y * 4 * COLS, c1 = c0 + 4 * COLS < a.M ? c0 + 4 * COLS : a.M;
+    for (int64_t n0 = (int64_t)blockIdx.x * 64; n0 < a.N; n0 += (int64_t)gridDim.x * 64)
+      zero_rows(a.used, n0, a.N, c0, c1, a.ldo, (T*)a.zeroed);
+  }
+  int t = blockIdx.x * NARROW_TOKENS;
+  if (t >= N) return;
+  const int64_t m = m0 + MI * i16, left = a.M - m;  // this lane's columns (may be none)
+  frag w[MI][KK];
+#pragma unroll
+  for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      const int k = kk * 4 * E + g * E + j;
+      typename pmg_vec16<T>::vec x = {};
+      if (k < a.K && left > 0) x = pmg_vec16<T>::load((const T*)a.A + k * a.lda + m, left);
+#pragma unroll
+      for (int i = 0; i < MI; ++i) w[i][kk][j] = x[i];
+    }
+  const float f = a.factor[0];
+  frag next[FETCH];
+  unsigned next_place;
+  const auto fetch = [&](int at) {  // rows behind the last: the last one
+    next_place = a.list[at + (threadIdx.x & 63)];
+#pragma unroll
+    for (int q = 0; q < FETCH; ++q) {
+      const int piece = q * 256 + threadIdx.x, r = piece / PIECES, n = at + r < N ? at + r : N - 1;
+      next[q] = *(const frag*)((const T*)a.B + (int64_t)n * a.ldb + piece % PIECES * E);
+    }
+  };
+  const auto put = [&](int buf) {
+    if (threadIdx.x < NARROW_TOKENS) places[buf][threadIdx.x] = next_place;
+#pragma unroll
+    for (int q = 0; q < FETCH; ++q) {
+      const int piece = q * 256 + threadIdx.x, r = piece / PIECES;
+      slopes[buf][r * PIECES + ((piece ^ r) & (PIECES - 1))] = next[q];
+    }
+  };
+  // `whole`: all tokens and columns; without branches around the stores the compiler waits for the fetch alone, not for them
+  const auto multiply = [&](int at, int buf, auto whole) {
+#pragma unroll 1  // (more turns at a time take more registers than three workgroups a CU have)
+    for (int q = 0; q < NARROW_TOKENS / 16; ++q) {
+      const int r = q * 16 + i16;
+      frag b[KK];
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) b[kk] = slopes[buf][r * PIECES + (((kk * 4 + g) ^ r) & (PIECES - 1))];
+      f32x4 acc[MI];
+#pragma unroll
+      for (int i = 0; i < MI; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+          for (int i = 0; i < MI; ++i) acc[i] = pmg_frag<T>::mma(b[kk], w[i][kk], acc[i]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < E; ++j)
+#pragma unroll
+            for (int i = 0; i < MI; ++i) acc[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(b[kk][j], w[i][kk][j], acc[i], 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int row = q * 16 + 4 * g + e;
+        T* out = (T*)a.out + (uint64_t)places[buf][row] * (uint64_t)a.ldo + m;
+        f32x4 x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = acc[i][e] * f;
+        if (!whole && (at + row >= N || left <= 0)) continue;
+        if constexpr (MI == 8) {
+          f32x4 y;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) y[i] = acc[4 + i][e] * f;
+          pmg_store8(out, x, y, whole ? 8 : left);
+        } else {
+          pmg_store4(out, x, whole ? 4 : left);
+        }
+      }
+    }
+  };
+  fetch(t);
+  put(0);
+  __syncthreads();
+  for (int buf = 0;; buf ^= 1) {
+    const bool last = t >= N - step;
+    fetch(last ? t : t + step);
+    __builtin_amdgcn_sched_barrier(0);  // ahead of the products, not behind
+    if (m0 + COLS <= a.M && t + NARROW_TOKENS <= N) multiply(t, buf, std::true_type());
+    else multiply(t, buf, std::false_type());
+    if (last) break;
+    put(buf ^ 1);
+    __syncthreads();
+    t += step;
   }
 }
 
@@ -652,9 +770,9 @@ int logits_shape(int64_t V, int64_t N, int64_t H, int64_t eb, bool backward) {
   return best_square(V, N, H, eb, false);
 }
 
-// A short sum (few vocabulary entries) is bound by writing dx: small tiles, several a CU, so that some write while
-// others multiply, and in fp32 stores that pass the caches by (524288 x 512 over 60: 380 us; 410 us with plain stores, 478
-// us with 64 x 256, 506 us with the large square; bf16 stores of 8 bytes a lane need the cache to become whole lines).
+// A short sum (65 to 256 vocabulary entries) is bound by writing dx: small tiles, six a CU, so that some write while
+// others multiply (fp32 262144 x 512 over 65: 204 us, 305 with the best square; 131072 x 1024 over 250: 554 and 593; bf16
+// 262144 x 1024 over 100: 222 and 239; 131072 x 2048 over 250: 284 and 304).
 int dx_shape(int64_t H, int64_t N, int64_t K, int64_t eb, bool split) {
   return K <= 256 && H > 64 ? SD64 : best_square(H, N, K, eb, split);
 }
@@ -848,6 +966,14 @@ template <typename T, bool BKC> int grad(int s, GradArgs a, hipStream_t st) {
   return (int)hipGetLastError();
 }
 
+template <typename T> int dx_narrow(GradArgs a, hipStream_t st) {
+  const int64_t blocks_m = div_up(a.M, 1024 / (int64_t)sizeof(T)), chunks = div_up(a.N, NARROW_TOKENS);
+  const int64_t most = up(div_up((int64_t)CUS * NARROW_PER_CU, blocks_m), 8);  // (8: the columns of a token on one XCD)
+  const int64_t blocks = div_up(chunks, div_up(chunks, most));                 // as many turns for all
+  hipLaunchKernelGGL(lce_dx_narrow_kernel<T>, dim3((unsigned)blocks, (unsigned)blocks_m), dim3(256), 0, st, a);
+  return (int)hipGetLastError();
+}
+
 template <typename T> int pack(const void* src, int64_t ld, int64_t rows, const Problem& p, void* dst, hipStream_t st) {
   hipLaunchKernelGGL(lce_pack_kernel<T>, dim3((unsigned)div_up(rows * p.Hp, 256)), dim3(256), 0, st, (const T*)src, ld, rows, p.H,
                      (T*)dst, p.Hp);
@@ -968,7 +1094,7 @@ template <typename T> int backward(const pmg_linear_ce* a, const Problem& p, cha
       g.add = i > 0;
       g.used = sl.used;
       g.zeroed = i == 0 ? a->grad_hidden : nullptr;
-      if (const int rc = grad<T, true>(b.s_dx, g, st)) return rc;
+      if (const int rc = p.V <= NARROW ? dx_narrow<T>(g, st) : grad<T, true>(b.s_dx, g, st)) return rc;
     }
     if (a->grad_weight) {
       GradArgs g = {};
