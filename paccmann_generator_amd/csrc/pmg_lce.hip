@@ -853,7 +853,7 @@ BwdPlan bwd_plan(const Problem& p) {
   b.pieces = div_up(p.V, b.piece);
   b.ldl = up(b.piece, 64);
   const int64_t eb = (int64_t)p.eb;
-  b.s_dl = p.kept ? S64 : logits_shape(b.piece, p.N, p.Hp, eb, true);  // (kept: no product, any shape)
+  b.s_dl = p.kept ? SM64 : logits_shape(b.piece, p.N, p.Hp, eb, true);  // (kept: no product, any shape)
   b.s_dx = dx_shape(p.H, p.N, b.piece, eb, b.pieces == 1);
   b.s_dw = dw_shape(p.H, b.piece, p.N, eb);
   b.split_dx = b.pieces == 1 ? splits_of(b.s_dx, p.H, p.N, b.piece, eb) : 1;
@@ -915,11 +915,11 @@ template <typename T, int WAY> int logits(int s, LogitArgs a, hipStream_t st) {
   a.tiles_m = (int)div_up(a.V, SHAPES[s].BM);
   a.tiles_n = (int)div_up(a.N, SHAPES[s].BN);
   if ((int64_t)a.tiles_m * a.tiles_n > 0x7fffffff) return PMG_E_ARG;
-  if (s == S64) return launch_logits<T, S64, WAY>(a, st);
+  if (s == SM64) return launch_logits<T, SM64, WAY>(a, st);
   if constexpr (WAY != KEPT) switch (s) {
       case S256: return launch_logits<T, S256, WAY>(a, st);
       case S128: return launch_logits<T, S128, WAY>(a, st);
-      case SM64: return launch_logits<T, SM64, WAY>(a, st);
+      case S64: return launch_logits<T, S64, WAY>(a, st);
     }
   if constexpr (WAY == FORWARD) switch (s) {
       case SK16W: return launch_logits<T, SK16W, WAY>(a, st);
