@@ -86,8 +86,9 @@ typedef struct pmg_linear_ce {
                               row's V entries: anything), backward: read in place of forming them again */
 } pmg_linear_ce;
 
-/* Bytes of scratch of one direction.  It does not grow with N x V: the backward keeps the slopes of a
- * piece of the vocabulary at a time. */
+/* Bytes of scratch of one direction, for a call with these sizes, strides, operands (their alignment counts)
+ * and logits.  It does not grow with N x V: the backward keeps the slopes of a piece of the vocabulary at a
+ * time. */
 int pmg_linear_ce_workspace(const pmg_linear_ce* a, int backward, size_t* out);
 int pmg_linear_ce_fwd(const pmg_linear_ce* a, void* ws, pmg_stream stream);
 int pmg_linear_ce_bwd(const pmg_linear_ce* a, void* ws, pmg_stream stream);

@@ -717,10 +717,10 @@ __global__ __launch_bounds__(1024) void lce_scan_kernel(int* __restrict__ first,
 template <typename T>
 __global__ __launch_bounds__(256) void lce_pack_kernel(const T* __restrict__ src, int64_t ld, int64_t rows, int64_t width,
                                                        T* __restrict__ dst, int64_t wide) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= rows * wide) return;
-  const int64_t r = i / wide, c = i - r * wide;
-  dst[i] = c < width ? src[r * ld + c] : (T)0.0f;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * wide; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / wide, c = i - r * wide;
+    dst[i] = c < width ? src[r * ld + c] : (T)0.0f;
+  }
 }
 
 // ------------------------------------------------------------------------------------------ host
@@ -875,7 +875,7 @@ Layout bwd_layout(const Problem& p, const BwdPlan& b) {
   L.dl = take((size_t)p.N * b.ldl * p.eb);
   L.dxacc = take(b.pieces > 1 || b.split_dx > 1 ? (size_t)b.split_dx * p.N * p.H * 4 : 0);
   L.dwacc = take(b.split_dw > 1 ? (size_t)b.split_dw * b.piece * p.H * 4 : 0);
-  L.dbias = take((size_t)div_up(p.N, SHAPES[b.s_dl].BN) * b.ldl * 4);
+  L.dbias = take((size_t)div_up(p.N, 64) * b.ldl * 4);  // tiles of 64 tokens or more, with kept logits or without
   L.bytes = take.at + 256;
   return L;
 }
@@ -975,8 +975,9 @@ template <typename T> int dx_narrow(GradArgs a, hipStream_t st) {
 }
 
 template <typename T> int pack(const void* src, int64_t ld, int64_t rows, const Problem& p, void* dst, hipStream_t st) {
-  hipLaunchKernelGGL(lce_pack_kernel<T>, dim3((unsigned)div_up(rows * p.Hp, 256)), dim3(256), 0, st, (const T*)src, ld, rows, p.H,
-                     (T*)dst, p.Hp);
+  const int64_t blocks = div_up(rows * p.Hp, 256), most = 1 << 20;  // (a launch has fewer than 2^32 threads)
+  hipLaunchKernelGGL(lce_pack_kernel<T>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, st, (const T*)src, ld, rows,
+                     p.H, (T*)dst, p.Hp);
   return (int)hipGetLastError();
 }
 

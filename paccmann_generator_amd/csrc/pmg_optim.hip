@@ -501,13 +501,16 @@ extern "C" int pmg_adamw_step(const pmg_adamw* a, void* ws, pmg_stream stream) {
     if (bad) return PMG_E_ALIGN;
   }
   if (chunks_all > 0x7fffffff) return PMG_E_ARG;
-  Range* r = new (std::nothrow) Range[(size_t)a->n * 7 + 1];
+  Range* r = new (std::nothrow) Range[(size_t)a->n * 7 + 4];
   if (!r) return PMG_E_ARG;
   int nr = 0;
   auto add = [&](const void* p, size_t bytes, int written) {
     r[nr++] = Range{(uintptr_t)p, (uintptr_t)p + bytes, written};
   };
   add(a->step, 8, 1);
+  add(ws, PMG_ADAMW_WS, 1);
+  if (a->lr_dev) add(a->lr_dev, 4, 0);
+  if (a->norm) add(a->norm, 4, 0);
   for (int i = 0; i < a->n; ++i) {
     const size_t n = (size_t)a->numel[i], nb = (n + PMG_STATE_BLOCK - 1) / PMG_STATE_BLOCK;
     if (n == 0) continue;

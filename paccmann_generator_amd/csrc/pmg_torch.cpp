@@ -82,6 +82,23 @@ Tensor rows_of(const Tensor& t, int64_t width, int64_t* ld) {
   return r;
 }
 
+// A gradient formed with create_graph: it is right, a backward through it to what it was made from is refused (and not
+// taken for zero).
+struct NotTwice : torch::autograd::Function<NotTwice> {
+  static Tensor forward(AutogradContext*, const Tensor& grad, const OptTensor&, const OptTensor&, const OptTensor&, const OptTensor&,
+                        const OptTensor&) {
+    return grad.view_as(grad);
+  }
+  static variable_list backward(AutogradContext*, variable_list) {
+    TORCH_CHECK(false, "pmg: gradients of this operator are not differentiable");
+  }
+};
+
+Tensor last(const Tensor& grad, const OptTensor& a, const OptTensor& b = {}, const OptTensor& c = {}, const OptTensor& d = {},
+            const OptTensor& e = {}) {
+  return at::GradMode::is_enabled() && grad.defined() ? NotTwice::apply(grad, a, b, c, d, e) : grad;
+}
+
 // ------------------------------------------------------------------------------------------ embedding
 Tensor embedding(const Tensor& weight, const Tensor& ids, double scale, int64_t padding_idx) {
   need_device({weight, ids}, weight.device());
@@ -142,9 +159,13 @@ struct EmbeddingGrad : torch::autograd::Function<EmbeddingGrad> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grad) {
     const auto saved = ctx->get_saved_variables();
-    return {call_embedding_bwd(grad[0], saved[0], ctx->saved_data["v"].toInt(), ctx->saved_data["scale"].toDouble(),
-                               ctx->saved_data["pad"].toInt()),
-            Tensor(), Tensor(), Tensor()};
+    Tensor dw;
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      dw = call_embedding_bwd(grad[0], saved[0], ctx->saved_data["v"].toInt(), ctx->saved_data["scale"].toDouble(),
+                              ctx->saved_data["pad"].toInt());
+    }
+    return {last(dw, grad[0]), Tensor(), Tensor(), Tensor()};
   }
 };
 
@@ -303,12 +324,16 @@ struct LinearCeGrad : torch::autograd::Function<LinearCeGrad> {
     if (!grad[0].defined() && !grad[1].defined()) return out;
     const auto s = ctx->get_saved_variables();
     const auto opt = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
-    auto [dx, dw, db] = op.call(opt(grad[0]), opt(grad[1]), s[0], s[1], opt(s[2]), s[3], opt(s[4]), s[5], s[6],
+    const auto [dx, dw, db] = [&] {
+      at::AutoDispatchBelowADInplaceOrView below;
+      return op.call(opt(grad[0]), opt(grad[1]), s[0], s[1], opt(s[2]), s[3], opt(s[4]), s[5], s[6],
                                 ctx->saved_data["ignore"].toInt(), ctx->saved_data["scale"].toDouble(),
                                 ctx->saved_data["reduction"].toInt(), {wanted.get(0), wanted.get(1), wanted.get(2)}, s[7]);
-    if (wanted.get(0)) out[0] = dx;
-    if (wanted.get(1)) out[1] = dw;
-    if (wanted.get(2)) out[2] = db;
+    }();
+    const OptTensor from[5] = {opt(grad[0]), opt(grad[1]), s[0], s[1], opt(s[2])};
+    if (wanted.get(0)) out[0] = last(dx, from[0], from[1], from[2], from[3], from[4]);
+    if (wanted.get(1)) out[1] = last(dw, from[0], from[1], from[2], from[3], from[4]);
+    if (wanted.get(2)) out[2] = last(db, from[0], from[1], from[2], from[3], from[4]);
     return out;
   }
 };

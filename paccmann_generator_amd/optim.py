@@ -24,8 +24,8 @@ class AdamW(torch.optim.Optimizer):
     lr:              a number, or an fp32 tensor of one element on the device (schedules under a captured step)
 
     Steps are counted on the device, so ``step`` can be captured into a graph once the state exists (after one eager
-    step); parameters that always step together share a counter, as in the torch classes a parameter without a
-    gradient keeps its count."""
+    step with the same gradients present; else the capture is refused); parameters that always step together share a
+    counter, as in the torch classes a parameter without a gradient keeps its count.  States of the torch classes load."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2,
                  decoupled: bool = True, state_bits: int = 32, master_weights: bool = False,
@@ -48,6 +48,12 @@ class AdamW(torch.optim.Optimizer):
             s['exp_avg_top'], s['exp_avg_sq_top'] = mt, vt
         if self.master_weights and p.dtype != torch.float32:
             s['master'] = p.detach().to(torch.float32)
+
+    @staticmethod
+    def _not_captured(what):
+        """What happens once must not be recorded: every replay would do it again."""
+        if torch.cuda.is_current_stream_capturing():
+            raise _ffi.PmgError(f'pmg: {what} while a graph is captured; make an eager step with the same gradients first')
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -73,6 +79,7 @@ class AdamW(torch.optim.Optimizer):
         for p in ps:
             s = self.state[p]
             if not s:
+                self._not_captured('the state of a parameter is made')
                 step = fresh.get(p.device)
                 if step is None:
                     step = fresh[p.device] = torch.zeros(1, dtype=torch.int64, device=p.device)
@@ -83,12 +90,14 @@ class AdamW(torch.optim.Optimizer):
         for key, members in buckets.items():
             step = self.state[members[0]]['step']
             if owner.setdefault(id(step), key) != key:
+                self._not_captured('a step counter is divided')
                 own = step.clone()
                 for p in members:
                     self.state[p]['step'] = own
         stepping = set(ps)
         for p in group['params']:
             if p not in stepping and self.state.get(p) and id(self.state[p]['step']) in owner:
+                self._not_captured('a step counter is divided')
                 self.state[p]['step'] = self.state[p]['step'].clone()
         return buckets.values()
 
@@ -104,23 +113,33 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """States keep their types (the base class would cast them to their parameter's).  A state of 8 bits loads into
-        an optimizer of 32; the other way round is refused."""
+        an optimizer of 32; the other way round is refused.  States of ``torch.optim.Adam`` and ``AdamW`` load with what
+        this class alone has (``decoupled``) as it is here."""
         state, groups = state_dict['state'], state_dict['param_groups']
+        if any(g.get('amsgrad') or g.get('maximize') for g in groups):
+            raise _ffi.PmgError('pmg: amsgrad and maximize are not supported')
+        before = [dict(g) for g in self.param_groups]
         super().load_state_dict(dict(state={}, param_groups=groups))
+        for g, old in zip(self.param_groups, before):
+            for key, value in old.items():
+                g.setdefault(key, value)
         ids = [i for g in groups for i in g['params']]
-        params = [p for g in self.param_groups for p in g['params']]
+        params = [(k, p) for k, g in enumerate(self.param_groups) for p in g['params']]
         shared = {}
-        for i, p in zip(ids, params):
+        for i, (k, p) in zip(ids, params):
             if i not in state or not state[i]:
                 continue
-            s = {k: v.detach().to(p.device).clone() for k, v in state[i].items()}
+            s = {name: torch.as_tensor(v).detach().to(p.device, copy=True) for name, v in state[i].items()}
+            s['step'] = s['step'].to(torch.int64).reshape(1)
             if 'exp_avg_top' in s and self.state_bits == 32:
                 for name in ('exp_avg', 'exp_avg_sq'):
                     s[name] = ops.adamw_state_values(s[name], s.pop(name + '_top'))
             elif 'exp_avg_top' not in s and self.state_bits == 8:
                 raise _ffi.PmgError('pmg: a state of 32 bits does not load into an optimizer with 8')
-            # parameters whose counters agree share one again
-            s['step'] = shared.setdefault((p.device, int(s['step'])), s['step'])
+            if self.state_bits == 32:
+                s['exp_avg'], s['exp_avg_sq'] = s['exp_avg'].float(), s['exp_avg_sq'].float()
+            # parameters of a group whose counters agree share one again
+            s['step'] = shared.setdefault((k, p.device, int(s['step'])), s['step'])
             if self.master_weights and p.dtype != torch.float32:
                 s.setdefault('master', p.detach().to(torch.float32))
             else:

@@ -171,3 +171,37 @@ def test_opcheck_and_differences(gpu):
     with torch.no_grad():
         diff = ((ops.embedding(along, ids, 2.0) * probe).double().sum())
     assert abs(float((got * along).double().sum() - diff)) < 1e-5 * float(probe.abs().sum() * 4)
+
+
+def test_offsets_beyond_32_bits(gpu):
+    """A table of 4.9 GB and its gradient."""
+    from paccmann_generator_amd import ops
+    V, E = 1200000, 1024
+    table = torch.zeros(V, E, device='cuda')
+    ids = torch.cat([torch.tensor([V - 1, 0, V - 2, V - 1]), torch.randint(0, V, (3000,), generator=torch.Generator().manual_seed(1))])
+    rows = torch.randn(len(ids), E, generator=torch.Generator().manual_seed(2))
+    first = {int(v): n for n, v in reversed(list(enumerate(ids.tolist())))}
+    there = torch.tensor([first[int(v)] for v in ids])
+    table[ids.cuda()] = rows[there].cuda()
+    table.requires_grad_(True)
+    y = ops.embedding(table, ids.cuda())
+    assert torch.equal(y.detach().cpu(), rows[there])
+    slope = torch.randn(len(ids), E, generator=torch.Generator().manual_seed(3))
+    dw, = torch.autograd.grad(y, table, slope.cuda())
+    unique, place = ids.unique(return_inverse=True)
+    exact = torch.zeros(len(unique), E, dtype=torch.float64).index_add_(0, place, slope.double())
+    size = torch.zeros_like(exact).index_add_(0, place, slope.double().abs())
+    count = torch.bincount(place).double().unsqueeze(1)
+    assert bool(((dw[unique.cuda()].cpu().double() - exact).abs() <= size * (count + 2) * 2.0 ** -24 + exact.abs() * 2.0 ** -23).all())
+    dw[unique.cuda()] = 0.0
+    assert not bool(dw.any())
+
+
+def test_the_gradient_is_not_differentiated_again(gpu):
+    from paccmann_generator_amd import ops
+    w = torch.randn(9, 5, device='cuda', requires_grad=True)
+    y = ops.embedding(w, torch.tensor([1, 2, 1], device='cuda'))
+    d, = torch.autograd.grad((y * y).sum(), w, create_graph=True)
+    assert bool((d[1] - 4 * w[1]).abs().max() <= 1e-5) and not d[0].any()
+    with pytest.raises(RuntimeError, match='not differentiable'):
+        torch.autograd.grad(d.sum(), w)

@@ -326,3 +326,42 @@ def test_kept_logits_give_the_gradients_of_formed_ones(gpu, dtype, N, V, H):
         assert bool(((a.float() - c.float()).abs() <= scale * (4 * size + 2 * step) + 2 * step * c.float().abs()).all())
     with pytest.raises(RuntimeError, match='logits must be'):
         back(logits[:, :-1] if V > 4 else logits[:-1])
+
+
+@pytest.mark.parametrize('V', [40, 300])
+def test_offsets_beyond_32_bits(gpu, V):
+    """Hidden rows of 4.9 GB; the rows with a slope lie at both ends."""
+    from paccmann_generator_amd import ops
+    N, H = 1200000, 1024
+    g = torch.Generator(device='cuda').manual_seed(5)
+    x = torch.randn(N, H, device='cuda', generator=g).requires_grad_(True)
+    w = (torch.randn(V, H, device='cuda', generator=g) / 16).requires_grad_(True)
+    t = torch.randint(0, V, (N,), device='cuda', generator=g)
+    rows = torch.cat([torch.arange(0, 300, 3), torch.arange(N - 200, N)])
+    r = torch.zeros(N, device='cuda')
+    r[rows.cuda()] = torch.rand(len(rows), device='cuda', generator=g) + 0.5
+    loss, lse = ops.linear_cross_entropy(x, w, t, row_weight=r, reduction='sum')
+    dx, dw = torch.autograd.grad(loss, (x, w))
+    part = x.detach()[rows.cuda()].cpu(), w.detach().cpu(), t[rows.cuda()].cpu(), None, r[rows.cuda()].cpu()
+    e = lm.linear_ce(*part, 1.0, 'sum', -100)
+    tol = (H + 16) * U * e['size'] + 8 * U
+    assert bool(((lse.detach()[rows.cuda()].cpu().double() - e['lse']).abs() <= tol + 2 * U * e['lse'].abs()).all())
+    grads = lm.linear_ce_grads(*part, 1.0, 'sum', -100, torch.tensor(1.0), None)
+    rel = 4 * float(tol.max()) + 16 * U
+    for got, name, length in ((dx[rows.cuda()], 'x', V), (dw, 'w', len(rows))):
+        bound = grads['|' + name + '|'] * (rel + (length + 8) * U) + grads[name].abs() * U * 1.01
+        assert bool(((got.cpu().double() - grads[name]).abs() <= bound).all()), name
+    dx[rows.cuda()] = 0.0
+    assert not bool(dx.any())
+
+
+def test_gradients_are_not_differentiated_again(gpu):
+    from paccmann_generator_amd import ops
+    x, w, b, t, _ = _cuda(*_data(20, 30, 16, torch.float32, seed=1, bias=True))
+    z = [v.requires_grad_(True) for v in (x, w, b)]
+    want = torch.autograd.grad(ops.linear_cross_entropy(x, w, t, bias=b)[0], z)
+    got = torch.autograd.grad(ops.linear_cross_entropy(x, w, t, bias=b)[0], z, create_graph=True)
+    assert all(torch.equal(p, q) for p, q in zip(want, got))
+    for p in got:
+        with pytest.raises(RuntimeError, match='not differentiable'):
+            torch.autograd.grad(p.sum(), z, allow_unused=True, retain_graph=True)

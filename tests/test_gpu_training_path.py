@@ -296,3 +296,58 @@ def test_learner_default_is_unchanged_and_8_bits_learn_alike(gpu, tmp_path, monk
     for a, b, c, z in zip(got[0][0], got[1][0], got[2][0], first):
         assert float((a - b).abs().max()) <= 0.02 * lr * 3
         assert float((b - c).abs().max()) <= 3 * lr and (not (a != z).any() or bool((c != z).any()))
+
+
+def test_states_of_torch_and_of_several_groups_load(gpu):
+    """A state of torch's Adam goes on as it would there; groups whose counters agree keep a counter each."""
+    from paccmann_generator_amd import AdamW
+    start = [torch.randn(300, generator=torch.Generator().manual_seed(k)).cuda() for k in range(3)]
+    slopes = [[torch.randn(300, generator=torch.Generator().manual_seed(10 * n + k)).cuda() for k in range(3)] for n in range(6)]
+    groups = lambda ps: [dict(params=ps[:1], lr=1e-2), dict(params=ps[1:], lr=3e-3)]         # noqa: E731
+
+    def run(opt, ps, steps):
+        for n in steps:
+            for p, g in zip(ps, slopes[n]):
+                p.grad = g.clone()
+            opt.step()
+
+    a = [s.clone().requires_grad_(True) for s in start]
+    theirs = torch.optim.Adam(groups(a), weight_decay=0.01)
+    run(theirs, a, range(3))
+    b = [p.detach().clone().requires_grad_(True) for p in a]
+    ours = AdamW(groups(b), decoupled=False, weight_decay=0.01)
+    ours.load_state_dict(theirs.state_dict())
+    assert [g['lr'] for g in ours.param_groups] == [1e-2, 3e-3] and not any(g['decoupled'] for g in ours.param_groups)
+    c = [p.detach().clone().requires_grad_(True) for p in a]
+    again = AdamW(groups(c), decoupled=False, weight_decay=0.01)
+    again.load_state_dict(ours.state_dict())
+    run(theirs, a, range(3, 6))
+    run(ours, b, range(3, 6))
+    run(again, c, range(3, 6))
+    for x, y, z in zip(a, b, c):
+        assert int(ours.state[y]['step']) == 6 == int(again.state[z]['step'])
+        assert torch.equal(y, z)
+        # three steps of at most lr (1 + decay) each, every step's quotient off by a few roundings
+        assert float((x - y).abs().max()) <= 3 * 1e-2 * 32 * 2.0 ** -24 + float(x.abs().max()) * 6 * 2.0 ** -24
+    bad = theirs.state_dict()
+    bad['param_groups'][0]['amsgrad'] = True
+    with pytest.raises(Exception, match='amsgrad'):
+        ours.load_state_dict(bad)
+
+
+def test_what_must_not_be_captured_is_refused(gpu, monkeypatch):
+    from paccmann_generator_amd import AdamW
+    from paccmann_generator_amd._ffi import PmgError
+    ps = [torch.randn(40, device='cuda', requires_grad=True) for _ in range(2)]
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    fresh, used = AdamW(ps), AdamW(ps)
+    used.step()
+    monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: True)
+    before = [p.detach().clone() for p in ps]
+    with pytest.raises(PmgError, match='state of a parameter'):
+        fresh.step()
+    ps[1].grad = None
+    with pytest.raises(PmgError, match='counter'):
+        used.step()
+    assert all(torch.equal(p, b) for p, b in zip(ps, before))

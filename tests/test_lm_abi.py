@@ -162,3 +162,20 @@ def test_operators_are_registered_and_refuse_cpu_tensors():
         assert torch.ops.pmg.embedding(w, torch.empty(2, 3, dtype=torch.long), 1.0, -1).shape == (2, 3, 8)
         assert torch.ops.pmg.embedding_bwd(torch.empty(2, 3, 8), torch.empty(2, 3, dtype=torch.long), 9, 1.0, -1).shape == (9, 8)
         assert torch.ops.pmg.grad_norm([w]).shape == ()
+
+
+def test_update_refuses_to_write_what_it_reads():
+    """Workspace, norm and learning rate apart from everything the update writes."""
+    from paccmann_generator_amd import _ffi
+    a = _ffi.PmgAdamw()
+    d = dict(n=1, dtype=0, grad_dtype=0, state_bits=32, decoupled=1, lr=1e-3, beta1=0.9, beta2=0.99, eps=1e-8, max_norm=1.0,
+             step=FAKE - 64)
+    keep = {name: (C.c_void_p * 1)(FAKE + 4096 * k) for k, name in enumerate(('param', 'grad', 'm', 'v'))}
+    n = (C.c_int64 * 1)(10)
+    for name, x in {**d, **{k: C.addressof(v) for k, v in keep.items()}, 'numel': C.addressof(n)}.items():
+        setattr(a, name, x)
+    for ws, norm, lr in ((FAKE + 4096 * 2, None, None), (FAKE + 16, None, None), (FAKE - 64, None, None), (FAKE + 65536, FAKE + 36, None),
+                         (FAKE + 32768, FAKE + 4096 * 3, None), (FAKE + 32768, None, FAKE + 4096 * 2 + 8), (FAKE + 32768, FAKE + 32768 + 8, None)):
+        a.norm, a.lr_dev = norm, lr
+        rc = _ffi.lib.pmg_adamw_step(C.byref(a), ws, None)
+        assert rc < 0 and b'overlap' in _ffi.lib.pmg_strerror(rc), (ws, norm, lr)
