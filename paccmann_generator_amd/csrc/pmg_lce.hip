@@ -68,7 +68,9 @@ struct LogitArgs {
   float* kept;           // logits of all tokens, rows of ldk (a multiple of 4); forward: written, backward: read; or null
   int64_t ldk;
   // forward
-  float2* part;          // [tiles_m][N]
+  float2* part;          // [tiles_m][N]; or, where the hidden size is split,
+  int splits;
+  float* sums;           // [splits][N][ldk] products, and nothing else
   float* at_target;      // [N]
   // backward: over the listed rows
   const struct Row* row; // [count]
@@ -91,11 +93,12 @@ struct Row {
 };
 
 // ------------------------------------------------------------------------------------------ logits
-enum { FORWARD, REFORM, KEPT };  // the backward forms the logits again, or reads those that were kept
+// Forward: whole, or a part of the hidden size; backward: forms the logits again, or reads those that were kept
+enum { FORWARD, SPLIT, REFORM, KEPT };
 
 template <typename T, int S, int WAY>
 __global__ __launch_bounds__(THREADS_OF<S>) void lce_logits_kernel(const LogitArgs a) {
-  constexpr bool BACKWARD = WAY != FORWARD;
+  constexpr bool BACKWARD = WAY == REFORM || WAY == KEPT;
   typedef TileOf<T, S, true, true, false, BACKWARD> Tile;
   constexpr int BM = SHAPES[S].BM, BN = SHAPES[S].BN, WM = SHAPES[S].WM, WN = SHAPES[S].WN;
   constexpr int MI = Tile::MI, NI = Tile::NI;
@@ -105,16 +108,31 @@ __global__ __launch_bounds__(THREADS_OF<S>) void lce_logits_kernel(const LogitAr
   const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
   const int64_t N = BACKWARD ? uniform_of(a.count) : a.N;
   if (BACKWARD && n0 >= N) return;
+  int64_t k0 = 0, k1 = a.K;
+  if constexpr (WAY == SPLIT) {
+    const int64_t per = ((a.K + Tile::KSTEP - 1) / Tile::KSTEP + a.splits - 1) / a.splits * Tile::KSTEP;
+    k0 = per * blockIdx.y;
+    k1 = k0 + per < a.K ? k0 + per : a.K;
+  }
   f32x4 acc[MI][NI];
   if constexpr (WAY != KEPT)
-    Tile::run(acc, (lds_char*)smem, a.W, a.ldw, nullptr, m0, a.V, a.X, a.ldx, a.list, n0, N, 0, a.K);
+    Tile::run(acc, (lds_char*)smem, a.W, a.ldw, nullptr, m0, a.V, a.X, a.ldx, a.list, n0, N, k0, k1);
 
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / WN, wn = wave % WN;
   const int g = lane >> 4, col = lane & 15;
   const int64_t mw = m0 + wm * (BM / WM);               // this lane's rows: mw + row_of(i) + e
   const int rows = a.V - mw < BM ? (int)(a.V - mw) : BM;  // of them in the vocabulary (may be none)
   const T* bias = (const T*)a.bias;
-  if constexpr (WAY == KEPT) {
+  if constexpr (WAY == SPLIT) {
+    float* sums = a.sums + (int64_t)blockIdx.y * a.N * a.ldk + mw;
+#pragma unroll
+    for (int j = 0; j < NI; ++j) {
+      const int64_t n = n0 + wn * (BN / WN) + j * 16 + col;
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+        if (n < N && Tile::row_of(i) < rows) *(f32x4*)(sums + n * a.ldk + Tile::row_of(i)) = acc[i][j];
+    }
+  } else if constexpr (WAY == KEPT) {
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
       const int64_t n = n0 + wn * (BN / WN) + j * 16 + col;
@@ -143,7 +161,7 @@ __global__ __launch_bounds__(THREADS_OF<S>) void lce_logits_kernel(const LogitAr
     }
   }
 
-  if constexpr (!BACKWARD) {
+  if constexpr (WAY == FORWARD) {
     if (a.kept) {
 #pragma unroll
       for (int j = 0; j < NI; ++j) {
@@ -197,7 +215,7 @@ __global__ __launch_bounds__(THREADS_OF<S>) void lce_logits_kernel(const LogitAr
       }
       if (n0 + c < a.N) a.part[(int64_t)tm * a.N + n0 + c] = make_float2(top, sum);
     }
-  } else {
+  } else if constexpr (BACKWARD) {
     T* dl = (T*)a.dl;
     const int wide = a.ldl - mw < BM ? (int)(a.ldl - mw) : BM;  // ldl is a multiple of 64
 #pragma unroll
@@ -588,6 +606,75 @@ __global__ __launch_bounds__(1024) void lce_rows_kernel(const RowArgs a) {
   }
 }
 
+// The same from products split over the hidden size: a row's 1024 / rows threads (whole waves) add up the parts in order,
+// four entries a thread, with the running maximum and sum of the exponentials.
+struct SplitArgs {
+  const float* sums;     // [splits][N][ldk]
+  int splits;
+  int64_t ldk;
+  const void* bias;
+  float scale;
+  float* kept;           // [N][ldk] or null
+};
+
+template <typename T> __global__ __launch_bounds__(1024) void lce_split_rows_kernel(const SplitArgs b, const RowArgs a) {
+  __shared__ float2 red[16];
+  __shared__ float hit[16];
+  const int per = 1024 / a.rows, i = threadIdx.x % per, row = threadIdx.x / per, wave = threadIdx.x >> 6;
+  const int64_t n = (int64_t)blockIdx.x * a.rows + row;
+  const bool here = n < a.N;
+  const int64_t t = here ? target_of(a.targets, a.id_bits, n) : -1;
+  if (i == 0) hit[row] = 0.0f;
+  __syncthreads();
+  float top = -__builtin_inff(), sum = 0.0f;
+  for (int64_t v = i * 4; here && v < a.V; v += per * 4) {
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+    const float* from = b.sums + n * b.ldk + v;
+#pragma unroll 8
+    for (int k = 0; k < b.splits; ++k) x += *(const f32x4*)(from + (int64_t)k * a.N * b.ldk);
+    float most = -__builtin_inff();
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      x[e] = v + e < a.V ? (x[e] + (b.bias ? (float)((const T*)b.bias)[v + e] : 0.0f)) * b.scale : -__builtin_inff();
+      most = fmaxf(most, x[e]);
+      if (v + e == t) hit[row] = x[e];
+    }
+    if (b.kept) *(f32x4*)(b.kept + n * b.ldk + v) = x;
+    const float m = fmaxf(top, most);
+    float s = 0.0f;
+    // below -inf there is nothing to rescale; a NaN logit is not in the maximum and stays in the sum
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s += x[e] == -__builtin_inff() ? 0.0f : expf(m == -__builtin_inff() ? x[e] : x[e] - m);
+    sum = (top == -__builtin_inff() ? sum : sum * expf(top - m)) + s;
+    top = m;
+  }
+  const auto join = [](float2 p, float2 q) {
+    const float m = fmaxf(p.x, q.x);
+    return make_float2(m, (p.x == -__builtin_inff() ? p.y : p.y * expf(p.x - m)) + (q.x == -__builtin_inff() ? q.y : q.y * expf(q.x - m)));
+  };
+  float2 p = make_float2(top, sum);
+  for (int o = 32; o > 0; o >>= 1) p = join(p, make_float2(__shfl_xor(p.x, o, 64), __shfl_xor(p.y, o, 64)));
+  if ((threadIdx.x & 63) == 0) red[wave] = p;
+  __syncthreads();
+  float nll = 0.0f;
+  bool in = false;
+  if (i == 0 && here) {
+    for (int w = 1; w < per / 64; ++w) p = join(p, red[wave + w]);
+    const float lse = p.x + logf(p.y);
+    a.lse[n] = lse;
+    in = t != a.ignore;
+    if (in) nll = t >= 0 && t < a.V ? (lse - hit[row]) * (a.weight ? a.weight[n] : 1.0f) : __builtin_nanf("");
+    if (a.nll) a.nll[n] = nll;
+  }
+  if (a.sums) {
+    const LossPart q = block_sum((double)nll, in);
+    if (threadIdx.x == 0) {
+      if (a.loss) reduced_loss(q, a.mean, a.loss, a.count);
+      else a.sums[blockIdx.x] = q;
+    }
+  }
+}
+
 // count[0] = rows with a target; loss[0] = sum of nll (mean: over those rows; 0 without any).  One workgroup
 // over the workgroups of the rows, sums in fp64, in one order.
 __global__ __launch_bounds__(1024) void lce_loss_kernel(const LossPart* __restrict__ sums, int n, int mean,
@@ -828,15 +915,36 @@ int rows_of(int64_t N, int64_t tiles) {
   return rows;
 }
 
+// Few tiles (a small batch over a small vocabulary) are bound by the latency of their stages, one after the other: the
+// hidden size is split over the chip, into 16 parts at most of four stages at least (logits and rows; fp32 20 tokens of
+// 4096 over 100: 148 us whole, 22 in 16 parts, 22 in 32; 20 of 512 over 60: 27 whole, 18 in two parts, 14 in four; bf16 20
+// of 4096 over 3000: 35 and 17).
+struct FwdPlan {
+  int s, splits, rows;   // tile shape; rows a workgroup joins
+  int64_t groups;        // of rows
+};
+
+FwdPlan fwd_plan(const Problem& p) {
+  FwdPlan f;
+  f.s = logits_shape(p.V, p.N, p.Hp, (int64_t)p.eb, false);
+  const int64_t tiles = tiles_of(f.s, p.V, p.N), want = 2 * CUS / tiles;
+  const int64_t stages = p.Hp * (int64_t)p.eb / SHAPES[f.s].KB, most = stages / 4 < 16 ? stages / 4 : 16;
+  f.splits = (int)(want < most ? want : most);
+  if (f.splits < 2 || f.s == S256 || f.s == SM64) f.splits = 1;
+  f.rows = f.splits > 1 ? (p.V <= 256 ? 16 : p.V <= 1024 ? 4 : 1) : rows_of(p.N, div_up(p.V, SHAPES[f.s].BM));
+  f.groups = div_up(p.N, f.rows);
+  return f;
+}
+
 Layout fwd_layout(const Problem& p) {
   Layout L = {};
   Taker take;
   L.xp = take(p.pack_x ? (size_t)p.N * p.Hp * p.eb : 0);
   L.wp = take(p.pack_w ? (size_t)p.V * p.Hp * p.eb : 0);
-  const int s = logits_shape(p.V, p.N, p.Hp, (int64_t)p.eb, false);
-  L.part = take((size_t)div_up(p.V, SHAPES[s].BM) * p.N * sizeof(float2));
+  const FwdPlan f = fwd_plan(p);
+  L.part = take(f.splits > 1 ? (size_t)f.splits * p.N * up(p.V, 4) * 4 : (size_t)div_up(p.V, SHAPES[f.s].BM) * p.N * sizeof(float2));
   L.at = take((size_t)p.N * 4);
-  L.sums = take((size_t)div_up(p.N, rows_of(p.N, div_up(p.V, SHAPES[s].BM))) * sizeof(LossPart));
+  L.sums = take((size_t)f.groups * sizeof(LossPart));
   L.bytes = take.at + 256;
   return L;
 }
@@ -906,8 +1014,9 @@ template <typename T, int S, int WAY> int launch_logits(const LogitArgs& a, hipS
   static std::atomic<unsigned long long> done{0};
   if (const hipError_t e = pmg_full_lds_once((const void*)&lce_logits_kernel<T, S, WAY>, &done)) return (int)e;
   // without the product only the sums over the tokens are in LDS
-  constexpr int LDS = WAY == KEPT ? SHAPES[S].WN * SHAPES[S].BM * (int)sizeof(float) : TileOf<T, S, true, true, false, WAY != FORWARD>::LDS;
-  hipLaunchKernelGGL((lce_logits_kernel<T, S, WAY>), dim3((unsigned)((int64_t)a.tiles_m * a.tiles_n)), dim3(THREADS_OF<S>), LDS, st, a);
+  constexpr int LDS = WAY == KEPT ? SHAPES[S].WN * SHAPES[S].BM * (int)sizeof(float) : TileOf<T, S, true, true, false, WAY == REFORM>::LDS;
+  hipLaunchKernelGGL((lce_logits_kernel<T, S, WAY>), dim3((unsigned)((int64_t)a.tiles_m * a.tiles_n), WAY == SPLIT ? a.splits : 1),
+                     dim3(THREADS_OF<S>), LDS, st, a);
   return (int)hipGetLastError();
 }
 
@@ -915,14 +1024,18 @@ template <typename T, int WAY> int logits(int s, LogitArgs a, hipStream_t st) {
   a.tiles_m = (int)div_up(a.V, SHAPES[s].BM);
   a.tiles_n = (int)div_up(a.N, SHAPES[s].BN);
   if ((int64_t)a.tiles_m * a.tiles_n > 0x7fffffff) return PMG_E_ARG;
-  if (s == SM64) return launch_logits<T, SM64, WAY>(a, st);
+  if constexpr (WAY != SPLIT) {
+    if (s == SM64) return launch_logits<T, SM64, WAY>(a, st);
+    if constexpr (WAY != KEPT)
+      if (s == S256) return launch_logits<T, S256, WAY>(a, st);
+    if constexpr (WAY == FORWARD)
+      if (s == SK16W) return launch_logits<T, SK16W, WAY>(a, st);
+  }
   if constexpr (WAY != KEPT) switch (s) {
-      case S256: return launch_logits<T, S256, WAY>(a, st);
       case S128: return launch_logits<T, S128, WAY>(a, st);
       case S64: return launch_logits<T, S64, WAY>(a, st);
     }
-  if constexpr (WAY == FORWARD) switch (s) {
-      case SK16W: return launch_logits<T, SK16W, WAY>(a, st);
+  if constexpr (WAY == FORWARD || WAY == SPLIT) switch (s) {
       case SK16: return launch_logits<T, SK16, WAY>(a, st);
       case SK32: return launch_logits<T, SK32, WAY>(a, st);
       case SK64: return launch_logits<T, SK64, WAY>(a, st);
@@ -1011,12 +1124,14 @@ template <typename T> int forward(const pmg_linear_ce* a, const Problem& p, char
   l.v0 = 0;
   l.part = (float2*)(ws + L.part);
   l.at_target = (float*)(ws + L.at);
-  const int s = logits_shape(p.V, p.N, p.Hp, (int64_t)p.eb, false);
-  if (const int rc = logits<T, FORWARD>(s, l, st)) return rc;
+  const FwdPlan f = fwd_plan(p);
+  l.splits = f.splits;
+  l.sums = (float*)(ws + L.part);
+  if (const int rc = f.splits > 1 ? logits<T, SPLIT>(f.s, l, st) : logits<T, FORWARD>(f.s, l, st)) return rc;
   RowArgs r = {};
   r.part = l.part;
   r.at_target = l.at_target;
-  r.tiles = (int)div_up(p.V, SHAPES[s].BM);
+  r.tiles = (int)div_up(p.V, SHAPES[f.s].BM);
   r.N = p.N; r.V = p.V;
   r.targets = a->targets; r.id_bits = a->id_bits; r.ignore = a->ignore_index;
   r.weight = a->row_weight;
@@ -1024,14 +1139,19 @@ template <typename T> int forward(const pmg_linear_ce* a, const Problem& p, char
   const bool none = a->reduction == PMG_REDUCE_NONE;
   r.nll = none ? a->loss : nullptr;
   r.sums = none ? nullptr : (LossPart*)(ws + L.sums);
-  r.rows = rows_of(p.N, r.tiles);
-  const int groups = (int)div_up(p.N, r.rows);
+  r.rows = f.rows;
+  const int groups = (int)f.groups;
   r.mean = a->reduction == PMG_REDUCE_MEAN;
   if (groups == 1 && !none) {
     r.loss = a->loss;
     r.count = a->count;
   }
-  hipLaunchKernelGGL(lce_rows_kernel, dim3((unsigned)groups), dim3(1024), 0, st, r);
+  if (f.splits > 1) {
+    const SplitArgs b = {l.sums, f.splits, l.ldk, a->bias, a->logit_scale, a->logits};
+    hipLaunchKernelGGL(lce_split_rows_kernel<T>, dim3((unsigned)groups), dim3(1024), 0, st, b, r);
+  } else {
+    hipLaunchKernelGGL(lce_rows_kernel, dim3((unsigned)groups), dim3(1024), 0, st, r);
+  }
   if (!none && groups > 1)
     hipLaunchKernelGGL(lce_loss_kernel, dim3(1), dim3(1024), 0, st, r.sums, groups, r.mean, a->loss, a->count);
   return (int)hipGetLastError();

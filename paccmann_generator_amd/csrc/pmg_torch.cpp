@@ -342,10 +342,12 @@ std::tuple<Tensor, Tensor, Tensor> linear_ce_autograd(const Tensor& hidden, cons
                                                       const Tensor& targets, const OptTensor& row_weight, int64_t ignore_index,
                                                       double logit_scale, int64_t reduction) {
   // Training keeps logits that take at most a quarter of the bytes of the hidden rows they are made of: reading them (and
-  // their slopes) is then cheaper than reading the hidden rows once more, before any product.  524288 rows of 512 fp32 over
-  // 60: KEPT us a step, REFORMED without.
+  // their slopes) is cheaper than reading the hidden rows once more, before any product (524288 rows of 512 fp32 over 60:
+  // 1146 us a step, 1544 without).  And 4 MB of any: forming few takes the latency of a product (5 rows of 1024 bf16 over
+  // 50000: 5 us to read them, 18 to form them).
   const bool grads = at::GradMode::is_enabled() && (hidden.requires_grad() || weight.requires_grad() || (bias && bias->requires_grad()));
-  const bool keep = grads && weight.dim() == 2 && 16 * weight.sym_size(0) <= weight.sym_size(1) * weight.element_size();
+  const bool keep = grads && weight.dim() == 2 && (16 * weight.sym_size(0) <= weight.sym_size(1) * weight.element_size() ||
+                                                   targets.sym_numel() * weight.sym_size(0) <= (1 << 20));
   auto out = LinearCeGrad::apply(hidden, weight, bias, targets, row_weight, ignore_index, logit_scale, reduction, keep);
   return {out[0], out[1], out[2]};
 }

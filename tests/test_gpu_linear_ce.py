@@ -365,3 +365,41 @@ def test_gradients_are_not_differentiated_again(gpu):
     for p in got:
         with pytest.raises(RuntimeError, match='not differentiable'):
             torch.autograd.grad(p.sum(), z, allow_unused=True, retain_graph=True)
+
+
+# Few tiles and a long hidden size: the products are split over it
+LONG = [(1, 3, 2000), (16, 100, 4096), (17, 300, 1032), (64, 1030, 2048), (300, 300, 2001), (5, 12000, 1032), (700, 60, 1024)]
+
+
+@pytest.mark.parametrize('dtype', TYPES, ids=str)
+@pytest.mark.parametrize('N,V,H', LONG)
+def test_hidden_size_split(gpu, dtype, N, V, H):
+    _check(*_data(N, V, H, dtype, seed=N + V + H))
+    _check(*_data(N, V, H, dtype, seed=N, bias=True, weighted=True, ignored=0.3), scale=0.7, reduction='none')
+
+
+def test_masked_rows_of_a_split_hidden_size(gpu):
+    """Masked entries, rows without any entry, and rows with NaN that stay apart."""
+    from paccmann_generator_amd import ops
+    N, V, H = 20, 90, 2048
+    x, w, b, t, _ = _data(N, V, H, torch.float32, seed=6, bias=True)
+    t = t % 40
+    b[40:] = -float('inf')
+    with torch.no_grad():
+        _, lse = ops.linear_cross_entropy(*_cuda(x, w, t), bias=b.cuda())
+        _, want = ops.linear_cross_entropy(*_cuda(x, w[:40], t), bias=b[:40].cuda())
+        assert torch.allclose(lse, want, rtol=1e-6, atol=0)
+        _, lse = ops.linear_cross_entropy(*_cuda(x, w, t), bias=torch.full((V,), torch.finfo(torch.float32).min).cuda())
+        assert bool((lse <= torch.finfo(torch.float32).min * 0.99).all())
+        _, lse = ops.linear_cross_entropy(*_cuda(x, w, t), bias=torch.full((V,), -float('inf')).cuda())
+        assert bool((lse == -float('inf')).all())
+        x[3] = float('nan')
+        loss, lse = ops.linear_cross_entropy(*_cuda(x, w, t), bias=b.cuda(), reduction='none')
+        rest = torch.arange(N) != 3
+        assert bool(lse[3].isnan()) and bool(loss[3].isnan()) and torch.equal(lse.cpu()[rest].isnan(), torch.zeros(N - 1, dtype=torch.bool))
+        assert torch.allclose(lse.cpu()[rest], want.cpu()[rest], rtol=1e-6, atol=0)
+    # ignored, the row with NaN leaves every gradient alone
+    t[3] = -100
+    z = [v.requires_grad_(True) for v in _cuda(x, w, b)]
+    got = torch.autograd.grad(ops.linear_cross_entropy(z[0], z[1], t.cuda(), bias=z[2])[0], z)
+    assert not any(bool(g.isnan().any()) for g in got) and not got[0][3].any()
