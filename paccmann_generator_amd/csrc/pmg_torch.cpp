@@ -338,16 +338,26 @@ struct LinearCeGrad : torch::autograd::Function<LinearCeGrad> {
   }
 };
 
+// Whether training keeps the logits, in fp32, rather than form them again.
+//   - a row of them takes at most a quarter of the bytes of the hidden row it is made of: reading them (and their slopes) is
+//     cheaper than reading the hidden rows once more, before any product (524288 rows of 512 fp32 over 60: 1146 us a step,
+//     1544 without)
+//   - all of them take 4 MB: forming few takes the latency of a product (5 rows of 1024 bf16 over 50000: 5 us to read them,
+//     18 to form them)
+//   - all of them take 256 MB, no more than the backward's own scratch, and the hidden size is long enough for writing and
+//     reading 8 bytes to take less than 2 H operations (bf16 8000
+//     rows of 1024 over 8000: 108 us to write and read them, 142 to form them; 2000 of 4096 over 32000: 136 and 466; fp32
+//     30000 of 136 over 2000: 132 and 198)
+bool keep_logits(int64_t n, int64_t v, int64_t h, int64_t size) {
+  const int64_t all = n * v;
+  return 16 * v <= h * size || all <= (1 << 20) || (all <= (64 << 20) && h >= (size == 4 ? 128 : 1024));
+}
+
 std::tuple<Tensor, Tensor, Tensor> linear_ce_autograd(const Tensor& hidden, const Tensor& weight, const OptTensor& bias,
                                                       const Tensor& targets, const OptTensor& row_weight, int64_t ignore_index,
                                                       double logit_scale, int64_t reduction) {
-  // Training keeps logits that take at most a quarter of the bytes of the hidden rows they are made of: reading them (and
-  // their slopes) is cheaper than reading the hidden rows once more, before any product (524288 rows of 512 fp32 over 60:
-  // 1146 us a step, 1544 without).  And 4 MB of any: forming few takes the latency of a product (5 rows of 1024 bf16 over
-  // 50000: 5 us to read them, 18 to form them).
   const bool grads = at::GradMode::is_enabled() && (hidden.requires_grad() || weight.requires_grad() || (bias && bias->requires_grad()));
-  const bool keep = grads && weight.dim() == 2 && (16 * weight.sym_size(0) <= weight.sym_size(1) * weight.element_size() ||
-                                                   targets.sym_numel() * weight.sym_size(0) <= (1 << 20));
+  const bool keep = grads && weight.dim() == 2 && keep_logits(targets.numel(), weight.size(0), weight.size(1), weight.element_size());
   auto out = LinearCeGrad::apply(hidden, weight, bias, targets, row_weight, ignore_index, logit_scale, reduction, keep);
   return {out[0], out[1], out[2]};
 }

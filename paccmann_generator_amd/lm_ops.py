@@ -111,8 +111,7 @@ def linear_cross_entropy(hidden: Tensor, weight: Tensor, targets: Tensor, bias: 
                          row_weight: Optional[Tensor] = None, ignore_index: int = -100, logit_scale: float = 1.0,
                          reduction: str = 'mean', trusted_tokens: bool = False) -> Tuple[Tensor, Tensor]:
     """(loss, lse) of ``logit_scale * (hidden @ weight.T + bias)`` against ``targets``.  The logits are not kept
-    (for training they are where a row of them, in fp32, takes at most a quarter of the bytes of a hidden row, or all of
-    them 4 MB).
+    for training, save up to 256 MB of them, in fp32, or where a row takes at most a quarter of the bytes of a hidden row.
 
     ``hidden`` [..., H], ``weight`` [V, H] and ``bias`` [V] are all fp32 or all bf16; ``targets`` [...] int64 or int32.
     The loss of a row is its negative log-probability times ``row_weight`` (fp32 [...], a reward say; it gets no
