@@ -348,16 +348,16 @@ struct LinearCeGrad : torch::autograd::Function<LinearCeGrad> {
 //     reading 8 bytes to take less than 2 H operations (bf16 8000
 //     rows of 1024 over 8000: 108 us to write and read them, 142 to form them; 2000 of 4096 over 32000: 136 and 466; fp32
 //     30000 of 136 over 2000: 132 and 198)
-bool keep_logits(int64_t n, int64_t v, int64_t h, int64_t size) {
-  const int64_t all = n * v;
-  return 16 * v <= h * size || all <= (1 << 20) || (all <= (64 << 20) && h >= (size == 4 ? 128 : 1024));
+bool keep_logits(const c10::SymInt& n, const c10::SymInt& v, const c10::SymInt& h, int64_t size) {
+  const c10::SymInt all = n * v;
+  return v * 16 <= h * size || all <= (1 << 20) || (all <= (64 << 20) && h >= (size == 4 ? 128 : 1024));
 }
 
 std::tuple<Tensor, Tensor, Tensor> linear_ce_autograd(const Tensor& hidden, const Tensor& weight, const OptTensor& bias,
                                                       const Tensor& targets, const OptTensor& row_weight, int64_t ignore_index,
                                                       double logit_scale, int64_t reduction) {
   const bool grads = at::GradMode::is_enabled() && (hidden.requires_grad() || weight.requires_grad() || (bias && bias->requires_grad()));
-  const bool keep = grads && weight.dim() == 2 && keep_logits(targets.numel(), weight.size(0), weight.size(1), weight.element_size());
+  const bool keep = grads && weight.dim() == 2 && keep_logits(targets.sym_numel(), weight.sym_size(0), weight.sym_size(1), weight.element_size());
   auto out = LinearCeGrad::apply(hidden, weight, bias, targets, row_weight, ignore_index, logit_scale, reduction, keep);
   return {out[0], out[1], out[2]};
 }

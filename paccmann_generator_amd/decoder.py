@@ -91,7 +91,7 @@ class StackGRUDecoder(nn.Module):
                    reduction: str = 'mean', trusted_tokens: bool = False):
         """Negative log-probability of ``targets`` [...] under ``output_layer(hidden [..., H]) / temperature``, times
         ``reward`` [...] where given: output_layer, log_softmax, gather and the reward-weighted mean of
-        reinforce_omics.py:326-332 without keeping the logits, for a vocabulary of any size."""
+        reinforce_omics.py:326-332 without keeping large logits, for a vocabulary of any size."""
         loss, _ = ops.linear_cross_entropy(hidden, self.output_layer.weight, targets, bias=self.output_layer.bias,
                                            row_weight=reward, ignore_index=ignore_index, logit_scale=1.0 / temperature,
                                            reduction=reduction, trusted_tokens=trusted_tokens)

@@ -2,7 +2,7 @@
 
     torch.ops.pmg.embedding                -> pmg_embedding_fwd   rows of a table by token id, scaled; differentiable
     torch.ops.pmg.embedding_bwd            -> pmg_embedding_bwd   the gradient of the table, by sorted tokens
-    torch.ops.pmg.linear_cross_entropy     -> pmg_linear_ce_fwd   loss over a vocabulary, logits not kept; differentiable
+    torch.ops.pmg.linear_cross_entropy     -> pmg_linear_ce_fwd   loss over a vocabulary, large logits not kept; differentiable
     torch.ops.pmg.linear_cross_entropy_bwd -> pmg_linear_ce_bwd   its gradients
     torch.ops.pmg.grad_norm                -> pmg_grad_norm       norm over many gradients
     torch.ops.pmg.clip_grad_norm_          -> pmg_grad_norm, pmg_grad_clip   and their scaling, in place
@@ -110,8 +110,8 @@ def _(grad_loss, grad_lse, hidden, weight, bias, targets, row_weight, lse, count
 def linear_cross_entropy(hidden: Tensor, weight: Tensor, targets: Tensor, bias: Optional[Tensor] = None,
                          row_weight: Optional[Tensor] = None, ignore_index: int = -100, logit_scale: float = 1.0,
                          reduction: str = 'mean', trusted_tokens: bool = False) -> Tuple[Tensor, Tensor]:
-    """(loss, lse) of ``logit_scale * (hidden @ weight.T + bias)`` against ``targets``.  The logits are not kept
-    for training, save up to 256 MB of them, in fp32, or where a row takes at most a quarter of the bytes of a hidden row.
+    """(loss, lse) of ``logit_scale * (hidden @ weight.T + bias)`` against ``targets``, without keeping the logits: for
+    training at most 256 MB of them are, in fp32, or any number whose rows take a quarter of the bytes of a hidden row.
 
     ``hidden`` [..., H], ``weight`` [V, H] and ``bias`` [V] are all fp32 or all bf16; ``targets`` [...] int64 or int32.
     The loss of a row is its negative log-probability times ``row_weight`` (fp32 [...], a reward say; it gets no
