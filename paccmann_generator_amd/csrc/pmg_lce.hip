@@ -38,12 +38,14 @@ template <> __device__ __forceinline__ float exp_of<bf16_t>(float x) { return __
 // products with fp32 result, bf16 (operands with k / m and k / m contiguous), TFLOP/s: the large square 1152 / 1281 /
 // 1303 at 8192 x 8192 x 4096 (4096 x 8192 x 8192), the middle one 1067 / 1029 / 968; with two stages of 128 bytes the
 // large one gets 950 / 1007 / 1216, with four waves the middle one 906 / 989 / 929.  fp32: 142, of 157 the units give.
+// 64 words by 128 tokens, 524288 x 512 fp32 over 60: 321 us with the waves along the tokens, 340 in a square, 328 with 256
+// tokens; weights' gradient there 336 in a square, 318 with 256 of m, which costs bf16 2 %, 408 with two waves.
 struct Shape {
   int BM, BN, WM, WN, KB, stages, per_cu;
 };
 enum { S256, S128, S64, SN64, SM64, SK16W, SK16, SK32, SK64, SD64 };  // S: square, SN / SM / SD: 64 of n or m, SK: few tokens
 constexpr Shape SHAPES[] = {{256, 256, 2, 4, 64, 3, 1}, {128, 128, 2, 4, 128, 2, 2}, {64, 64, 2, 2, 128, 2, 5},
-                            {128, 64, 2, 2, 128, 2, 3}, {64, 128, 2, 2, 128, 2, 3},  {128, 16, 2, 1, 128, 2, 4},
+                            {128, 64, 2, 2, 128, 2, 3}, {64, 128, 1, 4, 128, 2, 3},  {128, 16, 2, 1, 128, 2, 4},
                             {64, 16, 2, 1, 128, 2, 8},  {128, 32, 2, 1, 128, 2, 4},  {128, 64, 2, 1, 128, 2, 3},
                             {128, 64, 2, 2, 64, 2, 6}};
 template <typename T, int S, bool AKC, bool BKC, bool ALIST, bool BLIST>
