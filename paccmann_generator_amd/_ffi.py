@@ -21,9 +21,9 @@ PMG_FLAG_NO_CLUSTER = 32
 PMG_ABI_VERSION = 3
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
-# PMG_LIB selects a tuning variant built by __graft_entry__.build(extra_flags=..., libname=...)
 # the PyTorch operators over include/pmg_lm.h (csrc/pmg_torch.cpp); links to lib/libpmg.so
 TORCH_LIB_PATH = os.path.join(_HERE, 'lib', 'libpmg_torch.so')
+# PMG_LIB selects a tuning variant built by __graft_entry__.build(extra_flags=..., libname=...)
 LIB_PATH = os.environ.get('PMG_LIB') or os.path.join(_HERE, 'lib', 'libpmg.so')
 
 
