@@ -113,11 +113,15 @@ __global__ __launch_bounds__(THREADS) void embed_count_kernel(const Src src, int
   for (int b = threadIdx.x; b < bins; b += THREADS) bin[b] = 0;
   __syncthreads();
   const int64_t base = (int64_t)blockIdx.x * (ROUNDS * ROUND);
+  uint32_t key[ROUNDS];
 #pragma unroll
   for (int r = 0; r < ROUNDS; ++r) {
     const int64_t i = base + r * THREADS + threadIdx.x;
-    if (i < N) atomicAdd(&bin[(src.key(i) >> shift) & (bins - 1)], 1);  // integers: any order, one result
+    key[r] = src.key(i < N ? i : N - 1);
   }
+#pragma unroll
+  for (int r = 0; r < ROUNDS; ++r)
+    if (base + r * THREADS + threadIdx.x < N) atomicAdd(&bin[(key[r] >> shift) & (bins - 1)], 1);  // integers: any order, one result
   __syncthreads();
   for (int b = threadIdx.x; b < bins; b += THREADS) count[(int64_t)b * tiles + blockIdx.x] = bin[b];
 }
@@ -184,13 +188,17 @@ __global__ __launch_bounds__(THREADS) void embed_scatter_kernel(const Src src, i
     __syncthreads();
   }
   const int64_t base = (int64_t)blockIdx.x * (ROUNDS * ROUND) + wave * (ROUNDS * 64) + lane;
-  uint32_t key[ROUNDS];
+  uint32_t key[ROUNDS], from[ROUNDS];
   uint64_t same[ROUNDS];
 #pragma unroll
   for (int r = 0; r < ROUNDS; ++r) {
-    const int64_t i = base + r * 64;
-    const bool in = i < N;
-    key[r] = in ? src.key(i) : 0;
+    const int64_t i = base + r * 64 < N ? base + r * 64 : N - 1;
+    key[r] = src.key(i);
+    from[r] = src.pos(i);
+  }
+#pragma unroll
+  for (int r = 0; r < ROUNDS; ++r) {
+    const bool in = base + r * 64 < N;
     const int d = (key[r] >> shift) & (bins - 1);
     uint64_t m = __ballot(in);
     for (int b = 0; b < bits; ++b) {
@@ -219,7 +227,7 @@ __global__ __launch_bounds__(THREADS) void embed_scatter_kernel(const Src src, i
       const int at = place[wave][d];
       wave_sync();
       keys[at + rank] = key[r];
-      pos[at + rank] = src.pos(base + r * 64);
+      pos[at + rank] = from[r];
       if (rank == 0) place[wave][d] = at + __popcll(same[r]);
     }
     wave_sync();
@@ -236,7 +244,11 @@ struct ReduceArgs {
   float* part;               // [chunks][2][E]: [0] of the run that began earlier, [1] of the run that goes on
 };
 
-template <typename T>
+// WHOLE: rows of 16 bytes or more; the last 16 bytes of a row that is no multiple of them overlap those before (both
+// threads form and write the same values), so that no load needs a branch: loads with branches between them wait for each
+// other (32767 x 2048 bf16: 74 us, 79 with branches; 417792 x 128 fp32: 52 and 61; 524288 x 512 bf16: 160 and 173, joining
+// 34 and 48).
+template <typename T, bool WHOLE>
 __global__ __launch_bounds__(THREADS) void embed_reduce_kernel(const ReduceArgs a, const T* __restrict__ g,
                                                                T* __restrict__ dW) {
   constexpr int VEC = pmg_vec16<T>::N;
@@ -274,10 +286,11 @@ __global__ __launch_bounds__(THREADS) void embed_reduce_kernel(const ReduceArgs 
     if (i >= 1 && i <= per && p < a.N) pos[i - 1] = a.pos[p];
   }
   __syncthreads();
-  const int64_t c = ((int64_t)blockIdx.y * a.tpr + (threadIdx.x & (a.tpr - 1))) * VEC;
+  int64_t c = ((int64_t)blockIdx.y * a.tpr + (threadIdx.x & (a.tpr - 1))) * VEC;
   const int grp = threadIdx.x / a.tpr;
   const int64_t ch = (int64_t)blockIdx.x * (THREADS / a.tpr) + grp;
   if (c >= a.E || ch >= a.chunks) return;
+  if (WHOLE && c > a.E - VEC) c = a.E - VEC;
   const int lo = grp * a.chunk, n = (int)(a.N - ch * a.chunk < a.chunk ? a.N - ch * a.chunk : a.chunk);
   const uint32_t* k = key + 1 + lo;  // k[-1] and k[n]: the neighbours
   const uint32_t* at = pos + lo;
@@ -285,29 +298,31 @@ __global__ __launch_bounds__(THREADS) void embed_reduce_kernel(const ReduceArgs 
 #pragma unroll
   for (int j = 0; j < VEC; ++j) acc[j] = 0.0f;
   uint32_t cur = k[0];
+  if (cur >= (uint32_t)a.V) return;  // dropped positions sort last
   bool before = k[-1] == cur;
-  auto put_part = [&](int slot) {
+  auto put_part = [&](int slot) __attribute__((always_inline)) {
     float* p = a.part + (ch * 2 + slot) * a.E + c;
 #pragma unroll
     for (int j = 0; j < VEC; j += 4) {
-      if (c + j < a.E) pmg_store4(p + j, f32x4{acc[j], acc[j + 1], acc[j + 2], acc[j + 3]}, a.E - c - j);
+      if (WHOLE || c + j < a.E) pmg_store4(p + j, f32x4{acc[j], acc[j + 1], acc[j + 2], acc[j + 3]}, WHOLE ? 4 : a.E - c - j);
     }
   };
-  auto put_row = [&]() {
+  auto put_row = [&]() __attribute__((always_inline)) {
     float y[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; ++j) y[j] = acc[j] * a.scale;
-    pmg_vec16<T>::store(dW + (int64_t)cur * a.E + c, y, a.E - c);
+    pmg_vec16<T>::store(dW + (int64_t)cur * a.E + c, y, WHOLE ? VEC : a.E - c);
   };
   typedef typename pmg_vec16<T>::vec vec;
   vec x[2][U];
-  auto load = [&](vec(&v)[U], int i) {
+  // no branches between the loads (behind the end the last row again; dropped positions have a row too)
+  auto load = [&](vec(&v)[U], int i) __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (i + u < n && k[i + u] < (uint32_t)a.V) v[u] = pmg_vec16<T>::load(g + (int64_t)at[i + u] * a.ldg + c, a.E - c);
+      v[u] = pmg_vec16<T>::load(g + (int64_t)at[i + u < n ? i + u : n - 1] * a.ldg + c, WHOLE ? VEC : a.E - c);
   };
   // false: what follows takes no part (dropped positions sort last)
-  auto add = [&](const vec(&v)[U], int i) {
+  auto add = [&](const vec(&v)[U], int i) __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (i + u < n) {
@@ -343,7 +358,7 @@ __global__ __launch_bounds__(THREADS) void embed_reduce_kernel(const ReduceArgs 
 // tokens are frequent, with two or three parts each: small workgroups, 43 us with 1024 threads at 32767 x 2048): the
 // parts of the run are dealt to the workgroup's groups of tpr threads in turn, and the groups' sums are
 // added in order.
-template <typename T>
+template <typename T, bool WHOLE>
 __global__ __launch_bounds__(JOIN_THREADS) void embed_join_kernel(const ReduceArgs a, T* __restrict__ dW) {
   constexpr int VEC = pmg_vec16<T>::N;
   __shared__ float sum[JOIN_THREADS * VEC];
@@ -367,18 +382,20 @@ __global__ __launch_bounds__(JOIN_THREADS) void embed_join_kernel(const ReduceAr
     __syncthreads();
   }
   const int groups = JOIN_THREADS / a.tpr, grp = threadIdx.x / a.tpr, t = threadIdx.x & (a.tpr - 1);
-  const int64_t c = ((int64_t)blockIdx.y * a.tpr + t) * VEC;
+  int64_t c = ((int64_t)blockIdx.y * a.tpr + t) * VEC;
+  const bool in = c < a.E;
+  if (WHOLE && c > a.E - VEC) c = a.E - VEC;
   float acc[VEC];
 #pragma unroll
   for (int j = 0; j < VEC; ++j) acc[j] = 0.0f;
-  if (c < a.E) {
+  if (in) {
 #pragma unroll 16
     for (int64_t k = ch + grp; k <= last; k += groups) {  // long runs: many loads under way
       const float* p = a.part + (k * 2 + (k == ch ? 1 : 0)) * a.E + c;
 #pragma unroll
       for (int j = 0; j < VEC; j += 4) {
-        if (c + j < a.E) {
-          const f32x4 x = pmg_load4(p + j, a.E - c - j);
+        if (WHOLE || c + j < a.E) {
+          const f32x4 x = pmg_load4(p + j, WHOLE ? 4 : a.E - c - j);
           acc[j] += x.x; acc[j + 1] += x.y; acc[j + 2] += x.z; acc[j + 3] += x.w;
         }
       }
@@ -387,7 +404,7 @@ __global__ __launch_bounds__(JOIN_THREADS) void embed_join_kernel(const ReduceAr
 #pragma unroll
   for (int j = 0; j < VEC; ++j) sum[j * JOIN_THREADS + threadIdx.x] = acc[j];
   __syncthreads();
-  if (grp == 0 && c < a.E) {
+  if (grp == 0 && in) {
     float y[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
@@ -395,7 +412,7 @@ __global__ __launch_bounds__(JOIN_THREADS) void embed_join_kernel(const ReduceAr
       for (int q = 0; q < groups; ++q) s += sum[j * JOIN_THREADS + q * a.tpr + t];
       y[j] = s * a.scale;
     }
-    pmg_vec16<T>::store(dW + (int64_t)cur * a.E + c, y, a.E - c);
+    pmg_vec16<T>::store(dW + (int64_t)cur * a.E + c, y, WHOLE ? VEC : a.E - c);
   }
 }
 
@@ -530,9 +547,14 @@ int bwd(const void* g, int64_t ldg, const void* ids, int id_bits, int64_t N, int
   a.pos = (const uint32_t*)(ws + L.pos[at]);
   a.part = (float*)(ws + L.part);
   const int64_t blocks = a.reduce_blocks + (V + FILL_ROWS - 1) / FILL_ROWS;
-  hipLaunchKernelGGL(embed_reduce_kernel<T>, dim3((unsigned)blocks, (unsigned)cols), dim3(THREADS), 0, st, a, (const T*)g, (T*)dW);
-  if (L.chunks > 1)
-    hipLaunchKernelGGL(embed_join_kernel<T>, dim3((unsigned)L.chunks, (unsigned)cols), dim3(JOIN_THREADS), 0, st, a, (T*)dW);
+  const dim3 grid((unsigned)blocks, (unsigned)cols), joins((unsigned)L.chunks, (unsigned)cols);
+  if (E >= pmg_vec16<T>::N) {
+    hipLaunchKernelGGL((embed_reduce_kernel<T, true>), grid, dim3(THREADS), 0, st, a, (const T*)g, (T*)dW);
+    if (L.chunks > 1) hipLaunchKernelGGL((embed_join_kernel<T, true>), joins, dim3(JOIN_THREADS), 0, st, a, (T*)dW);
+  } else {
+    hipLaunchKernelGGL((embed_reduce_kernel<T, false>), grid, dim3(THREADS), 0, st, a, (const T*)g, (T*)dW);
+    if (L.chunks > 1) hipLaunchKernelGGL((embed_join_kernel<T, false>), joins, dim3(JOIN_THREADS), 0, st, a, (T*)dW);
+  }
   return (int)hipGetLastError();
 }
 

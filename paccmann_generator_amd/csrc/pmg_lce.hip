@@ -630,14 +630,20 @@ template <typename T> __global__ __launch_bounds__(1024) void lce_split_rows_ker
   __syncthreads();
   float top = -__builtin_inff(), sum = 0.0f;
   for (int64_t v = i * 4; here && v < a.V; v += per * 4) {
-    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+    f32x4 x = {0.f, 0.f, 0.f, 0.f}, bias = x;
+    if (b.bias) bias = pmg_load4((const T*)b.bias + v, a.V - v);
     const float* from = b.sums + n * b.ldk + v;
-#pragma unroll 8
-    for (int k = 0; k < b.splits; ++k) x += *(const f32x4*)(from + (int64_t)k * a.N * b.ldk);
+    for (int k = 0; k < b.splits; k += 8) {  // eight loads under way, added in order
+      f32x4 y[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) y[u] = *(const f32x4*)(from + (int64_t)(k + u < b.splits ? k + u : 0) * a.N * b.ldk);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) x += k + u < b.splits ? y[u] : f32x4{0.f, 0.f, 0.f, 0.f};
+    }
     float most = -__builtin_inff();
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      x[e] = v + e < a.V ? (x[e] + (b.bias ? (float)((const T*)b.bias)[v + e] : 0.0f)) * b.scale : -__builtin_inff();
+      x[e] = v + e < a.V ? (x[e] + bias[e]) * b.scale : -__builtin_inff();
       most = fmaxf(most, x[e]);
       if (v + e == t) hit[row] = x[e];
     }
@@ -922,8 +928,7 @@ int rows_of(int64_t N, int64_t tiles) {
 
 // Few tiles (a small batch over a small vocabulary) are bound by the latency of their stages, one after the other: the
 // hidden size is split over the chip, into 16 parts at most of four stages at least (logits and rows; fp32 20 tokens of
-// 4096 over 100: 148 us whole, 22 in 16 parts, 22 in 32; 20 of 512 over 60: 27 whole, 18 in two parts, 14 in four; bf16 20
-// of 4096 over 3000: 35 and 17).
+// 4096 over 100: 148 us whole, 18 in 16 parts; 20 of 512 over 60: 27 whole, 13 in four parts).
 struct FwdPlan {
   int s, splits, rows;   // tile shape; rows a workgroup joins
   int64_t groups;        // of rows

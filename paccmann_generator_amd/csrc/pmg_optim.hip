@@ -43,6 +43,23 @@ static_assert(sizeof(GradTable) <= 3800, "kernel arguments");
 template <typename T>
 __device__ __forceinline__ double square_sum(const T* __restrict__ g, int64_t n, int64_t lo, int chunk) {
   double s = 0.0;
+  // whole: loads of 16 bytes without a branch between them, eight under way (468 M bf16: 208 us, 229 with the loop below)
+  if (n - lo >= chunk) {
+    constexpr int VEC = pmg_vec16<T>::N;
+    for (int i = threadIdx.x * VEC; i < chunk; i += THREADS * VEC * 8) {
+      typename pmg_vec16<T>::vec x[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (i + u * THREADS * VEC < chunk) x[u] = pmg_vec16<T>::load(g + lo + i + u * THREADS * VEC, VEC);
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (i + u * THREADS * VEC < chunk) {
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) s = fma((double)(float)x[u][j], (double)(float)x[u][j], s);
+        }
+    }
+    return s;
+  }
 #pragma unroll 4
   for (int i = threadIdx.x * 4; i < chunk; i += THREADS * 4) {
     const int64_t left = n - lo - i;
