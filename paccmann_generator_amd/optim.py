@@ -39,6 +39,11 @@ class AdamW(torch.optim.Optimizer):
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=float(eps), weight_decay=float(weight_decay),
                                       decoupled=bool(decoupled)))
 
+    def __getstate__(self):
+        """What copies and pickles carry: the base class names its own attributes only."""
+        return dict(super().__getstate__(), state_bits=self.state_bits, master_weights=self.master_weights,
+                    max_grad_norm=self.max_grad_norm, grad_norm=self.grad_norm)
+
     def _init_state(self, p, step):
         s = self.state[p]
         s['step'] = step
