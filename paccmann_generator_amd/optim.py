@@ -123,30 +123,53 @@ class AdamW(torch.optim.Optimizer):
         state, groups = state_dict['state'], state_dict['param_groups']
         if any(g.get('amsgrad') or g.get('maximize') for g in groups):
             raise _ffi.PmgError('pmg: amsgrad and maximize are not supported')
+        # all states are converted before anything is replaced: a refused load leaves the optimizer as it was
+        loaded, shared = {}, {}
+        if [len(g['params']) for g in groups] == [len(g['params']) for g in self.param_groups]:    # else the base class refuses
+            for k, (given, mine) in enumerate(zip(groups, self.param_groups)):
+                for i, p in zip(given['params'], mine['params']):
+                    if state.get(i):
+                        s = loaded[p] = self._converted(p, state[i])
+                        # parameters of a group whose counters agree share one again
+                        s['step'] = shared.setdefault((k, p.device, int(s['step'])), s['step'])
         before = [dict(g) for g in self.param_groups]
         super().load_state_dict(dict(state={}, param_groups=groups))
         for g, old in zip(self.param_groups, before):
             for key, value in old.items():
                 g.setdefault(key, value)
-        ids = [i for g in groups for i in g['params']]
-        params = [(k, p) for k, g in enumerate(self.param_groups) for p in g['params']]
-        shared = {}
-        for i, (k, p) in zip(ids, params):
-            if i not in state or not state[i]:
-                continue
-            s = {name: torch.as_tensor(v).detach().to(p.device, copy=True) for name, v in state[i].items()}
-            s['step'] = s['step'].to(torch.int64).reshape(1)
-            if 'exp_avg_top' in s and self.state_bits == 32:
-                for name in ('exp_avg', 'exp_avg_sq'):
-                    s[name] = ops.adamw_state_values(s[name], s.pop(name + '_top'))
-            elif 'exp_avg_top' not in s and self.state_bits == 8:
-                raise _ffi.PmgError('pmg: a state of 32 bits does not load into an optimizer with 8')
-            if self.state_bits == 32:
-                s['exp_avg'], s['exp_avg_sq'] = s['exp_avg'].float(), s['exp_avg_sq'].float()
-            # parameters of a group whose counters agree share one again
-            s['step'] = shared.setdefault((k, p.device, int(s['step'])), s['step'])
-            if self.master_weights and p.dtype != torch.float32:
-                s.setdefault('master', p.detach().to(torch.float32))
-            else:
-                s.pop('master', None)
-            self.state[p] = s
+        self.state.update(loaded)
+
+    def _converted(self, p, given):
+        """The state of a checkpoint for ``p`` as this optimizer holds it."""
+        s = {name: torch.as_tensor(v).detach().to(p.device, copy=True) for name, v in given.items()}
+        moments = ('exp_avg', 'exp_avg_sq')
+        if any(name not in s for name in ('step', *moments)) or s['step'].numel() != 1:
+            raise _ffi.PmgError(f'pmg: a state needs a step, exp_avg and exp_avg_sq, got {sorted(given)}')
+        coded = [name + '_top' in s for name in moments]
+        for name, signed in zip(moments, (True, False)):
+            m, top = s[name], s.get(name + '_top')
+            if m.shape != p.shape:
+                raise _ffi.PmgError(f'pmg: {name} of shape {tuple(m.shape)} for a parameter {tuple(p.shape)}')
+            if any(coded) and (not all(coded) or m.dtype != (torch.int8 if signed else torch.uint8) or top.dtype != torch.float32
+                               or top.numel() != -(-p.numel() // _ffi.PMG_STATE_BLOCK)):
+                raise _ffi.PmgError('pmg: a state of 8 bits needs int8 and uint8 codes and a scale per block of each')
+            if not any(coded) and not m.is_floating_point():
+                raise _ffi.PmgError(f'pmg: {name} of 32 bits must be a floating-point tensor, got {m.dtype}')
+        if self.state_bits == 8 and not all(coded):
+            raise _ffi.PmgError('pmg: a state of 32 bits does not load into an optimizer with 8')
+        s['step'] = s['step'].to(torch.int64).reshape(1)
+        like = torch.empty_like(p.detach(), dtype=torch.float32)     # in the parameter's memory order, as the update asks for
+        if self.state_bits == 32:
+            for name in moments:
+                m = ops.adamw_state_values(s[name], s.pop(name + '_top')) if all(coded) else s[name]
+                s[name] = torch.empty_like(like).copy_(m)
+        elif any(s[name].stride() != like.stride() and not (s[name].is_contiguous() and like.is_contiguous()) for name in moments):
+            raise _ffi.PmgError('pmg: the blocks of a state of 8 bits follow the memory order, which is another than the parameter\'s')
+        if self.master_weights and p.dtype != torch.float32:
+            master = s.get('master', p.detach())
+            if master.shape != p.shape:
+                raise _ffi.PmgError(f'pmg: a copy of shape {tuple(master.shape)} for a parameter {tuple(p.shape)}')
+            s['master'] = like.copy_(master)
+        else:
+            s.pop('master', None)
+        return s

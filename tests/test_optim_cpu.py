@@ -54,3 +54,64 @@ def test_copies_keep_the_settings(through):
     # a load replaces groups and state, not the settings
     again.load_state_dict(opt.state_dict())
     assert all(getattr(again, k) == x for k, x in KEPT.items())
+
+
+def _frozen(opt):
+    return ([{k: x for k, x in g.items() if k != 'params'} for g in opt.param_groups],
+            [{k: x.clone() for k, x in opt.state[p].items()} for g in opt.param_groups for p in g['params']])
+
+
+def _as_before(opt, before):
+    groups, states = _frozen(opt)
+    return groups == before[0] and all(a.keys() == b.keys() and all(torch.equal(a[k], b[k]) for k in a)
+                                       for a, b in zip(states, before[1]))
+
+
+def _changed(sd, i, **kw):
+    """A state dict with entries of state i replaced (None: taken out) and another learning rate."""
+    state = {k: dict(s) for k, s in sd['state'].items()}
+    for name, x in kw.items():
+        if x is None:
+            del state[i][name]
+        else:
+            state[i][name] = x
+    return dict(state=state, param_groups=[dict(g, lr=7.0) for g in sd['param_groups']])
+
+
+@pytest.mark.parametrize('bits', [32, 8])
+def test_a_refused_load_changes_nothing(bits):
+    from paccmann_generator_amd._ffi import PmgError
+    opt, _ = _optimizer(1, state_bits=bits)
+    other, _ = _optimizer(2, state_bits=bits)
+    sd, before = other.state_dict(), _frozen(opt)
+    bad = [_changed(sd, 2, step=None), _changed(sd, 2, exp_avg=None), _changed(sd, 1, exp_avg_sq=None),
+           _changed(sd, 2, exp_avg=sd['state'][2]['exp_avg'][:6]), _changed(sd, 0, step=torch.zeros(2))]
+    if bits == 8:
+        s = sd['state'][1]
+        bad += [_changed(sd, 1, exp_avg_top=s['exp_avg_top'][:1]), _changed(sd, 1, exp_avg_sq_top=None),
+                _changed(sd, 1, exp_avg=s['exp_avg'].to(torch.uint8)), _changed(sd, 1, exp_avg_top=s['exp_avg_top'].double()),
+                _changed(sd, 0, exp_avg=sd['state'][0]['exp_avg'].t().contiguous().t()),      # blocks in another order
+                _changed(_optimizer(3, state_bits=32)[0].state_dict(), 0)]
+    else:
+        bad += [_changed(sd, 2, exp_avg=torch.zeros(7, dtype=torch.int8))]
+    bad.append(_changed(sd, 0))
+    bad[-1]['param_groups'][1]['maximize'] = True
+    for k, wrong in enumerate(bad):
+        with pytest.raises(PmgError):
+            opt.load_state_dict(wrong)
+        assert _as_before(opt, before), k
+    with pytest.raises(ValueError):          # groups of other sizes: the base class's refusal
+        opt.load_state_dict(dict(state=sd['state'], param_groups=sd['param_groups'][:1]))
+    assert _as_before(opt, before)
+    opt.load_state_dict(sd)
+    assert _as_before(opt, _frozen(other)) and not _as_before(opt, before)
+
+
+def test_a_state_in_another_memory_order_loads():
+    opt, ps = _optimizer(1, state_bits=32)
+    sd = opt.state_dict()
+    turned = _changed(sd, 0, exp_avg=sd['state'][0]['exp_avg'].t().contiguous().t())
+    before = opt.state[ps[0]]['exp_avg'].clone()
+    opt.load_state_dict(turned)
+    got = opt.state[ps[0]]['exp_avg']
+    assert torch.equal(got, before) and got.stride() == ps[0].stride() and opt.param_groups[0]['lr'] == 7.0
