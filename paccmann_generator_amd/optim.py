@@ -25,7 +25,8 @@ class AdamW(torch.optim.Optimizer):
 
     Steps are counted on the device, so ``step`` can be captured into a graph once the state exists (after one eager
     step with the same gradients present; else the capture is refused); parameters that always step together share a
-    counter, as in the torch classes a parameter without a gradient keeps its count.  States of the torch classes load."""
+    counter, as in the torch classes a parameter without a gradient keeps its count.  States of the torch classes load, and
+    states of 32 bits load there."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2,
                  decoupled: bool = True, state_bits: int = 32, master_weights: bool = False,
@@ -115,6 +116,17 @@ class AdamW(torch.optim.Optimizer):
                        betas=group['betas'], eps=group['eps'], weight_decay=group['weight_decay'],
                        decoupled=group['decoupled'], exp_avg_top=of('exp_avg_top'), exp_avg_sq_top=of('exp_avg_sq_top'),
                        master=of('master'), grad_norm=norm, max_norm=self.max_grad_norm or 0.0)
+
+    def state_dict(self):
+        """As the torch classes write it: a counter of its own per parameter, fp32 on the host (counters shared by a group
+        would be counted up once per parameter there), so that a state of 32 bits loads into ``torch.optim.Adam`` and
+        ``AdamW``.  Reading the counters synchronises."""
+        out = super().state_dict()
+        counts = {id(s['step']): s['step'] for s in out['state'].values() if 'step' in s}
+        counts = {k: float(x) for k, x in counts.items()}
+        out['state'] = {i: dict(s, step=torch.tensor(counts[id(s['step'])], dtype=torch.float32)) if 'step' in s else s
+                        for i, s in out['state'].items()}
+        return out
 
     def load_state_dict(self, state_dict):
         """States keep their types (the base class would cast them to their parameter's).  A state of 8 bits loads into

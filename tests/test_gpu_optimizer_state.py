@@ -35,3 +35,28 @@ def test_a_copy_steps_like_its_original(gpu, bits, through):
         for p, q in zip(a['params'], b['params']):
             assert p is not q and torch.equal(p, q) and int(again.state[q]['step']) == 3
             assert all(torch.equal(x, again.state[q][n]) for n, x in opt.state[p].items())
+
+
+@pytest.mark.parametrize('foreach', [False, True])
+@pytest.mark.parametrize('decoupled', [False, True])
+def test_torch_goes_on_from_our_checkpoint(gpu, decoupled, foreach):
+    """Three steps here, two there, against five steps here: the classes make the same update up to roundings."""
+    from paccmann_generator_amd import AdamW
+    a, b = _params(1), _params(1)
+    kw = dict(lr=1e-2, weight_decay=0.1)
+    opt, ref = AdamW(a, decoupled=decoupled, **kw), AdamW(b, decoupled=decoupled, **kw)
+    for k in range(3):
+        _step(opt, k)
+        _step(ref, k)
+    theirs = (torch.optim.AdamW if decoupled else torch.optim.Adam)(a, foreach=foreach, **kw)
+    theirs.load_state_dict(opt.state_dict())
+    for g in theirs.param_groups:
+        g['foreach'] = foreach
+    for k in (3, 4):
+        _step(theirs, k)
+        _step(ref, k)
+    assert all(float(theirs.state[p]['step']) == 5 for p in a)
+    for x, y in zip(a, b):
+        # a step moves by at most lr / (1 - 0.9^4) |m| / sqrt(v) < 10 lr, off by up to 32 roundings (moments, root, quotient);
+        # the parameter's own two roundings a step
+        assert float((x - y).detach().abs().max()) <= 2 * (10 * 1e-2 * 32 + 2 * float(y.detach().abs().max())) * 2.0 ** -24

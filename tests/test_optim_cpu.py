@@ -115,3 +115,40 @@ def test_a_state_in_another_memory_order_loads():
     opt.load_state_dict(turned)
     got = opt.state[ps[0]]['exp_avg']
     assert torch.equal(got, before) and got.stride() == ps[0].stride() and opt.param_groups[0]['lr'] == 7.0
+
+
+@pytest.mark.parametrize('foreach', [False, True])
+@pytest.mark.parametrize('decoupled', [False, True])
+def test_states_load_into_the_torch_classes(decoupled, foreach):
+    """One update of torch's class from our checkpoint is the update it makes from its own at that count."""
+    opt, ps = _optimizer(3, state_bits=32, decoupled=decoupled)
+    sd = opt.state_dict()
+    counters = [s['step'] for s in sd['state'].values()]
+    assert len({c.data_ptr() for c in counters}) == len(ps) and all(float(c) == 7 for c in counters)
+    kind = torch.optim.AdamW if decoupled else torch.optim.Adam
+    make = lambda: [p.detach().clone().requires_grad_(True) for p in ps]        # noqa: E731
+    runs = []
+    for own in (True, False):
+        qs = make()
+        theirs = kind([dict(params=qs[:2], lr=1e-2), dict(params=qs[2:], weight_decay=0.5)], foreach=foreach)
+        if own:                                            # a state of torch's own at seven steps
+            for q, p in zip(qs, ps):
+                theirs.state[q] = dict(step=torch.tensor(7.0), exp_avg=opt.state[p]['exp_avg'].to(q.dtype, copy=True),
+                                       exp_avg_sq=opt.state[p]['exp_avg_sq'].to(q.dtype, copy=True))
+            for g, mine in zip(theirs.param_groups, opt.param_groups):
+                g.update(weight_decay=mine['weight_decay'])
+        else:
+            theirs.load_state_dict(copy.deepcopy(sd))
+            for g in theirs.param_groups:
+                g['foreach'] = foreach
+        for _ in range(2):
+            for k, q in enumerate(qs):
+                q.grad = torch.full_like(q, 0.5 + k)
+            theirs.step()
+        assert all(float(theirs.state[q]['step']) == 9 for q in qs)
+        runs.append(qs)
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
+    # the optimizer's own counters are untouched, and its checkpoint comes back into it, counters shared
+    assert all(int(opt.state[p]['step']) == 7 and opt.state[p]['step'].dtype == torch.int64 for p in ps)
+    opt.load_state_dict(sd)
+    assert opt.state[ps[0]]['step'] is opt.state[ps[1]]['step'] and int(opt.state[ps[0]]['step']) == 7
