@@ -75,12 +75,18 @@ def embedding(weight: Tensor, tokens: Tensor, scale: float = 1.0, padding_idx: O
               trusted_tokens: bool = False) -> Tensor:
     """``scale * weight[tokens]``: [..., E] in the type of the table [V, E] (fp32, bf16, fp16), differentiable w.r.t.
     the table.  The rows of its gradient are sums in fp32 over a token's positions, in one order whatever the launch
-    (no atomics); ``padding_idx`` gets a zero row.  ``tokens``: int64 or int32 of any shape.  ``trusted_tokens`` skips
-    the id range check, which synchronises (captured graphs need it skipped): an id out of range then gives NaN."""
+    (no atomics); ``padding_idx`` gets a zero row, a negative one counts from the table's end.  ``tokens``: int64 or int32
+    of any shape.  ``trusted_tokens`` skips the id range check, which synchronises (captured graphs need it skipped): an id
+    out of range then gives NaN."""
+    if padding_idx is not None:
+        padding_idx, V = int(padding_idx), weight.shape[0]
+        if not -V <= padding_idx < V:
+            raise _ffi.PmgError(f'pmg::embedding: padding_idx must lie in [{-V}, {V}), got {padding_idx}')
+        padding_idx %= V
     _need_cuda(weight, tokens)
     if not trusted_tokens:
         check_ids(tokens, weight.shape[0], 'token ids')
-    return _ops.embedding.default(weight, tokens, float(scale), -1 if padding_idx is None else int(padding_idx))
+    return _ops.embedding.default(weight, tokens, float(scale), -1 if padding_idx is None else padding_idx)
 
 
 # --------------------------------------------------------------------------- linear cross entropy

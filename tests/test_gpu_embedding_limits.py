@@ -1,0 +1,27 @@
+"""pmg::embedding at the ends of what its arguments allow: padding ids counted from either end of the table."""
+import pytest
+import torch
+
+from oracle import lm
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize('V', [1, 9, 3000])
+def test_padding_counted_from_either_end(gpu, V):
+    from paccmann_generator_amd import _ffi, ops
+    torch.manual_seed(V)
+    w = torch.randn(V, 12, device='cuda', requires_grad=True)
+    ids = torch.cat([torch.arange(V), torch.randint(0, V, (50,))]).cuda()
+    slope = torch.randn(len(ids), 12, device='cuda')
+    for pad in {-V, -1, -(V // 2) - 1, V - 1, 0}:
+        out = ops.embedding(w, ids, padding_idx=pad)
+        assert torch.equal(out, w[ids])                      # the padding row is looked up like any other
+        got, = torch.autograd.grad(out, w, slope)
+        want, size, count = lm.embedding_grad(slope.cpu(), ids.cpu(), V, 1.0, pad % V)
+        # a token's positions are added in fp32 (dropping the padding's positions moves where the sums are cut)
+        assert bool(((got.cpu().double() - want).abs() <= size * (count.unsqueeze(1) + 2) * 2.0 ** -24).all()), pad
+        assert not got[pad].any() and (V == 1 or bool(got.any(1).sum() == V - 1)), pad
+    for pad in (V, -V - 1):
+        with pytest.raises(_ffi.PmgError, match='padding_idx'):
+            ops.embedding(w, ids, padding_idx=pad)
