@@ -463,9 +463,10 @@ extern "C" int pmg_grad_clip_check(void* const* grads, const int64_t* numel, con
   if (n == 0) return PMG_OK;
   Range* r = new (std::nothrow) Range[n];
   if (!r) return PMG_E_ARG;
-  for (int i = 0; i < n; ++i)
-    r[i] = Range{(uintptr_t)grads[i], (uintptr_t)grads[i] + (size_t)numel[i] * pmg_elem_bytes(dtype[i]), numel[i] > 0};
-  const int ov = check_disjoint(r, n);
+  int nr = 0;
+  for (int i = 0; i < n; ++i)  // an empty tensor has no elements to share, wherever it points
+    if (numel[i] > 0) r[nr++] = Range{(uintptr_t)grads[i], (uintptr_t)grads[i] + (size_t)numel[i] * pmg_elem_bytes(dtype[i]), 1};
+  const int ov = check_disjoint(r, nr);
   delete[] r;
   return ov;
 }
