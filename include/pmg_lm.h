@@ -52,7 +52,7 @@ int pmg_embedding_bwd(const void* grad, int64_t ld_grad, const void* ids, int id
 #define PMG_REDUCE_MEAN 2 /* over the rows with a target; 0 without any */
 
 /* With logits l = logit_scale (hidden weight^T + bias), kept only where `logits` is given:
- *   lse[n]  = log sum_v exp l[n,v]
+ *   lse[n]  = log sum_v exp l[n,v]                     (+inf with a logit of +inf, -inf with nothing but -inf)
  *   nll[n]  = row_weight[n] (lse[n] - l[n,targets[n]]), 0 where targets[n] == ignore_index
  *   loss    = nll [N] (PMG_REDUCE_NONE), its sum, or its sum / count; count[0] = rows with a target
  * and, from grad_loss ([N] or [1], as loss) and grad_lse ([N]; either may be NULL: no slope), the

@@ -57,6 +57,14 @@ constexpr int LIST_SLACK = 256;  // entries behind the list of rows that a tile 
 // a value in memory that is the same for the whole launch, into a scalar register
 __device__ __forceinline__ int uniform_of(const int* p) { return *(const __attribute__((address_space(4))) int*)p; }
 
+// Sums of exponentials are held below a maximum, (top, sum).  A top of -inf (nothing, or NaN) or +inf has no difference to
+// itself: such a sum is held below 0, and one whose maximum stays is not rescaled.  A NaN logit is in no maximum and stays
+// in the sum; below -inf the sum is 0 or NaN.
+__device__ __forceinline__ float below(float top) { return fabsf(top) == __builtin_inff() ? 0.0f : top; }
+template <typename T> __device__ __forceinline__ float rescaled(float2 p, float top) {
+  return p.x == top ? p.y : p.y * exp_of<T>(p.x - top);
+}
+
 // ------------------------------------------------------------------------------------------ arguments
 struct LogitArgs {
   const void *W, *X, *bias;
@@ -185,12 +193,12 @@ __global__ __launch_bounds__(THREADS_OF<S>) void lce_logits_kernel(const LogitAr
         for (int e = 0; e < 4; ++e) top = fmaxf(top, acc[i][j][e]);
       top = fmaxf(top, __shfl_xor(top, 16, 64));
       top = fmaxf(top, __shfl_xor(top, 32, 64));
-      const float base = top == -__builtin_inff() ? 0.0f : top;  // nothing but -inf: the sum is 0
+      const float base = below(top);
       float sum = 0.0f;
 #pragma unroll
       for (int i = 0; i < MI; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sum += exp_of<T>(acc[i][j][e] - base);  // a NaN logit makes a NaN sum
+        for (int e = 0; e < 4; ++e) sum += exp_of<T>(acc[i][j][e] - base);
       sum += __shfl_xor(sum, 16, 64);
       sum += __shfl_xor(sum, 32, 64);
       if (g == 0) red[wm * BN + wn * (BN / WN) + j * 16 + col] = make_float2(top, sum);
@@ -211,10 +219,7 @@ __global__ __launch_bounds__(THREADS_OF<S>) void lce_logits_kernel(const LogitAr
 #pragma unroll
       for (int w = 0; w < WM; ++w) top = fmaxf(top, red[w * BN + c].x);
 #pragma unroll
-      for (int w = 0; w < WM; ++w) {
-        const float2 r = red[w * BN + c];
-        sum += r.x == -__builtin_inff() ? r.y : r.y * exp_of<T>(r.x - top);
-      }
+      for (int w = 0; w < WM; ++w) sum += rescaled<T>(red[w * BN + c], top);
       if (n0 + c < a.N) a.part[(int64_t)tm * a.N + n0 + c] = make_float2(top, sum);
     }
   } else if constexpr (BACKWARD) {
@@ -573,8 +578,7 @@ __global__ __launch_bounds__(1024) void lce_rows_kernel(const RowArgs a) {
     for (int t = grp; t < a.tiles; t += groups) {
       const float2 p = a.part[(int64_t)t * a.N + n];
       const float m = fmaxf(top, p.x);
-      // below -inf there is nothing to rescale (and inf - inf would be NaN); a NaN sum stays
-      sum = (top == -__builtin_inff() ? sum : sum * expf(top - m)) + (p.x == -__builtin_inff() ? p.y : p.y * expf(p.x - m));
+      sum = rescaled<float>(make_float2(top, sum), m) + rescaled<float>(p, m);
       top = m;
     }
   }
@@ -584,8 +588,7 @@ __global__ __launch_bounds__(1024) void lce_rows_kernel(const RowArgs a) {
     if (grp < half) {
       const float2 p = red[threadIdx.x], q = red[threadIdx.x + half * a.rows];
       const float m = fmaxf(p.x, q.x);
-      const float s = (p.x == -__builtin_inff() ? p.y : p.y * expf(p.x - m)) + (q.x == -__builtin_inff() ? q.y : q.y * expf(q.x - m));
-      red[threadIdx.x] = make_float2(m, s);
+      red[threadIdx.x] = make_float2(m, rescaled<float>(p, m) + rescaled<float>(q, m));
     }
   }
   float nll = 0.0f;
@@ -648,17 +651,16 @@ template <typename T> __global__ __launch_bounds__(1024) void lce_split_rows_ker
       if (v + e == t) hit[row] = x[e];
     }
     if (b.kept) *(f32x4*)(b.kept + n * b.ldk + v) = x;
-    const float m = fmaxf(top, most);
+    const float m = fmaxf(top, most), base = below(m);
     float s = 0.0f;
-    // below -inf there is nothing to rescale; a NaN logit is not in the maximum and stays in the sum
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s += x[e] == -__builtin_inff() ? 0.0f : expf(m == -__builtin_inff() ? x[e] : x[e] - m);
-    sum = (top == -__builtin_inff() ? sum : sum * expf(top - m)) + s;
+    for (int e = 0; e < 4; ++e) s += expf(x[e] - base);
+    sum = rescaled<float>(make_float2(top, sum), m) + s;
     top = m;
   }
   const auto join = [](float2 p, float2 q) {
     const float m = fmaxf(p.x, q.x);
-    return make_float2(m, (p.x == -__builtin_inff() ? p.y : p.y * expf(p.x - m)) + (q.x == -__builtin_inff() ? q.y : q.y * expf(q.x - m)));
+    return make_float2(m, rescaled<float>(p, m) + rescaled<float>(q, m));
   };
   float2 p = make_float2(top, sum);
   for (int o = 32; o > 0; o >>= 1) p = join(p, make_float2(__shfl_xor(p.x, o, 64), __shfl_xor(p.y, o, 64)));

@@ -1,0 +1,69 @@
+"""pmg::linear_cross_entropy at the ends of what its arguments allow: infinite logits."""
+import math
+
+import pytest
+import torch
+
+from oracle import lm
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+TYPES = [torch.float32, torch.bfloat16]
+
+
+def _data(N, V, H, dtype, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(N, H, generator=g).to(dtype)
+    w = (torch.randn(V, H, generator=g) * 2 / math.sqrt(H)).to(dtype)
+    return x, w, (torch.randn(V, generator=g) * 0.3).to(dtype), torch.randint(0, V, (N,), generator=g)
+
+
+# one wave's tile, several waves and tiles, few tokens over many words, a hidden size that is split, kept logits
+SIZES = [(20, 30, 16), (300, 700, 64), (5, 5000, 96), (20, 90, 2048), (3000, 60, 512)]
+
+
+@pytest.mark.parametrize('dtype', TYPES, ids=str)
+@pytest.mark.parametrize('N,V,H', SIZES)
+def test_infinite_logits(gpu, dtype, N, V, H):
+    """lse is +inf where a logit is, NaN where one is NaN, and untouched in the other rows; the loss follows from it."""
+    from paccmann_generator_amd import ops
+    x, w, b, t = _data(N, V, H, dtype, seed=N)
+    x[:, 0] = 0
+    w[:, 0] = 0
+    up = [7, V - 2 if V % 3 == 1 else V - 1]        # no multiples of 3: those are masked out below
+    w[up, 0] = 16.0
+    hot, nan = [3, N - 2], 4
+    x[hot, 0] = 3e38                    # 16 x 3e38 leaves fp32 in the columns `up`, and no other
+    x[nan, 0], x[nan, 1] = 3e38, float('nan')
+    t[3], t[N - 2] = 7, 5
+    rest = torch.ones(N, dtype=torch.bool)
+    rest[hot + [nan]] = False
+    for bias in (b, b.masked_fill(torch.arange(V) % 3 == 0, -float('inf'))):      # and with others masked out
+        t = torch.where(t % 3 == 0, (t + 1) % V, t) if bias is not b else t
+        t = torch.where(t % 3 == 0, torch.ones_like(t), t) if bias is not b else t
+        e = lm.linear_ce(x[rest], w, t[rest], bias, None, 1.0, 'none', -100)
+        size = lm.linear_ce(x[rest], w, t[rest], b, None, 1.0, 'none', -100)['size']
+        tol = (H + 16) * U * size + 8 * U
+        for train in (False, True):
+            z = [v.cuda().requires_grad_(train) for v in (x, w, bias)]
+            loss, lse = ops.linear_cross_entropy(z[0], z[1], t.cuda(), bias=z[2], reduction='none')
+            lse, loss = lse.detach().cpu(), loss.detach().cpu()
+            assert bool((lse[hot] == float('inf')).all()) and bool(lse[nan].isnan())
+            for n in hot:                       # inf - inf, or inf - finite
+                assert bool(loss[n].isnan()) if int(t[n]) in up else float(loss[n]) == float('inf')
+            assert bool(((lse[rest].double() - e['lse']).abs() <= tol + 2 * U * e['lse'].abs()).all())
+            assert bool(((loss[rest].double() - e['loss']).abs() <= 2 * tol + 4 * U * (e['lse'].abs() + e['loss'].abs())).all())
+    # a bias of +inf is in every row
+    b2 = b.clone()
+    b2[V // 2] = float('inf')
+    _, lse = ops.linear_cross_entropy(x.cuda(), w.cuda(), t.cuda(), bias=b2.cuda())
+    keep = torch.arange(N) != nan
+    assert bool((lse.cpu()[keep] == float('inf')).all()) and bool(lse[nan].isnan())
+    b2[V // 3] = float('nan')
+    assert bool(ops.linear_cross_entropy(x.cuda(), w.cuda(), t.cuda(), bias=b2.cuda())[1].isnan().all())
+    # ignored, such rows leave the loss and the gradients alone
+    t[hot + [nan]] = -100
+    z = [v.cuda().requires_grad_(True) for v in (x, w, b)]
+    loss, _ = ops.linear_cross_entropy(z[0], z[1], t.cuda(), bias=z[2])
+    g = torch.autograd.grad(loss, z)
+    assert bool(loss.isfinite()) and all(bool(v.isfinite().all()) for v in g) and not g[0][hot + [nan]].any()
