@@ -87,8 +87,11 @@ typedef struct pmg_linear_ce {
 } pmg_linear_ce;
 
 /* Bytes of scratch of one direction, for a call with these sizes, strides, operands (their alignment counts)
- * and logits.  It does not grow with N x V: the backward keeps the slopes of a piece of the vocabulary at a
- * time. */
+ * and logits.  It does not grow with N x V, but with the larger of N and V:
+ *   forward   statistics of tiles, at most 256 MB or 128 V bytes; 4 N
+ *   backward  slopes of a piece of the vocabulary, about 256 MB or 256 N elements; 25 N; where there are several
+ *             pieces, fp32 sums of grad_hidden, 4 N H; parts of sums that are split over the chip, some 100 MB
+ * and copies of hidden or weight where their rows do not begin and end at multiples of 16 bytes. */
 int pmg_linear_ce_workspace(const pmg_linear_ce* a, int backward, size_t* out);
 int pmg_linear_ce_fwd(const pmg_linear_ce* a, void* ws, pmg_stream stream);
 int pmg_linear_ce_bwd(const pmg_linear_ce* a, void* ws, pmg_stream stream);

@@ -891,7 +891,8 @@ struct Problem {
   size_t eb;
 };
 
-// Vocabulary entries of a backward piece: dl of a piece takes about 256 MB.  8192 tokens over 128000 (2 GB in one piece):
+// Vocabulary entries of a backward piece: dl of a piece takes about 256 MB, or 256 entries where those are more (from 524288
+// tokens in bf16).  8192 tokens over 128000 (2 GB in one piece):
 // 27.4 ms a step with 256 MB, 27.2 with 128, 27.7 with 1024; 4095 over 32001 (250 MB): 1.80 ms, 1.90 in pieces of 128 MB.
 constexpr int64_t PIECE_BYTES = 256 << 20;
 int64_t piece_of(const Problem& p) {
@@ -931,9 +932,13 @@ int rows_of(int64_t N, int64_t tiles) {
 // Few tiles (a small batch over a small vocabulary) are bound by the latency of their stages, one after the other: the
 // hidden size is split over the chip, into 16 parts at most of four stages at least (logits and rows; fp32 20 tokens of
 // 4096 over 100: 148 us whole, 18 in 16 parts; 20 of 512 over 60: 27 whole, 13 in four parts).
+// The statistics of the tiles (8 bytes for a token and a tile's words) are held for a block of tokens at a time, 256 MB of
+// them: 524288 tokens over 128000 would leave 2.1 GB.  A block has 1024 tokens at least (rows a workgroup joins, and some
+// tiles of tokens; then it is V that is long, and the statistics take 128 bytes a word at most).
+constexpr int64_t PART_BYTES = 256 << 20;
 struct FwdPlan {
   int s, splits, rows;   // tile shape; rows a workgroup joins
-  int64_t groups;        // of rows
+  int64_t groups, block; // of rows; tokens at a time
 };
 
 FwdPlan fwd_plan(const Problem& p) {
@@ -945,6 +950,9 @@ FwdPlan fwd_plan(const Problem& p) {
   if (f.splits < 2 || f.s == S256 || f.s == SM64) f.splits = 1;
   f.rows = f.splits > 1 ? (p.V <= 256 ? 16 : p.V <= 1024 ? 4 : 1) : rows_of(p.N, div_up(p.V, SHAPES[f.s].BM));
   f.groups = div_up(p.N, f.rows);
+  f.block = p.N;
+  const int64_t fit = PART_BYTES / ((int64_t)sizeof(float2) * div_up(p.V, SHAPES[f.s].BM)), most_tokens = fit < 1024 ? 1024 : fit / 1024 * 1024;
+  if (f.splits == 1 && p.N > most_tokens) f.block = up(div_up(p.N, div_up(p.N, most_tokens)), 1024);
   return f;
 }
 
@@ -954,8 +962,8 @@ Layout fwd_layout(const Problem& p) {
   L.xp = take(p.pack_x ? (size_t)p.N * p.Hp * p.eb : 0);
   L.wp = take(p.pack_w ? (size_t)p.V * p.Hp * p.eb : 0);
   const FwdPlan f = fwd_plan(p);
-  L.part = take(f.splits > 1 ? (size_t)f.splits * p.N * up(p.V, 4) * 4 : (size_t)div_up(p.V, SHAPES[f.s].BM) * p.N * sizeof(float2));
-  L.at = take((size_t)p.N * 4);
+  L.part = take(f.splits > 1 ? (size_t)f.splits * p.N * up(p.V, 4) * 4 : (size_t)div_up(p.V, SHAPES[f.s].BM) * f.block * sizeof(float2));
+  L.at = take((size_t)f.block * 4);
   L.sums = take((size_t)f.groups * sizeof(LossPart));
   L.bytes = take.at + 256;
   return L;
@@ -1141,33 +1149,42 @@ template <typename T> int forward(const pmg_linear_ce* a, const Problem& p, char
   const FwdPlan f = fwd_plan(p);
   l.splits = f.splits;
   l.sums = (float*)(ws + L.part);
-  if (const int rc = f.splits > 1 ? logits<T, SPLIT>(f.s, l, st) : logits<T, FORWARD>(f.s, l, st)) return rc;
   RowArgs r = {};
   r.part = l.part;
   r.at_target = l.at_target;
   r.tiles = (int)div_up(p.V, SHAPES[f.s].BM);
-  r.N = p.N; r.V = p.V;
-  r.targets = a->targets; r.id_bits = a->id_bits; r.ignore = a->ignore_index;
-  r.weight = a->row_weight;
-  r.lse = a->lse;
+  r.V = p.V;
+  r.id_bits = a->id_bits; r.ignore = a->ignore_index;
   const bool none = a->reduction == PMG_REDUCE_NONE;
-  r.nll = none ? a->loss : nullptr;
-  r.sums = none ? nullptr : (LossPart*)(ws + L.sums);
+  LossPart* sums = (LossPart*)(ws + L.sums);
   r.rows = f.rows;
-  const int groups = (int)f.groups;
   r.mean = a->reduction == PMG_REDUCE_MEAN;
-  if (groups == 1 && !none) {
+  if (f.groups == 1 && !none) {
     r.loss = a->loss;
     r.count = a->count;
   }
-  if (f.splits > 1) {
-    const SplitArgs b = {l.sums, f.splits, l.ldk, a->bias, a->logit_scale, a->logits};
-    hipLaunchKernelGGL(lce_split_rows_kernel<T>, dim3((unsigned)groups), dim3(1024), 0, st, b, r);
-  } else {
-    hipLaunchKernelGGL(lce_rows_kernel, dim3((unsigned)groups), dim3(1024), 0, st, r);
+  const char *X = (const char*)l.X, *targets = (const char*)a->targets;
+  for (int64_t n0 = 0; n0 < p.N; n0 += f.block) {
+    const int64_t n = n0 + f.block < p.N ? f.block : p.N - n0;
+    l.N = r.N = n;
+    l.X = X + n0 * l.ldx * (int64_t)p.eb;
+    l.targets = r.targets = targets + n0 * (a->id_bits / 8);
+    l.kept = a->logits ? a->logits + n0 * l.ldk : nullptr;
+    if (const int rc = f.splits > 1 ? logits<T, SPLIT>(f.s, l, st) : logits<T, FORWARD>(f.s, l, st)) return rc;
+    r.weight = a->row_weight ? a->row_weight + n0 : nullptr;
+    r.lse = a->lse + n0;
+    r.nll = none ? a->loss + n0 : nullptr;
+    r.sums = none ? nullptr : sums + n0 / f.rows;
+    const dim3 groups((unsigned)div_up(n, f.rows));
+    if (f.splits > 1) {
+      const SplitArgs b = {l.sums, f.splits, l.ldk, a->bias, a->logit_scale, l.kept};
+      hipLaunchKernelGGL(lce_split_rows_kernel<T>, groups, dim3(1024), 0, st, b, r);
+    } else {
+      hipLaunchKernelGGL(lce_rows_kernel, groups, dim3(1024), 0, st, r);
+    }
   }
-  if (!none && groups > 1)
-    hipLaunchKernelGGL(lce_loss_kernel, dim3(1), dim3(1024), 0, st, r.sums, groups, r.mean, a->loss, a->count);
+  if (!none && f.groups > 1)
+    hipLaunchKernelGGL(lce_loss_kernel, dim3(1), dim3(1024), 0, st, sums, (int)f.groups, r.mean, a->loss, a->count);
   return (int)hipGetLastError();
 }
 

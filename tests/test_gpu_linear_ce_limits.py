@@ -67,3 +67,68 @@ def test_infinite_logits(gpu, dtype, N, V, H):
     loss, _ = ops.linear_cross_entropy(z[0], z[1], t.cuda(), bias=z[2])
     g = torch.autograd.grad(loss, z)
     assert bool(loss.isfinite()) and all(bool(v.isfinite().all()) for v in g) and not g[0][hot + [nan]].any()
+
+
+def _in_64_bits(x, w, b, t, step):
+    """(lse, logit of the target, largest sum of magnitudes) of every row, a block of rows at a time, on the GPU."""
+    out = []
+    wd, bd = w.double(), b.double()
+    for n in range(0, len(x), step):
+        xd = x[n:n + step].double()
+        logits = torch.mm(xd, wd.t().contiguous()).add_(bd)
+        size = xd.abs().sum(1) * wd.abs().max() + bd.abs().max()
+        out.append((logits.logsumexp(1), logits.gather(1, t[n:n + step].clamp(min=0).unsqueeze(1)).squeeze(1), size))
+    return [torch.cat(c) for c in zip(*out)]
+
+
+@pytest.mark.parametrize('dtype', TYPES, ids=str)
+def test_tokens_in_blocks(gpu, dtype):
+    """More statistics of tiles than the scratch holds at a time: the last block is shorter, rows and sums run through."""
+    from paccmann_generator_amd import ops
+    N, V, H = 70001, 128000, 16
+    x, w, b, t = _data(N, V, H, dtype, seed=1)
+    t[torch.rand(N, generator=torch.Generator().manual_seed(2)) < 0.3] = -100
+    r = torch.rand(N, generator=torch.Generator().manual_seed(3)) - 0.3
+    x, w, b, t, r = (v.cuda() for v in (x, w, b, t, r))
+    lse, hit, size = _in_64_bits(x, w, b, t, 8192)
+    used = t != -100
+    tol = (H + 16) * U * size + 8 * U
+    nll = torch.where(used, (lse - hit) * r, torch.zeros_like(lse))
+    off = (2 * tol + 4 * U * lse.abs()) * r.abs() * used
+    for ids in (t, t.int()):
+        got, l = ops.linear_cross_entropy(x, w, ids, bias=b, row_weight=r, reduction='none')
+        assert bool(((l.double() - lse).abs() <= tol + 2 * U * lse.abs()).all())
+        assert bool(((got.double() - nll).abs() <= off + 2 * U * nll.abs()).all())
+        total, l2 = ops.linear_cross_entropy(x, w, ids, bias=b, row_weight=r, reduction='sum')
+        mean, l3 = ops.linear_cross_entropy(x, w, ids, bias=b, row_weight=r, reduction='mean')
+        assert torch.equal(l, l2) and torch.equal(l, l3)
+        assert abs(float(total) - float(nll.sum())) <= float(off.sum()) + 2 * U * abs(float(nll.sum()))
+        # the same sum, divided: rounded once more each
+        assert abs(float(mean) - float(total) / int(used.sum())) <= 2 * U * abs(float(mean))
+
+
+def test_tokens_in_blocks_with_kept_logits(gpu):
+    """Few words, so that a block is 33.5 million tokens; training keeps the logits of both blocks."""
+    from paccmann_generator_amd import ops
+    N, V, H = (1 << 25) + 5003, 2, 8
+    g = torch.Generator(device='cuda').manual_seed(4)
+    x = torch.randn(N, H, device='cuda', generator=g)
+    w, b = torch.randn(V, H, device='cuda', generator=g), torch.randn(V, device='cuda', generator=g)
+    t = torch.randint(0, V, (N,), device='cuda', generator=g)
+    x.requires_grad_(True)
+    loss, lse = ops.linear_cross_entropy(x, w, t, bias=b, trusted_tokens=True)
+    dx, = torch.autograd.grad(loss, x)
+    xd = x.detach()
+    want, hit, size = _in_64_bits(xd, w, b, t, 1 << 24)
+    tol = (H + 16) * U * size + 8 * U
+    assert bool(((lse.double() - want).abs() <= tol + 2 * U * want.abs()).all())
+    nll = want - hit
+    assert abs(float(loss) - float(nll.mean())) <= float((2 * tol + 4 * U * want.abs()).mean()) + 2 * U * float(nll.mean())
+    # dx = (p - onehot) W / N: the exponential's error, relative; a product, two sums and a factor
+    rel = 4 * float(tol.max()) + 32 * U
+    wd = w.double()
+    for n in range(0, N, 1 << 24):
+        p = (torch.mm(xd[n:n + (1 << 24)].double(), wd.t().contiguous()) + b.double() - want[n:n + (1 << 24)].unsqueeze(1)).exp()
+        one = torch.nn.functional.one_hot(t[n:n + (1 << 24)], V)
+        exact, most = torch.mm(p - one, wd) / N, torch.mm(p + one, wd.abs()) / N
+        assert bool(((dx[n:n + (1 << 24)].double() - exact).abs() <= most * rel).all())

@@ -22,3 +22,34 @@ def test_empty_tensors_overlap_nothing():
         bad = rc(many + [FAKE, FAKE + 252], [0] * 200 + [64, 8])
         assert bad < 0 and b'overlap' in _ffi.lib.pmg_strerror(bad)
     assert rc([FAKE, FAKE], [0, 0]) == 0 and rc([None, FAKE], [0, 4]) == 0
+
+
+def test_cross_entropy_scratch_does_not_grow_with_tokens_times_words():
+    """Tokens held, words doubled, and the other way round: what the header says, and no more."""
+    from paccmann_generator_amd import _ffi
+    size, MB = C.c_size_t(0), 1 << 20
+
+    def need(N, V, H, dtype, backward):
+        a = _ffi.PmgLinearCe()
+        for name, x in dict(N=N, V=V, H=H, dtype=dtype, id_bits=64, reduction=2, logit_scale=1.0, ld_hidden=H, ld_weight=H,
+                            hidden=FAKE, weight=FAKE, targets=FAKE).items():
+            setattr(a, name, x)
+        assert _ffi.lib.pmg_linear_ce_workspace(C.byref(a), backward, C.byref(size)) == 0
+        return size.value
+
+    for dtype, eb in ((0, 4), (1, 2)):
+        for H in (64, 1024, 4096):
+            for N in (1, 63, 1000, 8192, 65536, 524288, 4 << 20):
+                words = [2 << k for k in range(24)]
+                f = [need(N, V, H, dtype, 0) for V in words]
+                b = [need(N, V, H, dtype, 1) for V in words]
+                for V, x, y in zip(words, f, b):
+                    assert x <= max(256 * MB, 128 * V) + 4 * N + 32 * MB, (N, V, H)
+                    # slopes and their bias sums (a sixteenth of an fp32 row of them), rows, sums of grad_hidden, split sums
+                    slopes = max(256 * MB, 256 * N * eb) * 1.2 + 64 * MB
+                    assert y <= slopes * 1.07 + 25 * N + 4 * N * H + 160 * MB, (N, V, H)
+                    # far below a byte a logit where there are many
+                    assert N * V < 4e9 or max(x, y) < N * V + 4 * N * H + 256 * MB, (N, V, H)
+                many = [k for k, V in enumerate(words[:-1]) if V >= 1 << 17 and N >= 65536 and 128 * 2 * V < 256 * MB]
+                for k in many:          # twice the words, no more scratch
+                    assert f[k + 1] <= f[k] * 1.01 + MB and b[k + 1] <= b[k] * 1.15 + MB, (N, words[k], H)
