@@ -719,10 +719,12 @@ struct SlopeArgs {
   uint8_t* used;         // [N]
 };
 
-// What all rows have in common, without the logits' scale; 1 where that is 0 or not finite.
+// What all rows have in common, without the logits' scale; 1 where that is 0 or not finite, and where it is so far from 1 that
+// slopes of the log-sum-exps, which are divided by it, could leave fp32 (a loss of weight 1e-38 beside them, say).
 __device__ __forceinline__ float common_of(const SlopeArgs& a) {
   if (a.per_row || !a.g_loss) return 1.0f;
   const float g = a.mean ? a.g_loss[0] / a.count[0] : a.g_loss[0];
+  if (a.g_lse && !(fabsf(g) >= 0x1p-60f && fabsf(g) <= 0x1p60f)) return 1.0f;
   return g != 0.0f && fabsf(g) < __builtin_inff() ? g : 1.0f;
 }
 

@@ -132,3 +132,27 @@ def test_tokens_in_blocks_with_kept_logits(gpu):
         one = torch.nn.functional.one_hot(t[n:n + (1 << 24)], V)
         exact, most = torch.mm(p - one, wd) / N, torch.mm(p + one, wd.abs()) / N
         assert bool(((dx[n:n + (1 << 24)].double() - exact).abs() <= most * rel).all())
+
+
+@pytest.mark.parametrize('dtype', TYPES, ids=str)
+@pytest.mark.parametrize('weight', [1e-38, 1e-30, 1e-12, 1e12, 1e30])
+def test_losses_of_any_weight_beside_the_log_sum_exp(gpu, dtype, weight):
+    """weight * loss + sum(z lse): the gradients are sums of both, whichever is the smaller by far.  Ignored rows have the
+    slope of the log-sum-exp alone."""
+    from paccmann_generator_amd import ops
+    N, V, H = 40, 90, 48
+    x, w, b, t = _data(N, V, H, dtype, seed=5)
+    t[:10] = -100
+    z = torch.randn(N, generator=torch.Generator().manual_seed(6))
+    for reduction in ('mean', 'sum'):
+        leaves = [v.cuda().requires_grad_(True) for v in (x, w, b)]
+        loss, lse = ops.linear_cross_entropy(leaves[0], leaves[1], t.cuda(), bias=leaves[2], reduction=reduction)
+        got = torch.autograd.grad((loss, lse), leaves, (torch.tensor(weight, device='cuda'), z.cuda()))
+        grads = lm.linear_ce_grads(x, w, t, b, None, 1.0, reduction, -100, torch.tensor(weight, dtype=torch.float64), z)
+        size = lm.linear_ce(x, w, t, b)['size']
+        f = torch.finfo(dtype)
+        rel = 4 * ((H + 16) * U * float(size.max()) + 8 * U) + 16 * U + (0 if dtype == torch.float32 else f.eps / 2)
+        for name, length, g in zip('xwb', (V, N, N), got):
+            exact, mag = grads[name], grads['|' + name + '|']
+            bound = mag * (rel + (length + 8) * U) + exact.abs() * f.eps / 2 * 1.01
+            assert bool(((g.cpu().double() - exact).abs() <= bound + 1e-30).all()), (name, reduction)
