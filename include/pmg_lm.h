@@ -41,7 +41,7 @@ int pmg_embedding_bwd_workspace(int64_t N, int64_t V, int64_t E, int dtype, size
 /* grad_weight[v] = scale * (sum of grad[n] over the n with ids[n] == v), summed in fp32, rounded once; zero
  * for tokens that do not occur and for padding_idx (-1: none).  Every row is written; ids outside [0,V) add
  * nothing.
- *   grad [N,E] of `dtype`, rows ld_grad apart; grad_weight [V,E] contiguous. */
+ *   grad [N,E] of `dtype`, rows ld_grad apart; grad_weight [V,E] contiguous; V below 2^30. */
 int pmg_embedding_bwd(const void* grad, int64_t ld_grad, const void* ids, int id_bits, int64_t N, int64_t V, int64_t E,
                       int dtype, float scale, int64_t padding_idx, void* grad_weight, void* ws, pmg_stream stream);
 

@@ -242,6 +242,7 @@ struct ReduceArgs {
   int64_t chunks, reduce_blocks;
   const uint32_t *keys, *pos;
   float* part;               // [chunks][2][E]: [0] of the run that began earlier, [1] of the run that goes on
+  int64_t join_from;         // the first chunk of a launch that joins
 };
 
 // WHOLE: rows of 16 bytes or more; the last 16 bytes of a row that is no multiple of them overlap those before (both
@@ -362,7 +363,7 @@ template <typename T, bool WHOLE>
 __global__ __launch_bounds__(JOIN_THREADS) void embed_join_kernel(const ReduceArgs a, T* __restrict__ dW) {
   constexpr int VEC = pmg_vec16<T>::N;
   __shared__ float sum[JOIN_THREADS * VEC];
-  const int64_t ch = blockIdx.x, lo = ch * a.chunk, hi = lo + a.chunk;
+  const int64_t ch = a.join_from + blockIdx.x, lo = ch * a.chunk, hi = lo + a.chunk;
   if (hi >= a.N) return;
   const uint32_t cur = a.keys[hi];
   if (cur >= (uint32_t)a.V || a.keys[hi - 1] != cur) return;
@@ -536,24 +537,27 @@ int bwd(const void* g, int64_t ldg, const void* ids, int id_bits, int64_t N, int
   const BwdLayout L = bwd_layout(N, E, dtype);
   const int tpr = L.tpr;
   const int64_t cols = (E + (int64_t)tpr * pmg_vec16<T>::N - 1) / ((int64_t)tpr * pmg_vec16<T>::N);
-  if (cols > 65535) return PMG_E_ARG;
+  const int rpw = THREADS / tpr;
+  const int64_t reduce_blocks = (L.chunks + rpw - 1) / rpw, blocks = reduce_blocks + (V + FILL_ROWS - 1) / FILL_ROWS;
+  if (cols > 65535 || blocks >= ((int64_t)1 << 32) / THREADS) return PMG_E_ARG;
   int at = 0;
   if (N > 0) at = id_bits == 64 ? sort_ids((const int64_t*)ids, N, V, pad, L, ws, st) : sort_ids((const int32_t*)ids, N, V, pad, L, ws, st);
   ReduceArgs a;
   a.N = N; a.V = V; a.E = E; a.ldg = ldg; a.scale = scale; a.tpr = tpr; a.chunk = L.chunk; a.chunks = L.chunks;
-  const int rpw = THREADS / tpr;
-  a.reduce_blocks = (L.chunks + rpw - 1) / rpw;
+  a.reduce_blocks = reduce_blocks;
   a.keys = (const uint32_t*)(ws + L.keys[at]);
   a.pos = (const uint32_t*)(ws + L.pos[at]);
   a.part = (float*)(ws + L.part);
-  const int64_t blocks = a.reduce_blocks + (V + FILL_ROWS - 1) / FILL_ROWS;
-  const dim3 grid((unsigned)blocks, (unsigned)cols), joins((unsigned)L.chunks, (unsigned)cols);
-  if (E >= pmg_vec16<T>::N) {
-    hipLaunchKernelGGL((embed_reduce_kernel<T, true>), grid, dim3(THREADS), 0, st, a, (const T*)g, (T*)dW);
-    if (L.chunks > 1) hipLaunchKernelGGL((embed_join_kernel<T, true>), joins, dim3(JOIN_THREADS), 0, st, a, (T*)dW);
-  } else {
-    hipLaunchKernelGGL((embed_reduce_kernel<T, false>), grid, dim3(THREADS), 0, st, a, (const T*)g, (T*)dW);
-    if (L.chunks > 1) hipLaunchKernelGGL((embed_join_kernel<T, false>), joins, dim3(JOIN_THREADS), 0, st, a, (T*)dW);
+  a.join_from = 0;
+  const dim3 grid((unsigned)blocks, (unsigned)cols);
+  const bool whole = E >= pmg_vec16<T>::N;
+  if (whole) hipLaunchKernelGGL((embed_reduce_kernel<T, true>), grid, dim3(THREADS), 0, st, a, (const T*)g, (T*)dW);
+  else hipLaunchKernelGGL((embed_reduce_kernel<T, false>), grid, dim3(THREADS), 0, st, a, (const T*)g, (T*)dW);
+  constexpr int64_t MOST = 1 << 23;  // workgroups a launch: it has fewer than 2^32 threads (chunks of 8 from 2^27 positions on)
+  for (a.join_from = 0; L.chunks > 1 && a.join_from < L.chunks; a.join_from += MOST) {
+    const dim3 joins((unsigned)(L.chunks - a.join_from < MOST ? L.chunks - a.join_from : MOST), (unsigned)cols);
+    if (whole) hipLaunchKernelGGL((embed_join_kernel<T, true>), joins, dim3(JOIN_THREADS), 0, st, a, (T*)dW);
+    else hipLaunchKernelGGL((embed_join_kernel<T, false>), joins, dim3(JOIN_THREADS), 0, st, a, (T*)dW);
   }
   return (int)hipGetLastError();
 }

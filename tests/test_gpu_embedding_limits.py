@@ -25,3 +25,18 @@ def test_padding_counted_from_either_end(gpu, V):
     for pad in (V, -V - 1):
         with pytest.raises(_ffi.PmgError, match='padding_idx'):
             ops.embedding(w, ids, padding_idx=pad)
+
+
+@pytest.mark.parametrize('dtype,E', [(torch.float32, 3), (torch.bfloat16, 8)], ids=str)
+def test_more_positions_than_one_joining_launch_takes(gpu, dtype, E):
+    """Narrow rows in chunks of 8 positions, more than 2^24 of them.  Every position adds small whole numbers, so that all
+    partial sums are exact: a token's gradient is its number of positions times its row."""
+    N, V = (1 << 27) + 12345, 60001
+    ids = torch.randint(0, V - 1, (N,), device='cuda', dtype=torch.int32, generator=torch.Generator(device='cuda').manual_seed(1))
+    ids[-3000000:] = V - 1                     # a run over very many chunks, most of them of the last launch
+    row = torch.tensor([1.0, -2.0, 3.0, 0.0, 4.0, -1.0, 2.0, 5.0][:E], device='cuda', dtype=dtype)
+    got = torch.ops.pmg.embedding_bwd(row.repeat(N, 1), ids, V, 1.0, -1)
+    count = torch.bincount(ids, minlength=V)
+    want = count.double().unsqueeze(1) * row.double()
+    assert int(count.max()) * 5 < 1 << 24      # whole numbers that fp32 holds
+    assert torch.equal(got, want.to(dtype))

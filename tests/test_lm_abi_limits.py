@@ -53,3 +53,10 @@ def test_cross_entropy_scratch_does_not_grow_with_tokens_times_words():
                 many = [k for k, V in enumerate(words[:-1]) if V >= 1 << 17 and N >= 65536 and 128 * 2 * V < 256 * MB]
                 for k in many:          # twice the words, no more scratch
                     assert f[k + 1] <= f[k] * 1.01 + MB and b[k + 1] <= b[k] * 1.15 + MB, (N, words[k], H)
+
+
+def test_embedding_gradient_refuses_what_a_launch_cannot_cover():
+    from paccmann_generator_amd import _ffi
+    call = lambda N, V, E: _ffi.lib.pmg_embedding_bwd(FAKE, E, FAKE, 32, N, V, E, 1, 1.0, -1, FAKE, FAKE, None)     # noqa: E731
+    for N, V, E in ((4, 1 << 30, 2), (1 << 30, (1 << 30) + 5, 1), (0, 0x7ffffffe, 1)):
+        assert call(N, V, E) == -9, (N, V, E)
