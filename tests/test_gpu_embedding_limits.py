@@ -31,6 +31,7 @@ def test_padding_counted_from_either_end(gpu, V):
 def test_more_positions_than_one_joining_launch_takes(gpu, dtype, E):
     """Narrow rows in chunks of 8 positions, more than 2^24 of them.  Every position adds small whole numbers, so that all
     partial sums are exact: a token's gradient is its number of positions times its row."""
+    import paccmann_generator_amd  # noqa: F401  (registers the operators)
     N, V = (1 << 27) + 12345, 60001
     ids = torch.randint(0, V - 1, (N,), device='cuda', dtype=torch.int32, generator=torch.Generator(device='cuda').manual_seed(1))
     ids[-3000000:] = V - 1                     # a run over very many chunks, most of them of the last launch
