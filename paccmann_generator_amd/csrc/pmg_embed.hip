@@ -24,6 +24,8 @@ constexpr int MAX_BINS = 1 << MAX_BITS;
 constexpr int FILL_ROWS = 64;   // table rows a workgroup checks and zeroes
 constexpr int JOIN_THREADS = 256;
 constexpr int HELD = 2048;      // sorted keys and positions that a workgroup of the reduction holds in LDS
+// Workgroups a launch: of 2^32 threads or more in a dimension only some run, without an error.
+constexpr int64_t MOST_GROUPS = 1 << 23;
 
 // ids outside [0, V) and the padding id sort behind all tokens and take no part
 template <typename I> __device__ __forceinline__ uint32_t key_of(I id, int64_t V, int64_t pad) {
@@ -487,11 +489,15 @@ int fwd(const void* W, int64_t ldw, const void* ids, int64_t N, int64_t V, int64
   if (cols > 65535) return PMG_E_ARG;
   // four rows a thread once that leaves enough workgroups for the chip
   const int rows = (N / rpw) * cols >= 4 * 1024 ? 4 : 1;
-  const dim3 grid((unsigned)((N + (int64_t)rpw * rows - 1) / ((int64_t)rpw * rows)), (unsigned)cols);
-  if (rows == 4)
-    hipLaunchKernelGGL((embed_fwd_kernel<T, I, 4>), grid, dim3(THREADS), 0, st, (const T*)W, ldw, (const I*)ids, N, V, E, scale, tpr, (T*)out);
-  else
-    hipLaunchKernelGGL((embed_fwd_kernel<T, I, 1>), grid, dim3(THREADS), 0, st, (const T*)W, ldw, (const I*)ids, N, V, E, scale, tpr, (T*)out);
+  const int64_t most = MOST_GROUPS * rpw * rows;
+  for (int64_t n0 = 0; n0 < N; n0 += most) {
+    const int64_t n = N - n0 < most ? N - n0 : most;
+    const dim3 grid((unsigned)((n + (int64_t)rpw * rows - 1) / ((int64_t)rpw * rows)), (unsigned)cols);
+    const I* id = (const I*)ids + n0;
+    T* to = (T*)out + n0 * E;
+    if (rows == 4) hipLaunchKernelGGL((embed_fwd_kernel<T, I, 4>), grid, dim3(THREADS), 0, st, (const T*)W, ldw, id, n, V, E, scale, tpr, to);
+    else hipLaunchKernelGGL((embed_fwd_kernel<T, I, 1>), grid, dim3(THREADS), 0, st, (const T*)W, ldw, id, n, V, E, scale, tpr, to);
+  }
   return (int)hipGetLastError();
 }
 
@@ -553,9 +559,8 @@ int bwd(const void* g, int64_t ldg, const void* ids, int id_bits, int64_t N, int
   const bool whole = E >= pmg_vec16<T>::N;
   if (whole) hipLaunchKernelGGL((embed_reduce_kernel<T, true>), grid, dim3(THREADS), 0, st, a, (const T*)g, (T*)dW);
   else hipLaunchKernelGGL((embed_reduce_kernel<T, false>), grid, dim3(THREADS), 0, st, a, (const T*)g, (T*)dW);
-  constexpr int64_t MOST = 1 << 23;  // workgroups a launch: it has fewer than 2^32 threads (chunks of 8 from 2^27 positions on)
-  for (a.join_from = 0; L.chunks > 1 && a.join_from < L.chunks; a.join_from += MOST) {
-    const dim3 joins((unsigned)(L.chunks - a.join_from < MOST ? L.chunks - a.join_from : MOST), (unsigned)cols);
+  for (a.join_from = 0; L.chunks > 1 && a.join_from < L.chunks; a.join_from += MOST_GROUPS) {
+    const dim3 joins((unsigned)(L.chunks - a.join_from < MOST_GROUPS ? L.chunks - a.join_from : MOST_GROUPS), (unsigned)cols);
     if (whole) hipLaunchKernelGGL((embed_join_kernel<T, true>), joins, dim3(JOIN_THREADS), 0, st, a, (T*)dW);
     else hipLaunchKernelGGL((embed_join_kernel<T, false>), joins, dim3(JOIN_THREADS), 0, st, a, (T*)dW);
   }

@@ -41,3 +41,18 @@ def test_more_positions_than_one_joining_launch_takes(gpu, dtype, E):
     want = count.double().unsqueeze(1) * row.double()
     assert int(count.max()) * 5 < 1 << 24      # whole numbers that fp32 holds
     assert torch.equal(got, want.to(dtype))
+
+
+def test_more_rows_than_one_lookup_launch_takes(gpu):
+    """138 GB of rows: every one of them is looked up."""
+    from paccmann_generator_amd import ops
+    N, V, E = (1 << 28) + 1001, 1000, 257
+    if torch.cuda.mem_get_info()[0] < N * (E * 2 + 4) + (16 << 30):
+        pytest.skip('needs 160 GB of free memory')
+    table = torch.randn(V, E, device='cuda').bfloat16()
+    ids = torch.randint(0, V, (N,), device='cuda', dtype=torch.int32)
+    out = ops.embedding(table, ids, trusted_tokens=True)
+    wrong = sum(int((out[n:n + (1 << 23)] != table[ids[n:n + (1 << 23)]]).any()) for n in range(0, N, 1 << 23))
+    del out
+    torch.cuda.empty_cache()
+    assert wrong == 0
