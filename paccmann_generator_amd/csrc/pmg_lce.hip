@@ -833,6 +833,11 @@ constexpr int CUS = 256;
 
 int64_t tiles_of(int s, int64_t M, int64_t N) { return div_up(M, SHAPES[s].BM) * div_up(N, SHAPES[s].BN); }
 
+// Whether one launch covers the tiles and `more` workgroups: of 2^32 threads or more only some run, without an error.
+bool covers(int s, int64_t M, int64_t N, int64_t more = 0) {
+  return (tiles_of(s, M, N) + more) * SHAPES[s].WM * SHAPES[s].WN * 64 < (int64_t)1 << 32;
+}
+
 // Parts of a long sum where there are too few tiles for the chip; at least eight stages a part.
 int splits_of(int s, int64_t M, int64_t N, int64_t K, int64_t eb) {
   const int64_t tiles = tiles_of(s, M, N), slots = (int64_t)CUS * SHAPES[s].per_cu;
@@ -1045,7 +1050,6 @@ template <typename T, int S, int WAY> int launch_logits(const LogitArgs& a, hipS
 template <typename T, int WAY> int logits(int s, LogitArgs a, hipStream_t st) {
   a.tiles_m = (int)div_up(a.V, SHAPES[s].BM);
   a.tiles_n = (int)div_up(a.N, SHAPES[s].BN);
-  if ((int64_t)a.tiles_m * a.tiles_n > 0x7fffffff) return PMG_E_ARG;
   if constexpr (WAY != SPLIT) {
     if (s == SM64) return launch_logits<T, SM64, WAY>(a, st);
     if constexpr (WAY != KEPT)
@@ -1069,7 +1073,6 @@ template <typename T, int S, bool BKC> int launch_grad(const GradArgs& a, hipStr
   static std::atomic<unsigned long long> done{0};
   if (const hipError_t e = pmg_full_lds_once((const void*)&lce_grad_kernel<T, S, BKC>, &done)) return (int)e;
   const int64_t blocks = (int64_t)a.tiles_m * a.tiles_n + (BKC && a.zeroed ? div_up(a.N, 64) : 0);
-  if (blocks > 0x7fffffff) return PMG_E_ARG;
   hipLaunchKernelGGL((lce_grad_kernel<T, S, BKC>), dim3((unsigned)blocks, a.splits), dim3(THREADS_OF<S>),
                      (TileOf<T, S, false, BKC, !BKC, false>::LDS), st, a);
   return (int)hipGetLastError();
@@ -1079,7 +1082,6 @@ template <typename T, int S, bool BKC> int launch_grad(const GradArgs& a, hipStr
 template <typename T, bool BKC> int grad(int s, GradArgs a, hipStream_t st) {
   a.tiles_m = (int)div_up(a.M, SHAPES[s].BM);
   a.tiles_n = (int)div_up(a.N, SHAPES[s].BN);
-  if ((int64_t)a.tiles_m * a.tiles_n > 0x7fffffff) return PMG_E_ARG;
   void* out = a.out;
   if (a.splits > 1) a.out = nullptr;
   int rc = PMG_E_ARG;
@@ -1268,12 +1270,24 @@ template <typename T> int backward(const pmg_linear_ce* a, const Problem& p, cha
   return (int)hipGetLastError();
 }
 
+// What no launch covers (half a billion words or tokens) is refused before the first one.
+int forward_fits(const Problem& p) {
+  const FwdPlan f = fwd_plan(p);
+  return covers(f.s, p.V, f.block) ? PMG_OK : PMG_E_ARG;
+}
+int backward_fits(const Problem& p) {
+  const BwdPlan b = bwd_plan(p);
+  const bool ok = covers(b.s_dl, b.piece, p.N) && (p.V <= NARROW || covers(b.s_dx, p.H, p.N, div_up(p.N, 64))) && covers(b.s_dw, p.H, b.piece);
+  return ok ? PMG_OK : PMG_E_ARG;
+}
+
 }  // namespace
 
 extern "C" int pmg_linear_ce_workspace(const pmg_linear_ce* a, int backward, size_t* out) {
   if (!a || !out) return PMG_E_NULL;
   Problem p;
   if (const int rc = problem_of(a, &p)) return rc;
+  if (const int rc = backward ? backward_fits(p) : forward_fits(p)) return rc;
   *out = backward ? bwd_layout(p, bwd_plan(p)).bytes : fwd_layout(p).bytes;
   return PMG_OK;
 }
@@ -1283,6 +1297,7 @@ extern "C" int pmg_linear_ce_fwd(const pmg_linear_ce* a, void* ws, pmg_stream st
   if (a->reduction != PMG_REDUCE_NONE && !a->count) return PMG_E_NULL;
   Problem p;
   if (const int rc = problem_of(a, &p)) return rc;
+  if (const int rc = forward_fits(p)) return rc;
   if (((uintptr_t)ws & 15) || (((uintptr_t)a->loss | (uintptr_t)a->lse | (uintptr_t)a->count) & 3)) return PMG_E_ALIGN;
   hipStream_t st = (hipStream_t)stream;
   return a->dtype == PMG_F32 ? forward<float>(a, p, (char*)ws, st) : forward<bf16_t>(a, p, (char*)ws, st);
@@ -1294,6 +1309,7 @@ extern "C" int pmg_linear_ce_bwd(const pmg_linear_ce* a, void* ws, pmg_stream st
   if (a->grad_bias && !a->bias) return PMG_E_NULL;
   Problem p;
   if (const int rc = problem_of(a, &p)) return rc;
+  if (const int rc = backward_fits(p)) return rc;
   if (((uintptr_t)ws & 15) || (((uintptr_t)a->grad_loss | (uintptr_t)a->grad_lse | (uintptr_t)a->lse | (uintptr_t)a->count) & 3))
     return PMG_E_ALIGN;
   if (((uintptr_t)a->grad_hidden | (uintptr_t)a->grad_weight | (uintptr_t)a->grad_bias) & (p.eb - 1)) return PMG_E_ALIGN;

@@ -12,6 +12,8 @@
 namespace {
 
 constexpr int THREADS = 256;
+// Workgroups a launch: of 2^32 threads or more only some run, without an error.
+constexpr int64_t MOST_GROUPS = (((int64_t)1 << 32) - 1) / THREADS;
 
 // The tensor that owns chunk `c`: first[0] = 0, first[k] <= c < first[k+1].  Uniform: scalar loads.
 template <typename Table> __device__ __forceinline__ int owner(const Table& t, int c) {
@@ -423,7 +425,7 @@ extern "C" int pmg_grad_norm_workspace(const int64_t* numel, int n, size_t* out)
     if (numel[i] < 0 || numel[i] > ((int64_t)1 << 40)) return PMG_E_ARG;
     chunks += (size_t)((numel[i] + chunk - 1) / chunk);
   }
-  if (chunks > (size_t)0x7fffffff) return PMG_E_ARG;
+  if (chunks > (size_t)MOST_GROUPS) return PMG_E_ARG;
   *out = chunks * sizeof(double);
   return PMG_OK;
 }
@@ -518,7 +520,7 @@ extern "C" int pmg_adamw_step(const pmg_adamw* a, void* ws, pmg_stream stream) {
     if (a->master) bad |= (uintptr_t)a->master[i] & 3;
     if (bad) return PMG_E_ALIGN;
   }
-  if (chunks_all > 0x7fffffff) return PMG_E_ARG;
+  if (chunks_all > MOST_GROUPS) return PMG_E_ARG;
   Range* r = new (std::nothrow) Range[(size_t)a->n * 7 + 4];
   if (!r) return PMG_E_ARG;
   int nr = 0;
@@ -575,7 +577,7 @@ extern "C" int pmg_adamw_step(const pmg_adamw* a, void* ws, pmg_stream stream) {
 
 extern "C" int pmg_adamw_values(const void* code, const float* top, int64_t numel, int is_signed, float* out,
                                 pmg_stream stream) {
-  if (numel < 0 || numel > ((int64_t)1 << 40)) return PMG_E_ARG;
+  if (numel < 0 || numel > MOST_GROUPS * AW_CHUNK) return PMG_E_ARG;
   if (numel == 0) return PMG_OK;
   if (!code || !top || !out) return PMG_E_NULL;
   if (((uintptr_t)top | (uintptr_t)out) & 3) return PMG_E_ALIGN;

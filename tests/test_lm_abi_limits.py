@@ -60,3 +60,33 @@ def test_embedding_gradient_refuses_what_a_launch_cannot_cover():
     call = lambda N, V, E: _ffi.lib.pmg_embedding_bwd(FAKE, E, FAKE, 32, N, V, E, 1, 1.0, -1, FAKE, FAKE, None)     # noqa: E731
     for N, V, E in ((4, 1 << 30, 2), (1 << 30, (1 << 30) + 5, 1), (0, 0x7ffffffe, 1)):
         assert call(N, V, E) == -9, (N, V, E)
+
+
+def test_what_no_launch_covers_is_refused():
+    """2^32 threads or more in a launch: half a billion words beside a thousand tokens, or tokens beside a hundred words."""
+    from paccmann_generator_amd import _ffi
+    lib, size = _ffi.lib, C.c_size_t(0)
+
+    def args(N, V, H, dtype=1):
+        a = _ffi.PmgLinearCe()
+        for name, x in dict(N=N, V=V, H=H, dtype=dtype, id_bits=64, reduction=2, logit_scale=1.0, ld_hidden=H, ld_weight=H,
+                            hidden=FAKE, weight=FAKE, targets=FAKE, loss=FAKE, lse=FAKE, count=FAKE, grad_loss=FAKE,
+                            grad_hidden=FAKE).items():
+            setattr(a, name, x)
+        return C.byref(a)
+
+    for N, V, H, forward, backward in ((1024, 1 << 30, 16, False, True), (0x7fffff00, 100, 16, True, False),
+                                       (1 << 29, 128, 16, True, False), (1 << 28, 128, 16, True, True),
+                                       (1, 1 << 28, 16, True, True), (4 << 20, 128000, 4096, True, True),
+                                       (1 << 30, 60, 16, True, True), (1 << 20, 1 << 20, 64, True, True)):
+        for way, ok in ((0, forward), (1, backward)):
+            rc = lib.pmg_linear_ce_workspace(args(N, V, H), way, C.byref(size))
+            assert rc == (0 if ok else -9), (N, V, H, way)
+        if not forward:
+            assert lib.pmg_linear_ce_fwd(args(N, V, H), FAKE, None) == -9
+        if not backward:
+            assert lib.pmg_linear_ce_bwd(args(N, V, H), FAKE, None) == -9
+    numel = (C.c_int64 * 1)((1 << 38) + 1)
+    assert lib.pmg_grad_norm_workspace(numel, 1, C.byref(size)) == -9
+    assert lib.pmg_grad_clip_check((C.c_void_p * 1)(FAKE), numel, (C.c_int * 1)(1), 1, 1.0) == -9
+    assert lib.pmg_adamw_values(FAKE, FAKE, 1 << 37, 1, FAKE, None) == -9
