@@ -156,3 +156,40 @@ def test_losses_of_any_weight_beside_the_log_sum_exp(gpu, dtype, weight):
             exact, mag = grads[name], grads['|' + name + '|']
             bound = mag * (rel + (length + 8) * U) + exact.abs() * f.eps / 2 * 1.01
             assert bool(((g.cpu().double() - exact).abs() <= bound + 1e-30).all()), (name, reduction)
+
+
+@pytest.mark.parametrize('dtype', TYPES, ids=str)
+def test_kept_logits_over_pieces_of_the_vocabulary(gpu, dtype):
+    """Gradients from kept logits and from logits formed again, three pieces of the vocabulary, against 64 bits: every
+    element within its own sum of magnitudes.  Hidden states and rewards are positive and targets are a few words, so that
+    the sums of the others do not cancel: a gradient of zeros, or one with its pieces in another order, is far outside."""
+    import paccmann_generator_amd  # noqa: F401  (registers the operators)
+    N, V, H = 524288, 603, 16
+    x, w, b, _ = _data(N, V, H, dtype, seed=7)
+    x = x.abs()
+    g = torch.Generator().manual_seed(8)
+    t, r = torch.randint(0, 37, (N,), generator=g) * 16 + 5, torch.rand(N, generator=g) + 0.1
+    t[torch.rand(N, generator=g) < 0.4] = -100
+    x, w, b, t, r = (v.cuda() for v in (x, w, b, t, r))
+    call = (x, w, b, t, r, -100, 0.8, 1)
+    loss, lse, count, logits = torch.ops.pmg.linear_cross_entropy_keep(*call, True)
+    runs = [torch.ops.pmg.linear_cross_entropy_bwd(torch.ones_like(loss), None, *call[:5], lse, count, *call[5:], [True] * 3, k)
+            for k in (logits, None)]
+    size = lm.linear_ce(x, w, t, b, r, 0.8, 'sum')['size']
+    grads = lm.linear_ce_grads(x, w, t, b, r, 0.8, 'sum', -100, torch.tensor(1.0).cuda(), None)
+    f = torch.finfo(dtype)
+    rel = 4 * ((H + 16) * U * float(size.max()) + 8 * U) + 16 * U + (0 if dtype == torch.float32 else f.eps / 2)
+    for k, (name, length) in enumerate((('x', V), ('w', N), ('b', N))):
+        exact, mag = grads[name], grads['|' + name + '|']
+        bound = mag * (rel + (length + 8) * U) + exact.abs() * f.eps / 2 * 1.01
+        for got in runs:
+            assert bool(((got[k].double() - exact).abs() <= bound).all()), name
+        if name == 'x':          # rows without a slope are zeros; in the others nearly all elements stand out
+            assert float((exact.abs() > bound)[t != -100].double().mean()) > 0.9
+        else:
+            stands, targets = exact.abs() > 2 * bound, torch.unique(t[t != -100])
+            assert float(stands.double().mean()) > 0.95, name
+            stands[targets] = True
+            assert bool(stands.all()), name
+            turned = exact.roll(256, 0)
+            assert float(((turned - exact).abs() > 2 * bound).double().mean()) > 0.5, name
