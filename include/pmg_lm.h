@@ -59,7 +59,7 @@ int pmg_embedding_bwd(const void* grad, int64_t ld_grad, const void* ids, int id
  * gradients of hidden, weight and bias (each NULL: not formed).  row_weight has no gradient.  A row without
  * a slope (ignored, of weight 0) has a zero gradient and adds nothing to the others, whatever it holds.
  * A target outside [0,V) that is not ignore_index gives NaN (memory safety; validate on the host).
- * dtype PMG_F32 or PMG_BF16; the slopes of the logits are rounded to it once, all sums are fp32. */
+ * dtype PMG_F32 or PMG_BF16; the slopes of the logits are rounded to it once, all sums are fp32.  H up to 65536. */
 typedef struct pmg_linear_ce {
   int64_t N, V, H;
   int dtype;               /* of hidden, weight, bias and their gradients */

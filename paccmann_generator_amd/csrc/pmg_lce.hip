@@ -10,8 +10,9 @@
 // vocabulary tile the largest logit and the sum of exponentials below it, and the target's logit: 8 bytes
 // for 256 logits.  A second kernel joins them.  Few tokens (serving) take narrow tiles: W is streamed once.
 // Backward: the vocabulary goes in pieces; of each piece the logits are formed again, dl is written in the
-// operands' type (bf16: one rounding, relative 2^-9 at most, like the operands themselves; without f, so
-// that the targets' -1 and the zeros stay exact and the roundings of the rows are not all the same; the products sum
+// operands' type (bf16: one rounding, relative 2^-8 at most, like the operands themselves; without f, so
+// that the targets' -1 and the zeros stay exact and the roundings of the rows are not all the same; weights and slopes
+// of single rows stay in, because dx and dW read the same dl, and a target's -c_n is then rounded too; the products sum
 // in fp32) and read by the two products for dx and dW.  dx is summed over the pieces in fp32.  Long sums with
 // few result tiles are split and joined in a fixed order.  No atomics: equal inputs give equal bits.
 // Rows without a slope (ignored targets, zero weights) take no part in the backward: the others are listed, the
@@ -958,7 +959,8 @@ FwdPlan fwd_plan(const Problem& p) {
   f.rows = f.splits > 1 ? (p.V <= 256 ? 16 : p.V <= 1024 ? 4 : 1) : rows_of(p.N, div_up(p.V, SHAPES[f.s].BM));
   f.groups = div_up(p.N, f.rows);
   f.block = p.N;
-  const int64_t fit = PART_BYTES / ((int64_t)sizeof(float2) * div_up(p.V, SHAPES[f.s].BM)), most_tokens = fit < 1024 ? 1024 : fit / 1024 * 1024;
+  const int64_t fit = PART_BYTES / ((int64_t)sizeof(float2) * div_up(p.V, SHAPES[f.s].BM));
+  const int64_t most_tokens = fit < 1024 ? 1024 : fit / 1024 * 1024;
   if (f.splits == 1 && p.N > most_tokens) f.block = up(div_up(p.N, div_up(p.N, most_tokens)), 1024);
   return f;
 }
@@ -1277,8 +1279,8 @@ int forward_fits(const Problem& p) {
 }
 int backward_fits(const Problem& p) {
   const BwdPlan b = bwd_plan(p);
-  const bool ok = covers(b.s_dl, b.piece, p.N) && (p.V <= NARROW || covers(b.s_dx, p.H, p.N, div_up(p.N, 64))) && covers(b.s_dw, p.H, b.piece);
-  return ok ? PMG_OK : PMG_E_ARG;
+  const bool dx = p.V <= NARROW || covers(b.s_dx, p.H, p.N, div_up(p.N, 64));
+  return covers(b.s_dl, b.piece, p.N) && dx && covers(b.s_dw, p.H, b.piece) ? PMG_OK : PMG_E_ARG;
 }
 
 }  // namespace

@@ -1,7 +1,7 @@
 // PyTorch operators of the namespace `pmg` over include/pmg_lm.h: schemas, argument checks, autograd.
 //
-// In C++ because the calls are short: an update of the decoder's 15 tensors is about 20 us on the device, and
-// from Python the checks and pointer lists of four times 15 tensors take longer than that; a backward in
+// In C++ because the calls are short: an update of the decoder's 13 tensors is about 20 us on the device, and
+// from Python the checks and pointer lists of four times 13 tensors take longer than that; a backward in
 // Python also runs on autograd's own thread, which has to be handed the interpreter first (about 100 us a
 // call).  Every message begins with "pmg" (lm_ops.py turns such errors into PmgError).
 #include <ATen/ATen.h>
