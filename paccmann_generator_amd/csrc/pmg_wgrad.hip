@@ -176,7 +176,12 @@ __global__ __launch_bounds__(WG_THREADS, 2) void pmg_wgrad_kernel(const WgradArg
     WG_LOAD_A(fa0, 0)
     load_b(0, fb0);
 #pragma unroll 1
-    for (int k = 0; k < ns; k += 2) {
+    for (int k = 0; k < ns; k += 2) {  // (ns is the workgroup's)
+      // The four waves read each panel twice, and 64 workgroups of an XCD share them through its L2 while they are at the
+      // same slabs.  The barrier keeps a workgroup's waves together, which also holds the workgroups closer: at 4096 sequences
+      // of hidden 1024 x 2 layers, 256 steps, half of the L2 misses (275 GB counted, 574 without) and 157 ms, 184 without; at
+      // 8192 of hidden 512, 128 steps, 16.6 and 17.6 ms; at 4096 of those 8.2 and 8.35.  One a slab, or one every 16 slabs, is slower.
+      __builtin_amdgcn_s_barrier();
       const int k1 = (k + 1 < ns) ? k + 1 : k;
       WG_LOAD_A(fa1, k1)
       load_b(k1, fb1);
