@@ -136,12 +136,17 @@ def presampled_tokens(n, T, V, device, seed=5):
     return toks.to(device)
 
 
+# what the kernels of a step are built from (the training operators beside them have sources of their own)
+STEP_SOURCES = ('pmg_api.hip', 'pmg_bwd.hip', 'pmg_bwdc.hip', 'pmg_common.h', 'pmg_fwd.hip', 'pmg_fwdc.hip', 'pmg_kernels.h',
+                'pmg_pack.hip', 'pmg_wgrad.hip')
+
+
 def kernel_source_hash():
-    """sha256 over the HIP sources and headers the library is built from."""
+    """sha256 over the sources and headers that the kernels of a step are built from."""
     import hashlib
     h = hashlib.sha256()
     csrc = os.path.join(ROOT, 'paccmann_generator_amd', 'csrc')
-    for path in sorted(os.path.join(csrc, f) for f in os.listdir(csrc)) + [os.path.join(ROOT, 'include', 'pmg.h')]:
+    for path in [os.path.join(csrc, f) for f in STEP_SOURCES] + [os.path.join(ROOT, 'include', 'pmg.h')]:
         with open(path, 'rb') as f:
             h.update(os.path.basename(path).encode() + b'\0' + f.read())
     return h.hexdigest()
